@@ -23,6 +23,7 @@ Differences from the reference, all additive:
 
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass, replace
 
 import numpy as np
@@ -55,6 +56,18 @@ def _stream(t: torch.Tensor) -> int:
     if _RAW_STREAM is not None and t.device.index is not None:
         return _RAW_STREAM(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is torch's current CUDA device, which is
+    the one that a launch through the C ABI goes to (nothing to do, and nothing
+    paid, where it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _require_cuda(t: torch.Tensor, what: str) -> None:
