@@ -373,8 +373,12 @@ bpd_status bpd_pda_step_greedy_from_n(
  * rank has zero rows in a and zero columns in b. The entries of b must be
  * finite. in_features is a multiple of 8; x, weight, their rows, a, b and
  * workspace (bpd_lora_workspace_bytes, any contents) start on 16-byte
- * boundaries. In fp16 the inner sums (times scale) must stay below 65504. */
+ * boundaries. In fp16 the inner sums (times scale) must stay below 65504.
+ * bpd_lora_take_error waits for the device and tells whether a projection on
+ * the current device gave up waiting for its own loads since the last call
+ * (its result is then not complete); 0 unless the device misbehaves. */
 size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank);
+bpd_status bpd_lora_take_error(int32_t* error_out);
 bpd_status bpd_lora_project(
     const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
     int32_t dtype, int32_t rows, int32_t in_features, int32_t out_features,
