@@ -166,7 +166,7 @@ def project(
         ids64 = int(ids.dtype == torch.int64)
         a, b, scale = bank._a.data_ptr(), bank._b.data_ptr(), bank._scale.data_ptr()
         n, rank = bank.max_adapters, bank.rank_pad
-        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank), dtype=torch.uint8,
+        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank, n), dtype=torch.uint8,
                            device=x.device)
         ws_ptr = work.data_ptr()
     with on_device(x.device):

@@ -13,9 +13,9 @@
 // which is read once; the adapters' steps then cost what reading B_a costs.
 //
 // S goes into those steps in blocks of 16 rows, the smallest N of the matrix
-// unit at M = 128: a (block, adapter) pair exists only where one of the
-// block's rows has that adapter, so there are at most as many pairs as rows,
-// whatever their order. Rows need not be sorted.
+// unit at M = 128 (of 64 for prompts): a (block, adapter) pair exists only
+// where one of the block's rows has that adapter, so there are at most as many
+// pairs as rows, whatever their order. Rows need not be sorted.
 //
 // S is held as the sum of two 16-bit values (its rounding, and what that left
 // off): together 2^-17 of it in bf16, 2^-22 in fp16, so an fp32 result keeps
@@ -34,8 +34,8 @@ namespace {
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kTileN = 128;        // outputs of a tile: the M of the matrix instruction
 constexpr int kStepK = 64;         // inner elements of a step: one 128-byte swizzled row
-constexpr int kBlock = 16;         // rows of x of a pair
 constexpr int kRankStep = 64;      // inner elements of an adapter's step, at most
+constexpr int kMaxPairs = 32;      // pairs of an adapters' step, at most
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share one tile's inner elements
 constexpr int kThreads = 192;      // loads, products, four warps that write
 constexpr int kShrinkThreads = 256;
@@ -58,9 +58,10 @@ struct LoraArgs {
   int64_t out_stride;
   // workspace: the pairs of each tile of rows, in the order of their adapters
   int32_t* count;    // [row tiles]
-  uint32_t* pairs;   // [row tiles, tile]: adapter << 4 | block
-  uint8_t* low;      // [row tiles, tile, rank * 64 bytes]: S of a pair's 16 rows
-  int32_t tile;      // rows of a tile
+  uint32_t* pairs;   // [row tiles, most_pairs]: adapter << 4 | block
+  uint8_t* low;      // [row tiles, most_pairs, rank * block * 4 bytes]: S of a pair's rows
+  int32_t tile, block;  // rows of a tile and of a block
+  int32_t most_pairs;   // of a tile
   int32_t row_tiles, out_tiles;
 };
 
@@ -146,11 +147,15 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_float(uint32_t own, uint32_t rank) {
+// 16 bytes of the shared memory of the cluster's CTA `rank`; read behind a
+// cluster barrier and before the next, where nothing writes them.
+__device__ __forceinline__ float4 peer_float4(uint32_t own, uint32_t rank) {
   uint32_t a;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(own), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a));
   return v;
 }
 // 16 columns of this warp's 32 lanes of tensor memory.
@@ -186,12 +191,14 @@ constexpr uint32_t instruction(uint32_t n) {
 }
 
 // ---------------------------------------------------------------------------
-// S. One CTA for each row; the ones that are not the first of their block with
-// their adapter leave at once, the others compute their pair: 16 rows of x by
-// the adapter's A over all inner elements, split over the warps. Bound by
-// reading A once per pair; the products go through mma.sync, whose rate is no
-// limit here. The order of the inner elements within a step is permuted, alike
-// in both operands, so that every load is 16 bytes.
+// S. A few CTAs for each block of rows share the adapters that the block has:
+// BLOCK rows of x by the adapter's A over all inner elements, the warps split
+// over 16-row groups and over the inner elements. Bound by the latency of
+// reading A, and hidden behind the product's reading of W: a CTA is small
+// enough (18 KB of shared memory) to stand beside one of the product's. The
+// products go through mma.sync, whose rate is no limit here. The order of the
+// inner elements within a step is permuted, alike in both operands, so that
+// every load is 16 bytes.
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -211,127 +218,146 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kShrinkThreads) shrink_kernel(const LoraArgs g) {
+// CTAs of a block: as many as it can have adapters, or few where the rows are
+// a prompt's and come in runs.
+template <int BLOCK>
+constexpr int kShrinkCtas = BLOCK == 16 ? 16 : 4;
+
+template <typename T, int BLOCK, int RS>
+__global__ void __launch_bounds__(kShrinkThreads, 2) shrink_kernel(const LoraArgs g) {
   using Bits = typename Dt<T>::Bits;
-  constexpr int kWarps = kShrinkThreads / 32;
+  constexpr int kGroups = BLOCK / 16;                     // 16-row groups of a block
+  constexpr int kParts = kShrinkThreads / 32 / kGroups;   // parts of the inner elements
+  constexpr int kSlots = std::min(kParts, 4096 / (BLOCK * RS));  // parts that are added at once
+  constexpr int kUnroll = RS == 16 ? 4 : RS == 32 ? 3 : 2;
   __shared__ int32_t ids[256];
-  __shared__ float part[kWarps][kBlock][kRankStep];
+  __shared__ uint8_t leads[256];
+  __shared__ float sums[kSlots][BLOCK][RS];
+  const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t turn = blockIdx.x % kShrinkCtas<BLOCK>;
+  const int32_t r0 = blockIdx.x / kShrinkCtas<BLOCK> * BLOCK;  // the block's first row
+  const int32_t tile = r0 / g.tile, t0 = tile * g.tile, b0 = r0 - t0;
   pdl_wait();
   pdl_trigger();  // what ran before has completed: x is there for the next kernel, too
-  const int32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t tile = t / g.tile, t0 = tile * g.tile;
-  const int32_t mine = t - t0, block = mine / kBlock;
   if (tid < g.tile) ids[tid] = adapter_of(g, t0 + tid);
   __syncthreads();
-  // whether row i of the tile is the first of its block with its adapter
-  auto leads = [&](int32_t i) {
-    bool first = ids[i] >= 0;
-    for (int32_t j = i / kBlock * kBlock; j < i; ++j) first = first && ids[j] != ids[i];
-    return first;
-  };
-  const int32_t a = ids[mine];
-  const bool lead = leads(mine);
-  const bool theirs = tid < g.tile && leads(tid);
-  if (mine == 0) {
-    const int32_t total = __syncthreads_count(theirs);
-    if (tid == 0) g.count[tile] = total;
-  }
-  if (!lead) return;  // the same for the whole CTA
-  const int32_t rank_of = __syncthreads_count(
-      theirs && (ids[tid] < a || (ids[tid] == a && tid / kBlock < block)));
-  const int64_t pair = static_cast<int64_t>(tile) * g.tile + rank_of;
-  if (tid == 0)
-    g.pairs[pair] = (static_cast<uint32_t>(a) << 4) | static_cast<uint32_t>(block);
+  // the first row of each adapter in its block
+  bool lead = tid < g.tile && ids[tid] >= 0;
+  if (lead)
+    for (int32_t j = tid / BLOCK * BLOCK; j < tid; ++j) lead = lead && ids[j] != ids[tid];
+  leads[tid] = lead;
+  const int32_t total = __syncthreads_count(lead);
+  if (b0 == 0 && turn == 0 && tid == 0) g.count[tile] = total;
 
-  const int32_t r0 = block * kBlock;
-  const bool in0 = ids[r0 + (lane >> 2)] == a, in1 = ids[r0 + (lane >> 2) + 8] == a;
-  const Bits* x0 = static_cast<const Bits*>(g.x) + (t0 + r0 + (lane >> 2)) * g.x_stride;
+  const int32_t group = warp % kGroups, part = warp / kGroups;
+  const int32_t i0 = b0 + group * 16 + (lane >> 2);  // this lane's two rows in the tile
+  const Bits* x0 = static_cast<const Bits*>(g.x) + static_cast<int64_t>(t0 + i0) * g.x_stride;
   const Bits* x1 = x0 + 8 * g.x_stride;
-  const float scale = g.scale[a];
-  // each warp has a contiguous share of the inner elements, a multiple of 32
-  const int32_t share = ((g.K + 31) / 32 + kWarps - 1) / kWarps * 32;
-  const int32_t k0 = min(g.K, warp * share), k1 = min(g.K, k0 + share);
-  for (int32_t c = 0; c < g.rank; c += kRankStep) {
-    const int32_t rc = min(kRankStep, g.rank - c);
-    const Bits* w = static_cast<const Bits*>(g.a) +
-                    (static_cast<int64_t>(a) * g.rank + c + (lane >> 2)) * g.K;
-    float acc[kRankStep / 8][4] = {};
-#pragma unroll 2
-    for (int32_t k = k0; k < k1; k += 32) {
-      const int32_t at = k + (lane & 3) * 8;
-      const bool in = at < k1;
-      uint4 u = {}, v = {};
-      if (in && in0) u = *reinterpret_cast<const uint4*>(x0 + at);
-      if (in && in1) v = *reinterpret_cast<const uint4*>(x1 + at);
+  // each part is a contiguous share of the inner elements, a multiple of 32
+  const int32_t share = ((g.K + 31) / 32 + kParts - 1) / kParts * 32;
+  const int32_t k0 = min(g.K, part * share), k1 = min(g.K, k0 + share);
+  int32_t seen = 0;
+  for (int32_t i = b0; i < b0 + BLOCK; ++i) {
+    if (!leads[i] || seen++ % kShrinkCtas<BLOCK> != turn) continue;  // alike in all threads
+    const int32_t a = ids[i];
+    const int32_t at_pair = __syncthreads_count(
+        lead && (ids[tid] < a || (ids[tid] == a && tid / BLOCK < b0 / BLOCK)));
+    const int64_t pair = static_cast<int64_t>(tile) * g.most_pairs + at_pair;
+    if (tid == 0)
+      g.pairs[pair] = (static_cast<uint32_t>(a) << 4) | static_cast<uint32_t>(b0 / BLOCK);
+    const bool in0 = ids[i0] == a, in1 = ids[i0 + 8] == a;
+    const float scale = g.scale[a];
+    for (int32_t c = 0; c < g.rank; c += RS) {
+      const int32_t rc = min(RS, g.rank - c);
+      const Bits* w = static_cast<const Bits*>(g.a) +
+                      (static_cast<int64_t>(a) * g.rank + c + (lane >> 2)) * g.K;
+      float acc[RS / 8][4] = {};
+      for (int32_t k = k0; k < k1; k += 32 * kUnroll) {
+        uint4 u[kUnroll], v[kUnroll], q[kUnroll][RS / 8];
 #pragma unroll
-      for (int j = 0; j < kRankStep / 8; ++j) {
-        if (j * 8 < rc) {
-          uint4 q = {};
-          if (in) q = *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(j) * 8 * g.K + at);
-          mma_16816<T>(acc[j], u.x, v.x, u.y, v.y, q.x, q.y);
-          mma_16816<T>(acc[j], u.z, v.z, u.w, v.w, q.z, q.w);
+        for (int s = 0; s < kUnroll; ++s) {
+          const int32_t at = k + s * 32 + (lane & 3) * 8;
+          const bool in = at < k1;
+          u[s] = in && in0 ? *reinterpret_cast<const uint4*>(x0 + at) : uint4{};
+          v[s] = in && in1 ? *reinterpret_cast<const uint4*>(x1 + at) : uint4{};
+#pragma unroll
+          for (int j = 0; j < RS / 8; ++j)
+            q[s][j] = in && j * 8 < rc
+                          ? *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(j) * 8 * g.K + at)
+                          : uint4{};
         }
-      }
-    }
 #pragma unroll
-    for (int j = 0; j < kRankStep / 8; ++j) {
-      if (j * 8 < rc) {
-        const int32_t col = j * 8 + (lane & 3) * 2;
-        part[warp][lane >> 2][col] = acc[j][0];
-        part[warp][lane >> 2][col + 1] = acc[j][1];
-        part[warp][(lane >> 2) + 8][col] = acc[j][2];
-        part[warp][(lane >> 2) + 8][col + 1] = acc[j][3];
-      }
-    }
-    __syncthreads();
-    // the operand's layout: [rank / 8][16 rows][8], first the rounded values, then the rests
-    Bits* low = reinterpret_cast<Bits*>(g.low + pair * g.rank * 64 + c * 64);
-    for (int32_t i = tid; i < kBlock * rc; i += kShrinkThreads) {
-      const int32_t row = (i >> 3) & (kBlock - 1), col = (i >> 7) * 8 + (i & 7);
-      float s = 0.0f;
+        for (int s = 0; s < kUnroll; ++s)
 #pragma unroll
-      for (int p = 0; p < kWarps; ++p) s += part[p][row][col];
-      s = ids[r0 + row] == a ? s * scale : 0.0f;
-      const Bits hi = Dt<T>::from_float_dev(s);
-      low[i] = hi;
-      low[kBlock * rc + i] = Dt<T>::from_float_dev(s - Dt<T>::to_float(hi));
+          for (int j = 0; j < RS / 8; ++j) {
+            mma_16816<T>(acc[j], u[s].x, v[s].x, u[s].y, v[s].y, q[s][j].x, q[s][j].y);
+            mma_16816<T>(acc[j], u[s].z, v[s].z, u[s].w, v[s].w, q[s][j].z, q[s][j].w);
+          }
+      }
+      // the parts meet in a fixed order, kSlots at a time
+      for (int32_t round = 0; round < kParts; round += kSlots) {
+        if (part >= round && part < round + kSlots) {
+          float(*to)[RS] = sums[part - round];
+          const int32_t row = group * 16 + (lane >> 2);
+#pragma unroll
+          for (int j = 0; j < RS / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float& f = to[row + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)];
+              f = round == 0 ? acc[j][e] : f + acc[j][e];
+            }
+        }
+        __syncthreads();
+      }
+      // the operand's layout: [rank / 8][rows][8], first the rounded values, then the rests
+      Bits* low = reinterpret_cast<Bits*>(g.low + (pair * g.rank + c) * (BLOCK * 4));
+      for (int32_t e = tid; e < BLOCK * rc; e += kShrinkThreads) {
+        const int32_t row = (e >> 3) % BLOCK, col = e / (8 * BLOCK) * 8 + (e & 7);
+        float s = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kSlots; ++p) s += sums[p][row][col];
+        s = ids[b0 + row] == a ? s * scale : 0.0f;
+        const Bits hi = Dt<T>::from_float_dev(s);
+        low[e] = hi;
+        low[BLOCK * rc + e] = Dt<T>::from_float_dev(s - Dt<T>::to_float(hi));
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // The product.
 
-template <int NT>
+template <int NT, int BLOCK>
 struct Shape {
   static constexpr int kWeightBytes = kTileN * kStepK * 2;
   // a stage holds a step's rows of x, or the pairs of an adapter's step
-  static constexpr int kRowBytes = std::max(NT * kStepK * 2, kBlock * kRankStep * 4);
+  static constexpr int kRowBytes = std::max(NT * kStepK * 2, BLOCK * kRankStep * 4);
   static constexpr int kStageBytes = kWeightBytes + kRowBytes;
-  static constexpr int kStages = (220 * 1024) / kStageBytes;
+  // leaves room for a CTA of shrink_kernel on the same SM
+  static constexpr int kStages = (200 * 1024) / kStageBytes;
   static constexpr int kColumns = std::max(32, 2 * NT);  // tensor memory: two accumulators
   static constexpr int kBytes = kStages * kStageBytes + 1024;  // with room to align
 };
 
-constexpr int kMaxStages = 11;
+constexpr int kMaxStages = 10;
 constexpr uint32_t kEnd = 0;  // an empty step behind the last adapter of a tile
 
 struct ProjectShared {
   uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
-  uint64_t blocks[kMaxStages];  // the blocks of a stage's pairs, 4 bits each
-  uint32_t shape[kMaxStages];   // of an adapter's step: rank step << 8 | pairs; kEnd
+  uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | pairs; kEnd
+  uint8_t pair[kMaxStages][kMaxPairs];  // its pairs: adapter of the step << 4 | block
   uint32_t tmem;
   uint32_t failed;
   uint32_t list[256];
 };
 
-template <typename T, typename O, int NT>
+template <typename T, typename O, int NT, int BLOCK>
 __global__ void __launch_bounds__(kThreads, 1)
     project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const LoraArgs g, const int32_t split) {
-  using S = Shape<NT>;
+  using S = Shape<NT, BLOCK>;
   extern __shared__ uint8_t dynamic[];
   __shared__ ProjectShared sh;
   const uint32_t ring = (shared_addr(dynamic) + 1023u) & ~1023u;
@@ -404,48 +430,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         waited = true;
       }
       if (listed != rows) {
-        pairs = min(g.count[rows], NT);
+        pairs = min(g.count[rows], g.most_pairs);
         __syncwarp();
         for (int32_t i = lane; i < pairs; i += 32)
-          sh.list[i] = g.pairs[static_cast<int64_t>(rows) * NT + i];
+          sh.list[i] = g.pairs[static_cast<int64_t>(rows) * g.most_pairs + i];
         __syncwarp();
         listed = rows;
       }
       if (lane == 0) {
-        int32_t group = 0;
-        for (int32_t p = 0; p < pairs && ok;) {
-          const uint32_t a = sh.list[p] >> 4;
-          int32_t end = p + 1;
-          while (end < pairs && (sh.list[end] >> 4) == a) ++end;
-          if (group++ % split == part) {
-            for (int32_t c = 0; c < g.rank && ok; c += kRankStep) {
-              const int32_t rc = min(kRankStep, g.rank - c);
-              const int32_t most = min(kBlock, S::kRowBytes / (rc * 64));
-              for (int32_t q = p; q < end; q += most) {
-                const int32_t n = min(most, end - q);
-                if (!(ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) break;
-                const uint32_t bar = shared_addr(&sh.full[stage]),
-                               at = ring + stage * S::kStageBytes;
-                uint64_t blocks = 0;
-                for (int32_t i = 0; i < n; ++i)
-                  blocks |= static_cast<uint64_t>(sh.list[q + i] & 15u) << (4 * i);
-                sh.blocks[stage] = blocks;
-                sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
-                bar_expect(bar, rc * kTileN * 2 + n * rc * 64);
-                load_bulk(at, static_cast<const uint8_t*>(g.b) +
-                                  ((static_cast<int64_t>(a) * g.out_tiles + outs) * g.rank + c) *
-                                      (kTileN * 2),
-                          rc * kTileN * 2, bar);
-                for (int32_t i = 0; i < n; ++i)
-                  load_bulk(at + S::kWeightBytes + i * rc * 64,
-                            g.low + (static_cast<int64_t>(rows) * NT + q + i) * g.rank * 64 +
-                                c * 64,
-                            rc * 64, bar);
-                next();
+        // A step takes as many pairs as fit: the ring is as long as the queue
+        // of loads in front of HBM, so a step costs its share of that queue
+        // however little it carries (one adapter a step: 0.7 us each).
+        const int32_t p0 = pairs * part / split, p1 = pairs * (part + 1) / split;
+        for (int32_t c = 0; c < g.rank && ok; c += kRankStep) {
+          const int32_t rc = min(kRankStep, g.rank - c);
+          const int32_t adapters = kRankStep / rc;
+          const int32_t most = min(kMaxPairs, S::kRowBytes / (rc * BLOCK * 4));
+          for (int32_t p = p0; p < p1;) {
+            if (!(ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) break;
+            const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
+            int32_t n = 0, met = 0;
+            uint32_t last = 0;
+            for (; n < most && p + n < p1; ++n) {
+              const uint32_t pair = sh.list[p + n], a = pair >> 4;
+              if (met == 0 || a != last) {
+                if (met == adapters) break;
+                ++met;
+                last = a;
               }
+              sh.pair[stage][n] = static_cast<uint8_t>((met - 1) << 4 | (pair & 15u));
             }
+            sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
+            bar_expect(bar, met * rc * kTileN * 2 + n * rc * BLOCK * 4);
+            for (int32_t i = 0, m = -1; i < n; ++i) {
+              const uint32_t a = sh.list[p + i] >> 4;
+              if (i == 0 || a != last) {
+                last = a;
+                load_bulk(at + ++m * rc * kTileN * 2,
+                          static_cast<const uint8_t*>(g.b) +
+                              ((static_cast<int64_t>(a) * g.out_tiles + outs) * g.rank + c) *
+                                  (kTileN * 2),
+                          rc * kTileN * 2, bar);
+              }
+              // pairs that follow one another in memory, too, where rank is one step
+              if (rc != g.rank)
+                load_bulk(at + S::kWeightBytes + i * rc * BLOCK * 4,
+                          g.low + ((static_cast<int64_t>(rows) * g.most_pairs + p + i) * g.rank + c) *
+                                      (BLOCK * 4),
+                          rc * BLOCK * 4, bar);
+            }
+            if (rc == g.rank)
+              load_bulk(at + S::kWeightBytes,
+                        g.low + (static_cast<int64_t>(rows) * g.most_pairs + p) * g.rank *
+                                    (BLOCK * 4),
+                        n * rc * BLOCK * 4, bar);
+            next();
+            p += n;
           }
-          p = end;
         }
         if (ok && (ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) {
           sh.shape[stage] = kEnd;
@@ -501,15 +542,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             const int32_t rc = shape >> 8, n = shape & 255;
-            uint64_t blocks = sh.blocks[stage];
-            for (int32_t i = 0; i < n; ++i, blocks >>= 4) {
-              const uint32_t to = d + static_cast<uint32_t>(blocks & 15u) * kBlock;
-              const uint32_t from = at + S::kWeightBytes + i * rc * 64;
+            for (int32_t i = 0; i < n; ++i) {
+              const uint32_t pair = sh.pair[stage][i];
+              const uint32_t to = d + (pair & 15u) * BLOCK;
+              const uint32_t b = at + (pair >> 4) * rc * kTileN * 2;
+              const uint32_t low = at + S::kWeightBytes + i * rc * BLOCK * 4;
               for (int32_t half = 0; half < 2; ++half)
                 for (int32_t k = 0; k < rc; k += 16)
-                  mma(to, desc_plain(at + k * kTileN * 2, kTileN * 16),
-                      desc_plain(from + half * rc * 32 + k * 32, kBlock * 16),
-                      instruction<T>(kBlock), true);
+                  mma(to, desc_plain(b + k * kTileN * 2, kTileN * 16),
+                      desc_plain(low + half * rc * BLOCK * 2 + k * BLOCK * 2, BLOCK * 16),
+                      instruction<T>(BLOCK), true);
             }
             finish();
           }
@@ -572,18 +614,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   if (split > 1) {
     cluster_sync();
-    if (warp >= 2) {
-      // this CTA's share of the tile's rows, summed over the cluster in its order
-      const int32_t rows = first % g.row_tiles, outs = first / g.row_tiles;
-      const int32_t local = (warp & 3) * 32 + lane, n = outs * kTileN + local;
-      const int32_t have = min(NT, g.T - rows * NT);
-      using OBits = typename Dt<O>::Bits;
-      OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
-      for (int32_t r = part; r < have; r += split) {
-        float y = 0.0f;
-        for (int32_t p = 0; p < split; ++p) y += peer_float(ring + (r * kTileN + local) * 4, p);
-        if (n < g.N) out[r * g.out_stride] = Dt<O>::from_float_dev(y);
+    // this CTA's share of the tile's rows, summed over the cluster in its order
+    const int32_t rows = first % g.row_tiles, n = first / g.row_tiles * kTileN + lane * 4;
+    const int32_t have = min(NT, g.T - rows * NT);
+    using OBits = typename Dt<O>::Bits;
+    OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
+    for (int32_t r = part + split * warp; r < have; r += split * (kThreads / 32)) {
+      float4 v[kMaxSplit];
+#pragma unroll
+      for (int p = 0; p < kMaxSplit; ++p)
+        v[p] = p < split ? peer_float4(ring + (r * kTileN + lane * 4) * 4, p) : float4{};
+      float y[4] = {};
+#pragma unroll
+      for (int p = 0; p < kMaxSplit; ++p) {
+        y[0] += v[p].x;
+        y[1] += v[p].y;
+        y[2] += v[p].z;
+        y[3] += v[p].w;
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < g.N) out[r * g.out_stride + i] = Dt<O>::from_float_dev(y[i]);
     }
     cluster_sync();
   }
@@ -638,31 +689,39 @@ int32_t row_tile(int32_t rows) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
+// Rows of a pair. Wide ones need fewer, fuller matrix instructions (a prompt's
+// rows come in runs of one adapter); narrow ones carry fewer zeros where every
+// row may have an adapter of its own, as in a batch of single tokens.
+int32_t block_of(int32_t rows, int32_t adapters) { return rows > 256 && adapters <= 64 ? 64 : 16; }
+
 struct Workspace {
+  int32_t block, most_pairs;
   size_t count, pairs, low, bytes;
 };
-Workspace workspace_of(int32_t rows, int32_t rank) {
+Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters) {
   const int32_t nt = row_tile(rows);
   const size_t tiles = (static_cast<size_t>(rows) + nt - 1) / nt;
   Workspace w;
+  w.block = block_of(rows, adapters);
+  w.most_pairs = nt / w.block * std::min(w.block, std::max(adapters, 1));
   w.count = 0;
   w.pairs = align256(tiles * sizeof(int32_t));
-  w.low = w.pairs + align256(tiles * nt * sizeof(uint32_t));
-  w.bytes = w.low + align256(tiles * nt * rank * 64);
+  w.low = w.pairs + align256(tiles * w.most_pairs * sizeof(uint32_t));
+  w.bytes = w.low + align256(tiles * w.most_pairs * rank * w.block * 4);
   return w;
 }
 
-template <typename T, typename O, int NT>
+template <typename T, typename O, int NT, int BLOCK>
 cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
                         cudaStream_t st) {
   static std::atomic<bool> ready[64];
-  auto kernel = project_kernel<T, O, NT>;
+  auto kernel = project_kernel<T, O, NT, BLOCK>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Shape<NT>::kBytes);
+                             Shape<NT, BLOCK>::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
@@ -676,7 +735,7 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? tiles * split
                                                      : std::min<int64_t>(tiles, sms)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<NT>::kBytes;
+  cfg.dynamicSmemBytes = Shape<NT, BLOCK>::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -690,21 +749,28 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g, split);
 }
 
+template <typename T, int BLOCK>
+cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
+  const dim3 grid((g.T + BLOCK - 1) / BLOCK * kShrinkCtas<BLOCK>), block(kShrinkThreads);
+  return g.rank <= 16   ? launch_pdl(shrink_kernel<T, BLOCK, 16>, grid, block, 0, st, g)
+         : g.rank <= 32 ? launch_pdl(shrink_kernel<T, BLOCK, 32>, grid, block, 0, st, g)
+                        : launch_pdl(shrink_kernel<T, BLOCK, 64>, grid, block, 0, st, g);
+}
+
 template <typename T, typename O>
 cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
                            cudaStream_t st) {
-  if (g.ids) {
-    const cudaError_t e =
-        launch_pdl(shrink_kernel<T>, dim3(g.T), dim3(kShrinkThreads), 0, st, g);
-    if (e != cudaSuccess) return e;
-  }
-  cudaError_t e;
+  cudaError_t e = cudaSuccess;
+  if (g.ids) e = g.block == 64 ? launch_shrink<T, 64>(g, st) : launch_shrink<T, 16>(g, st);
+  if (e != cudaSuccess) return e;
   switch (g.tile) {
-    case 16: e = launch_tile<T, O, 16>(wmap, xmap, g, st); break;
-    case 32: e = launch_tile<T, O, 32>(wmap, xmap, g, st); break;
-    case 64: e = launch_tile<T, O, 64>(wmap, xmap, g, st); break;
-    case 128: e = launch_tile<T, O, 128>(wmap, xmap, g, st); break;
-    default: e = launch_tile<T, O, 256>(wmap, xmap, g, st);
+    case 16: e = launch_tile<T, O, 16, 16>(wmap, xmap, g, st); break;
+    case 32: e = launch_tile<T, O, 32, 16>(wmap, xmap, g, st); break;
+    case 64: e = launch_tile<T, O, 64, 16>(wmap, xmap, g, st); break;
+    case 128: e = launch_tile<T, O, 128, 16>(wmap, xmap, g, st); break;
+    default:
+      e = g.block == 64 ? launch_tile<T, O, 256, 64>(wmap, xmap, g, st)
+                        : launch_tile<T, O, 256, 16>(wmap, xmap, g, st);
   }
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e;
@@ -715,8 +781,8 @@ cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, con
 
 using namespace bpd;
 
-extern "C" size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank) {
-  return workspace_of(std::max(rows, 1), std::max(rank, 0)).bytes;
+extern "C" size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t num_adapters) {
+  return workspace_of(std::max(rows, 1), std::max(rank, 0), num_adapters).bytes;
 }
 
 extern "C" bpd_status bpd_lora_take_error(int32_t* error_out) {
@@ -776,13 +842,13 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   if (!matrix_map(&wmap, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
       !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, nt))
     return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
-  const Workspace w = workspace_of(rows, rank);
+  const Workspace w = workspace_of(rows, rank, num_adapters);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
-                   reinterpret_cast<uint32_t*>(ws + w.pairs), ws + w.low, nt, row_tiles,
-                   out_tiles};
+                   reinterpret_cast<uint32_t*>(ws + w.pairs), ws + w.low, nt, w.block,
+                   w.most_pairs, row_tiles, out_tiles};
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (bf16)

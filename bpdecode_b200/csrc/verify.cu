@@ -33,7 +33,6 @@ constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyArgs {
   const void* src;
