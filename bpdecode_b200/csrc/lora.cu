@@ -12,10 +12,14 @@
 // another adapter. Few rows are bound by reading W, which every row shares and
 // which is read once; the adapters' steps then cost what reading B_a costs.
 //
-// S goes into those steps in blocks of 16 rows, the smallest N of the matrix
-// unit at M = 128 (of 64 for prompts): a (block, adapter) pair exists only
-// where one of the block's rows has that adapter, so there are at most as many
-// pairs as rows, whatever their order. Rows need not be sorted.
+// The rows of S that a step covers are an item: a run of 16-row blocks that one
+// adapter's rows lie in, with zeros in the rows of others. An item has a row
+// for every kReach of its blocks at least, so a batch of single tokens has one
+// item for each adapter, a prompt's runs have one each, and rows far apart one
+// each; they need not be sorted. A matrix instruction over few rows costs
+// nearly what one over 128 costs (about 87 cycles at 16 rows), which is why
+// items are wide rather than exact: with 16-row items alone, 256 rows with 24
+// adapters took 226 us at 65,536 outputs, against 134 us without adapters.
 //
 // S is held as the sum of two 16-bit values (its rounding, and what that left
 // off): together 2^-17 of it in bf16, 2^-22 in fp16, so an fp32 result keeps
@@ -34,8 +38,10 @@ namespace {
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kTileN = 128;        // outputs of a tile: the M of the matrix instruction
 constexpr int kStepK = 64;         // inner elements of a step: one 128-byte swizzled row
-constexpr int kRankStep = 64;      // inner elements of an adapter's step, at most
-constexpr int kMaxPairs = 32;      // pairs of an adapters' step, at most
+constexpr int kBlock = 16;         // rows of x of a block
+constexpr int kRankStep = 32;      // inner elements of an adapter's step, at most
+constexpr int kMaxItems = 8;       // items of an adapters' step, at most
+constexpr int kReach = 4;          // blocks that an item spans for each row that it has, at most
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share one tile's inner elements
 constexpr int kThreads = 192;      // loads, products, four warps that write
 constexpr int kShrinkThreads = 256;
@@ -56,12 +62,12 @@ struct LoraArgs {
   int32_t ids64;
   void* out;
   int64_t out_stride;
-  // workspace: the pairs of each tile of rows, in the order of their adapters
-  int32_t* count;    // [row tiles]
-  uint32_t* pairs;   // [row tiles, most_pairs]: adapter << 4 | block
-  uint8_t* low;      // [row tiles, most_pairs, rank * block * 4 bytes]: S of a pair's rows
-  int32_t tile, block;  // rows of a tile and of a block
-  int32_t most_pairs;   // of a tile
+  // workspace: the items of each tile of rows
+  int32_t* count;       // [row tiles]
+  uint2* items;         // [row tiles, tile]: adapter; first block of S << 9 | first block << 5 | blocks
+  uint8_t* low;         // [row tiles, most_blocks, rank * 64 bytes]: S of the items' blocks
+  int32_t tile;         // rows of a tile
+  int32_t most_blocks;  // of S, of a tile's items
   int32_t row_tiles, out_tiles;
 };
 
@@ -191,14 +197,14 @@ constexpr uint32_t instruction(uint32_t n) {
 }
 
 // ---------------------------------------------------------------------------
-// S. A few CTAs for each block of rows share the adapters that the block has:
-// BLOCK rows of x by the adapter's A over all inner elements, the warps split
-// over 16-row groups and over the inner elements. Bound by the latency of
-// reading A, and hidden behind the product's reading of W: a CTA is small
-// enough (18 KB of shared memory) to stand beside one of the product's. The
-// products go through mma.sync, whose rate is no limit here. The order of the
-// inner elements within a step is permuted, alike in both operands, so that
-// every load is 16 bytes.
+// S. An item's rows are gathered, up to 16 * GROUPS of them, and multiplied by
+// its adapter's A over all inner elements; the warps split over 16-row groups
+// and over the inner elements, which a cluster splits further where there are
+// few items. Bound by the latency of reading A and x, and hidden behind the
+// product's reading of W: a CTA is small enough (20 KB of shared memory) to
+// stand beside one of the product's. The products go through mma.sync, whose
+// rate is no limit here. The order of the inner elements within a step is
+// permuted, alike in both operands, so that every load is 16 bytes.
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -218,110 +224,246 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
   }
 }
 
-// CTAs of a block: as many as it can have adapters, or few where the rows are
-// a prompt's and come in runs.
-template <int BLOCK>
-constexpr int kShrinkCtas = BLOCK == 16 ? 16 : 4;
-
-template <typename T, int BLOCK, int RS>
-__global__ void __launch_bounds__(kShrinkThreads, 2) shrink_kernel(const LoraArgs g) {
+template <typename T, int GROUPS, int RS>
+__global__ void __launch_bounds__(kShrinkThreads, 2)
+    shrink_kernel(const LoraArgs g, const int32_t turns, const int32_t split) {
   using Bits = typename Dt<T>::Bits;
-  constexpr int kGroups = BLOCK / 16;                     // 16-row groups of a block
-  constexpr int kParts = kShrinkThreads / 32 / kGroups;   // parts of the inner elements
-  constexpr int kSlots = std::min(kParts, 4096 / (BLOCK * RS));  // parts that are added at once
+  constexpr int kWarps = kShrinkThreads / 32;
+  constexpr int kRows = GROUPS * 16;           // rows of a unit
+  constexpr int kParts = kWarps / GROUPS;      // parts of the inner elements
+  constexpr int kSlots = std::min(kParts, 4096 / (kRows * RS));  // parts that are added at once
   constexpr int kUnroll = RS == 16 ? 4 : RS == 32 ? 3 : 2;
   __shared__ int32_t ids[256];
-  __shared__ uint8_t leads[256];
-  __shared__ float sums[kSlots][BLOCK][RS];
+  __shared__ uint2 items[256];
+  __shared__ uint16_t members[256];  // of an item
+  __shared__ uint8_t list[256];      // the rows of this item in the tile
+  __shared__ int32_t warp_items[kWarps], warp_blocks[kWarps], warp_rows[kWarps];
+  __shared__ float sums[kSlots][kRows][RS];
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t turn = blockIdx.x % kShrinkCtas<BLOCK>;
-  const int32_t r0 = blockIdx.x / kShrinkCtas<BLOCK> * BLOCK;  // the block's first row
-  const int32_t tile = r0 / g.tile, t0 = tile * g.tile, b0 = r0 - t0;
+  const int32_t kpart = blockIdx.x % split;
+  const int32_t turn = blockIdx.x / split % turns, tile = blockIdx.x / split / turns;
+  const int32_t t0 = tile * g.tile;
   pdl_wait();
   pdl_trigger();  // what ran before has completed: x is there for the next kernel, too
-  if (tid < g.tile) ids[tid] = adapter_of(g, t0 + tid);
+  const int32_t own = tid < g.tile ? adapter_of(g, t0 + tid) : -1;
+  ids[tid] = own;
   __syncthreads();
-  // the first row of each adapter in its block
-  bool lead = tid < g.tile && ids[tid] >= 0;
-  if (lead)
-    for (int32_t j = tid / BLOCK * BLOCK; j < tid; ++j) lead = lead && ids[j] != ids[tid];
-  leads[tid] = lead;
-  const int32_t total = __syncthreads_count(lead);
-  if (b0 == 0 && turn == 0 && tid == 0) g.count[tile] = total;
-
-  const int32_t group = warp % kGroups, part = warp / kGroups;
-  const int32_t i0 = b0 + group * 16 + (lane >> 2);  // this lane's two rows in the tile
-  const Bits* x0 = static_cast<const Bits*>(g.x) + static_cast<int64_t>(t0 + i0) * g.x_stride;
-  const Bits* x1 = x0 + 8 * g.x_stride;
-  // each part is a contiguous share of the inner elements, a multiple of 32
-  const int32_t share = ((g.K + 31) / 32 + kParts - 1) / kParts * 32;
-  const int32_t k0 = min(g.K, part * share), k1 = min(g.K, k0 + share);
-  int32_t seen = 0;
-  for (int32_t i = b0; i < b0 + BLOCK; ++i) {
-    if (!leads[i] || seen++ % kShrinkCtas<BLOCK> != turn) continue;  // alike in all threads
-    const int32_t a = ids[i];
-    const int32_t at_pair = __syncthreads_count(
-        lead && (ids[tid] < a || (ids[tid] == a && tid / BLOCK < b0 / BLOCK)));
-    const int64_t pair = static_cast<int64_t>(tile) * g.most_pairs + at_pair;
-    if (tid == 0)
-      g.pairs[pair] = (static_cast<uint32_t>(a) << 4) | static_cast<uint32_t>(b0 / BLOCK);
-    const bool in0 = ids[i0] == a, in1 = ids[i0 + 8] == a;
-    const float scale = g.scale[a];
-    for (int32_t c = 0; c < g.rank; c += RS) {
-      const int32_t rc = min(RS, g.rank - c);
-      const Bits* w = static_cast<const Bits*>(g.a) +
-                      (static_cast<int64_t>(a) * g.rank + c + (lane >> 2)) * g.K;
-      float acc[RS / 8][4] = {};
-      for (int32_t k = k0; k < k1; k += 32 * kUnroll) {
-        uint4 u[kUnroll], v[kUnroll], q[kUnroll][RS / 8];
+  // The first row of each adapter finds the adapter's items: runs of blocks
+  // that hold at least one of its rows for every kReach blocks.
+  uint32_t rows_in[8];  // the rows with this thread's adapter, a bit each
+  bool lead = own >= 0;
+  int32_t found = 0, blocks = 0;
+  auto each_item = [&](auto&& f) {
+    int32_t start = -1, end = 0, rows = 0;
 #pragma unroll
-        for (int s = 0; s < kUnroll; ++s) {
-          const int32_t at = k + s * 32 + (lane & 3) * 8;
-          const bool in = at < k1;
-          u[s] = in && in0 ? *reinterpret_cast<const uint4*>(x0 + at) : uint4{};
-          v[s] = in && in1 ? *reinterpret_cast<const uint4*>(x1 + at) : uint4{};
-#pragma unroll
-          for (int j = 0; j < RS / 8; ++j)
-            q[s][j] = in && j * 8 < rc
-                          ? *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(j) * 8 * g.K + at)
-                          : uint4{};
-        }
-#pragma unroll
-        for (int s = 0; s < kUnroll; ++s)
-#pragma unroll
-          for (int j = 0; j < RS / 8; ++j) {
-            mma_16816<T>(acc[j], u[s].x, v[s].x, u[s].y, v[s].y, q[s][j].x, q[s][j].y);
-            mma_16816<T>(acc[j], u[s].z, v[s].z, u[s].w, v[s].w, q[s][j].z, q[s][j].w);
-          }
+    for (int32_t b = 0; b < 16; ++b) {
+      const int32_t here = __popc((rows_in[b >> 1] >> ((b & 1) * 16)) & 0xFFFFu);
+      if (here == 0) continue;
+      if (start >= 0 && b + 1 - start > kReach * (rows + here)) {
+        f(start, end - start, rows);
+        start = -1;
       }
-      // the parts meet in a fixed order, kSlots at a time
-      for (int32_t round = 0; round < kParts; round += kSlots) {
-        if (part >= round && part < round + kSlots) {
-          float(*to)[RS] = sums[part - round];
-          const int32_t row = group * 16 + (lane >> 2);
+      if (start < 0) {
+        start = b;
+        rows = 0;
+      }
+      end = b + 1;
+      rows += here;
+    }
+    if (start >= 0) f(start, end - start, rows);
+  };
+  if (lead) {
 #pragma unroll
-          for (int j = 0; j < RS / 8; ++j)
+    for (int32_t w = 0; w < 8; ++w) {
+      uint32_t m = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float& f = to[row + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)];
-              f = round == 0 ? acc[j][e] : f + acc[j][e];
+      for (int32_t j = 0; j < 32; j += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(&ids[w * 32 + j]);
+        m |= (v.x == own ? 1u : 0u) << j | (v.y == own ? 2u : 0u) << j |
+             (v.z == own ? 4u : 0u) << j | (v.w == own ? 8u : 0u) << j;
+      }
+      rows_in[w] = m;
+      if (w < warp) lead = lead && m == 0;
+      if (w == warp) lead = lead && (m & ((1u << lane) - 1u)) == 0;
+    }
+    if (lead)
+      each_item([&](int32_t, int32_t n, int32_t) {
+        ++found;
+        blocks += n;
+      });
+  }
+  // where this thread's items go: the sums over the threads before it
+  int32_t at_item = found, at_block = blocks;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int32_t i = __shfl_up_sync(kFull, at_item, o), b = __shfl_up_sync(kFull, at_block, o);
+    if (lane >= o) {
+      at_item += i;
+      at_block += b;
+    }
+  }
+  if (lane == 31) {
+    warp_items[warp] = at_item;
+    warp_blocks[warp] = at_block;
+  }
+  __syncthreads();
+  int32_t total = 0;
+  at_item -= found;
+  at_block -= blocks;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      at_item += warp_items[w];
+      at_block += warp_blocks[w];
+    }
+    total += warp_items[w];
+  }
+  if (lead)
+    each_item([&](int32_t start, int32_t n, int32_t rows) {
+      items[at_item] = make_uint2(static_cast<uint32_t>(own),
+                                  static_cast<uint32_t>(at_block << 9 | start << 5 | n));
+      members[at_item++] = static_cast<uint16_t>(rows);
+      at_block += n;
+    });
+  __syncthreads();
+  if (turn == 0 && kpart == 0) {
+    if (tid < total) g.items[static_cast<int64_t>(tile) * g.tile + tid] = items[tid];
+    if (tid == 0) g.count[tile] = total;
+  }
+
+  const int32_t group = warp % GROUPS, part = warp / GROUPS + kpart * kParts;
+  // each part is a contiguous share of the inner elements, a multiple of 32
+  const int32_t share = ((g.K + 31) / 32 + kParts * split - 1) / (kParts * split) * 32;
+  const int32_t k0 = min(g.K, part * share), k1 = min(g.K, k0 + share);
+  int32_t unit = 0;
+  for (int32_t i = 0; i < total; ++i) {
+    const int32_t units = (members[i] + kRows - 1) / kRows;
+    const int32_t u0 = (turn - unit % turns + turns) % turns;  // the first one of this turn
+    unit += units;
+    if (u0 >= units) continue;  // alike in all threads of the cluster
+    const int32_t a = static_cast<int32_t>(items[i].x);
+    const int32_t n = items[i].y & 31u, b0 = (items[i].y >> 5) & 15u;
+    uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (items[i].y >> 9)) *
+                               (g.rank * 64);
+    const float scale = g.scale[a];
+    // the item's rows, in order
+    const bool mine = own == a && tid >= b0 * kBlock && tid < (b0 + n) * kBlock;
+    const uint32_t vote = __ballot_sync(kFull, mine);
+    if (lane == 0) warp_rows[warp] = __popc(vote);
+    __syncthreads();
+    int32_t at = __popc(vote & ((1u << lane) - 1u));
+    for (int32_t w = 0; w < warp; ++w) at += warp_rows[w];
+    if (mine) list[at] = static_cast<uint8_t>(tid);
+    __syncthreads();
+    // An operand's place: [rank step][rounded values, rests][rank / 8][rows][8].
+    auto place = [&](int32_t row, int32_t col, int32_t half) {
+      const int32_t c = col / kRankStep * kRankStep, wide = min(kRankStep, g.rank - c);
+      return low + (c * 2 + half * wide) * n * (kBlock * 2) +
+             ((col - c) >> 3) * n * (kBlock * 16) + row * 16;
+    };
+    if (u0 == 0) {  // the rows between
+      for (int32_t v = tid + kpart * kShrinkThreads; v < n * kBlock * (g.rank / 8);
+           v += kShrinkThreads * split) {
+        const int32_t row = v % (n * kBlock), col = v / (n * kBlock) * 8;
+        if (ids[b0 * kBlock + row] != a) {
+          *reinterpret_cast<uint4*>(place(row, col, 0)) = uint4{};
+          *reinterpret_cast<uint4*>(place(row, col, 1)) = uint4{};
+        }
+      }
+    }
+    for (int32_t u = u0; u < units; u += turns) {
+      const int32_t m0 = u * kRows, have = min(kRows, members[i] - m0);
+      const int32_t r0 = group * 16 + (lane >> 2), r1 = r0 + 8;  // this lane's two rows
+      const bool in0 = r0 < have, in1 = r1 < have;
+      const Bits* x0 = static_cast<const Bits*>(g.x) +
+                       static_cast<int64_t>(t0 + (in0 ? list[m0 + r0] : 0)) * g.x_stride;
+      const Bits* x1 = static_cast<const Bits*>(g.x) +
+                       static_cast<int64_t>(t0 + (in1 ? list[m0 + r1] : 0)) * g.x_stride;
+      const bool idle = group * 16 >= have;
+      for (int32_t c = 0; c < g.rank; c += RS) {
+        const int32_t rc = min(RS, g.rank - c);
+        const Bits* w = static_cast<const Bits*>(g.a) +
+                        (static_cast<int64_t>(a) * g.rank + c + (lane >> 2)) * g.K;
+        float acc[RS / 8][4] = {};
+        for (int32_t k = idle ? k1 : k0; k < k1; k += 32 * kUnroll) {
+          uint4 p[kUnroll], q[kUnroll], v[kUnroll][RS / 8];
+#pragma unroll
+          for (int s = 0; s < kUnroll; ++s) {
+            const int32_t e = k + s * 32 + (lane & 3) * 8;
+            const bool in = e < k1;
+            p[s] = in && in0 ? *reinterpret_cast<const uint4*>(x0 + e) : uint4{};
+            q[s] = in && in1 ? *reinterpret_cast<const uint4*>(x1 + e) : uint4{};
+#pragma unroll
+            for (int j = 0; j < RS / 8; ++j)
+              v[s][j] = in && j * 8 < rc ? *reinterpret_cast<const uint4*>(
+                                               w + static_cast<int64_t>(j) * 8 * g.K + e)
+                                         : uint4{};
+          }
+#pragma unroll
+          for (int s = 0; s < kUnroll; ++s)
+#pragma unroll
+            for (int j = 0; j < RS / 8; ++j) {
+              mma_16816<T>(acc[j], p[s].x, q[s].x, p[s].y, q[s].y, v[s][j].x, v[s][j].y);
+              mma_16816<T>(acc[j], p[s].z, q[s].z, p[s].w, q[s].w, v[s][j].z, v[s][j].w);
             }
         }
-        __syncthreads();
-      }
-      // the operand's layout: [rank / 8][rows][8], first the rounded values, then the rests
-      Bits* low = reinterpret_cast<Bits*>(g.low + (pair * g.rank + c) * (BLOCK * 4));
-      for (int32_t e = tid; e < BLOCK * rc; e += kShrinkThreads) {
-        const int32_t row = (e >> 3) % BLOCK, col = e / (8 * BLOCK) * 8 + (e & 7);
-        float s = 0.0f;
+        // the parts meet in a fixed order, kSlots at a time
+        for (int32_t round = 0; round < kParts; round += kSlots) {
+          const int32_t slot = warp / GROUPS - round;
+          if (slot >= 0 && slot < kSlots) {
 #pragma unroll
-        for (int p = 0; p < kSlots; ++p) s += sums[p][row][col];
-        s = ids[b0 + row] == a ? s * scale : 0.0f;
-        const Bits hi = Dt<T>::from_float_dev(s);
-        low[e] = hi;
-        low[BLOCK * rc + e] = Dt<T>::from_float_dev(s - Dt<T>::to_float(hi));
+            for (int j = 0; j < RS / 8; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float& f = sums[slot][r0 + (e >> 1) * 8][j * 8 + (lane & 3) * 2 + (e & 1)];
+                f = round == 0 ? acc[j][e] : f + acc[j][e];
+              }
+          }
+          __syncthreads();
+        }
+        if constexpr (kSlots > 1) {
+          for (int32_t e = tid; e < have * RS; e += kShrinkThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kSlots; ++p) s += sums[p][e / RS][e % RS];
+            sums[0][e / RS][e % RS] = s;
+          }
+        }
+        if (split > 1)
+          cluster_sync();
+        else
+          __syncthreads();
+        for (int32_t v = tid; v < have * (rc / 8); v += kShrinkThreads) {
+          const int32_t r = v / (rc / 8), col = v % (rc / 8) * 8;
+          if (split > 1 && r % split != kpart) continue;
+          float s[8] = {};
+          if (split > 1) {
+            for (int32_t p = 0; p < split; ++p) {
+              const uint32_t from = shared_addr(&sums[0][r][col]);
+              const float4 f = peer_float4(from, p), h = peer_float4(from + 16, p);
+              s[0] += f.x; s[1] += f.y; s[2] += f.z; s[3] += f.w;
+              s[4] += h.x; s[5] += h.y; s[6] += h.z; s[7] += h.w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = sums[0][r][col + e];
+          }
+          alignas(16) Bits hi[8], rest[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            s[e] *= scale;
+            hi[e] = Dt<T>::from_float_dev(s[e]);
+            rest[e] = Dt<T>::from_float_dev(s[e] - Dt<T>::to_float(hi[e]));
+          }
+          const int32_t row = list[m0 + r] - b0 * kBlock;
+          *reinterpret_cast<uint4*>(place(row, c + col, 0)) = *reinterpret_cast<uint4*>(hi);
+          *reinterpret_cast<uint4*>(place(row, c + col, 1)) = *reinterpret_cast<uint4*>(rest);
+        }
+        if (split > 1)
+          cluster_sync();
+        else
+          __syncthreads();
       }
-      __syncthreads();
     }
   }
 }
@@ -329,35 +471,37 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) shrink_kernel(const LoraArg
 // ---------------------------------------------------------------------------
 // The product.
 
-template <int NT, int BLOCK>
+template <int NT>
 struct Shape {
   static constexpr int kWeightBytes = kTileN * kStepK * 2;
-  // a stage holds a step's rows of x, or the pairs of an adapter's step
-  static constexpr int kRowBytes = std::max(NT * kStepK * 2, BLOCK * kRankStep * 4);
-  static constexpr int kStageBytes = kWeightBytes + kRowBytes;
+  // a stage holds a step's tiles of W and x, or at least one item of any size
+  static constexpr int kStageBytes =
+      std::max(kWeightBytes + NT * kStepK * 2, kRankStep * (kTileN * 2 + NT * 4));
   // leaves room for a CTA of shrink_kernel on the same SM
   static constexpr int kStages = (200 * 1024) / kStageBytes;
   static constexpr int kColumns = std::max(32, 2 * NT);  // tensor memory: two accumulators
   static constexpr int kBytes = kStages * kStageBytes + 1024;  // with room to align
 };
 
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 11;
 constexpr uint32_t kEnd = 0;  // an empty step behind the last adapter of a tile
 
 struct ProjectShared {
   uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
-  uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | pairs; kEnd
-  uint8_t pair[kMaxStages][kMaxPairs];  // its pairs: adapter of the step << 4 | block
+  uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | items; kEnd
+  uint32_t item[kMaxStages][kMaxItems];  // B << 19 | S << 9 (their places / 128) | block << 5 | blocks
   uint32_t tmem;
   uint32_t failed;
-  uint32_t list[256];
+  uint2 list[256];
 };
 
-template <typename T, typename O, int NT, int BLOCK>
+template <typename T, typename O, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const LoraArgs g, const int32_t split) {
-  using S = Shape<NT, BLOCK>;
+  using S = Shape<NT>;
+  static_assert(S::kStages <= kMaxStages && S::kStages * S::kStageBytes >= NT * kTileN * 4,
+                "barriers for each stage, room for a tile of sums");
   extern __shared__ uint8_t dynamic[];
   __shared__ ProjectShared sh;
   const uint32_t ring = (shared_addr(dynamic) + 1023u) & ~1023u;
@@ -400,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // --- loads ---------------------------------------------------------------
     if (!g.ids) pdl_wait();  // else what ran before the first kernel has completed
     bool waited = false;
-    int32_t listed = -1, pairs = 0;
+    int32_t listed = -1, items = 0;
     int32_t stage = 0;
     uint32_t phase = 0;
     int32_t issued = 0;
@@ -430,60 +574,62 @@ __global__ void __launch_bounds__(kThreads, 1)
         waited = true;
       }
       if (listed != rows) {
-        pairs = min(g.count[rows], g.most_pairs);
+        items = min(g.count[rows], NT);
         __syncwarp();
-        for (int32_t i = lane; i < pairs; i += 32)
-          sh.list[i] = g.pairs[static_cast<int64_t>(rows) * g.most_pairs + i];
+        for (int32_t i = lane; i < items; i += 32)
+          sh.list[i] = g.items[static_cast<int64_t>(rows) * NT + i];
         __syncwarp();
         listed = rows;
       }
       if (lane == 0) {
-        // A step takes as many pairs as fit: the ring is as long as the queue
+        // A step takes as many items as fit: the ring is as long as the queue
         // of loads in front of HBM, so a step costs its share of that queue
         // however little it carries (one adapter a step: 0.7 us each).
-        const int32_t p0 = pairs * part / split, p1 = pairs * (part + 1) / split;
+        const int32_t p0 = items * part / split, p1 = items * (part + 1) / split;
         for (int32_t c = 0; c < g.rank && ok; c += kRankStep) {
           const int32_t rc = min(kRankStep, g.rank - c);
-          const int32_t adapters = kRankStep / rc;
-          const int32_t most = min(kMaxPairs, S::kRowBytes / (rc * BLOCK * 4));
           for (int32_t p = p0; p < p1;) {
             if (!(ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) break;
             const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
-            int32_t n = 0, met = 0;
-            uint32_t last = 0;
-            for (; n < most && p + n < p1; ++n) {
-              const uint32_t pair = sh.list[p + n], a = pair >> 4;
-              if (met == 0 || a != last) {
-                if (met == adapters) break;
-                ++met;
-                last = a;
-              }
-              sh.pair[stage][n] = static_cast<uint8_t>((met - 1) << 4 | (pair & 15u));
+            // first the sum of the bytes, then the copies
+            int32_t n = 0, used = 0, b_at = 0;
+            uint32_t last = ~0u;
+            for (; n < kMaxItems && p + n < p1; ++n) {
+              const uint2 item = sh.list[p + n];
+              const int32_t b_bytes = item.x == last ? 0 : rc * kTileN * 2;
+              const int32_t s_bytes = static_cast<int32_t>(item.y & 31u) * rc * 64;
+              if (used + b_bytes + s_bytes > S::kStageBytes) break;
+              if (b_bytes) b_at = used;
+              sh.item[stage][n] = static_cast<uint32_t>(b_at / 128) << 19 |
+                                  static_cast<uint32_t>((used + b_bytes) / 128) << 9 |
+                                  (item.y & 511u);
+              used += b_bytes + s_bytes;
+              last = item.x;
             }
             sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
-            bar_expect(bar, met * rc * kTileN * 2 + n * rc * BLOCK * 4);
-            for (int32_t i = 0, m = -1; i < n; ++i) {
-              const uint32_t a = sh.list[p + i] >> 4;
-              if (i == 0 || a != last) {
-                last = a;
-                load_bulk(at + ++m * rc * kTileN * 2,
+            bar_expect(bar, used);
+            last = ~0u;
+            used = 0;
+            for (int32_t i = 0; i < n; ++i) {
+              const uint2 item = sh.list[p + i];
+              if (item.x != last) {
+                last = item.x;
+                load_bulk(at + used,
                           static_cast<const uint8_t*>(g.b) +
-                              ((static_cast<int64_t>(a) * g.out_tiles + outs) * g.rank + c) *
+                              ((static_cast<int64_t>(item.x) * g.out_tiles + outs) * g.rank + c) *
                                   (kTileN * 2),
                           rc * kTileN * 2, bar);
+                used += rc * kTileN * 2;
               }
-              // pairs that follow one another in memory, too, where rank is one step
-              if (rc != g.rank)
-                load_bulk(at + S::kWeightBytes + i * rc * BLOCK * 4,
-                          g.low + ((static_cast<int64_t>(rows) * g.most_pairs + p + i) * g.rank + c) *
-                                      (BLOCK * 4),
-                          rc * BLOCK * 4, bar);
+              const int32_t s_bytes = static_cast<int32_t>(item.y & 31u) * rc * 64;
+              load_bulk(at + used,
+                        g.low +
+                            (static_cast<int64_t>(rows) * g.most_blocks + (item.y >> 9)) *
+                                (g.rank * 64) +
+                            static_cast<int32_t>(item.y & 31u) * c * 64,
+                        s_bytes, bar);
+              used += s_bytes;
             }
-            if (rc == g.rank)
-              load_bulk(at + S::kWeightBytes,
-                        g.low + (static_cast<int64_t>(rows) * g.most_pairs + p) * g.rank *
-                                    (BLOCK * 4),
-                        n * rc * BLOCK * 4, bar);
             next();
             p += n;
           }
@@ -543,15 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int32_t rc = shape >> 8, n = shape & 255;
             for (int32_t i = 0; i < n; ++i) {
-              const uint32_t pair = sh.pair[stage][i];
-              const uint32_t to = d + (pair & 15u) * BLOCK;
-              const uint32_t b = at + (pair >> 4) * rc * kTileN * 2;
-              const uint32_t low = at + S::kWeightBytes + i * rc * BLOCK * 4;
-              for (int32_t half = 0; half < 2; ++half)
-                for (int32_t k = 0; k < rc; k += 16)
-                  mma(to, desc_plain(b + k * kTileN * 2, kTileN * 16),
-                      desc_plain(low + half * rc * BLOCK * 2 + k * BLOCK * 2, BLOCK * 16),
-                      instruction<T>(BLOCK), true);
+              const uint32_t item = sh.item[stage][i], wide = item & 31u;
+              const uint32_t to = d + ((item >> 5) & 15u) * kBlock;
+              const uint64_t b = desc_plain(at + (item >> 19) * 128, kTileN * 16);
+              const uint64_t low = desc_plain(at + ((item >> 9) & 1023u) * 128, wide * kBlock * 16);
+              const uint32_t idesc = instruction<T>(0) | (wide * (kBlock >> 3)) << 17;
+              for (int32_t k = 0; k < 2 * rc; k += 16)  // the rounded values, then the rests
+                mma(to, b + (k < rc ? k : k - rc) * (kTileN * 2 / 16),
+                    low + k * (wide * kBlock * 2 / 16), idesc, true);
             }
             finish();
           }
@@ -689,39 +834,34 @@ int32_t row_tile(int32_t rows) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
-// Rows of a pair. Wide ones need fewer, fuller matrix instructions (a prompt's
-// rows come in runs of one adapter); narrow ones carry fewer zeros where every
-// row may have an adapter of its own, as in a batch of single tokens.
-int32_t block_of(int32_t rows, int32_t adapters) { return rows > 256 && adapters <= 64 ? 64 : 16; }
-
 struct Workspace {
-  int32_t block, most_pairs;
-  size_t count, pairs, low, bytes;
+  int32_t most_blocks;
+  size_t count, items, low, bytes;
 };
 Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters) {
   const int32_t nt = row_tile(rows);
   const size_t tiles = (static_cast<size_t>(rows) + nt - 1) / nt;
   Workspace w;
-  w.block = block_of(rows, adapters);
-  w.most_pairs = nt / w.block * std::min(w.block, std::max(adapters, 1));
+  w.most_blocks = std::min<int64_t>(kReach * nt, static_cast<int64_t>(nt / kBlock) *
+                                                     std::max(adapters, 1));
   w.count = 0;
-  w.pairs = align256(tiles * sizeof(int32_t));
-  w.low = w.pairs + align256(tiles * w.most_pairs * sizeof(uint32_t));
-  w.bytes = w.low + align256(tiles * w.most_pairs * rank * w.block * 4);
+  w.items = align256(tiles * sizeof(int32_t));
+  w.low = w.items + align256(tiles * nt * sizeof(uint2));
+  w.bytes = w.low + align256(tiles * w.most_blocks * rank * 64);
   return w;
 }
 
-template <typename T, typename O, int NT, int BLOCK>
+template <typename T, typename O, int NT>
 cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
                         cudaStream_t st) {
   static std::atomic<bool> ready[64];
-  auto kernel = project_kernel<T, O, NT, BLOCK>;
+  auto kernel = project_kernel<T, O, NT>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Shape<NT, BLOCK>::kBytes);
+                             Shape<NT>::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
@@ -735,7 +875,7 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? tiles * split
                                                      : std::min<int64_t>(tiles, sms)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<NT, BLOCK>::kBytes;
+  cfg.dynamicSmemBytes = Shape<NT>::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -749,28 +889,58 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g, split);
 }
 
-template <typename T, int BLOCK>
+template <typename T, int GROUPS, int RS>
+cudaError_t launch_shrink_rank(const LoraArgs& g, int32_t turns, int32_t split, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(g.row_tiles * turns * split));
+  cfg.blockDim = dim3(kShrinkThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = BPD_PDL ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, shrink_kernel<T, GROUPS, RS>, g, turns, split);
+}
+
+template <typename T, int GROUPS>
+cudaError_t launch_shrink_groups(const LoraArgs& g, int32_t turns, int32_t split, cudaStream_t st) {
+  return g.rank <= 16   ? launch_shrink_rank<T, GROUPS, 16>(g, turns, split, st)
+         : g.rank <= 32 ? launch_shrink_rank<T, GROUPS, 32>(g, turns, split, st)
+                        : launch_shrink_rank<T, GROUPS, 64>(g, turns, split, st);
+}
+
+template <typename T>
 cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
-  const dim3 grid((g.T + BLOCK - 1) / BLOCK * kShrinkCtas<BLOCK>), block(kShrinkThreads);
-  return g.rank <= 16   ? launch_pdl(shrink_kernel<T, BLOCK, 16>, grid, block, 0, st, g)
-         : g.rank <= 32 ? launch_pdl(shrink_kernel<T, BLOCK, 32>, grid, block, 0, st, g)
-                        : launch_pdl(shrink_kernel<T, BLOCK, 64>, grid, block, 0, st, g);
+  // A tile's items go round its CTAs in turn: as many CTAs as it can have
+  // items where there is one tile, a few for each tile of a prompt. What is
+  // left of the SMs splits the inner elements.
+  const bool prompt = g.row_tiles > 1;
+  const int32_t turns = prompt ? 4 : std::min(g.T, g.adapters);
+  int32_t split = 1;
+  while (split < kMaxSplit && static_cast<int64_t>(g.row_tiles) * turns * split * 2 <= sm_count() &&
+         split * 512 <= g.K)
+    split *= 2;
+  return prompt ? launch_shrink_groups<T, 4>(g, turns, split, st)
+                : launch_shrink_groups<T, 1>(g, turns, split, st);
 }
 
 template <typename T, typename O>
 cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
                            cudaStream_t st) {
-  cudaError_t e = cudaSuccess;
-  if (g.ids) e = g.block == 64 ? launch_shrink<T, 64>(g, st) : launch_shrink<T, 16>(g, st);
-  if (e != cudaSuccess) return e;
-  switch (g.tile) {
-    case 16: e = launch_tile<T, O, 16, 16>(wmap, xmap, g, st); break;
-    case 32: e = launch_tile<T, O, 32, 16>(wmap, xmap, g, st); break;
-    case 64: e = launch_tile<T, O, 64, 16>(wmap, xmap, g, st); break;
-    case 128: e = launch_tile<T, O, 128, 16>(wmap, xmap, g, st); break;
-    default:
-      e = g.block == 64 ? launch_tile<T, O, 256, 64>(wmap, xmap, g, st)
-                        : launch_tile<T, O, 256, 16>(wmap, xmap, g, st);
+  cudaError_t e = g.ids ? launch_shrink<T>(g, st) : cudaSuccess;
+  if (e == cudaSuccess) {
+    switch (g.tile) {
+      case 16: e = launch_tile<T, O, 16>(wmap, xmap, g, st); break;
+      case 32: e = launch_tile<T, O, 32>(wmap, xmap, g, st); break;
+      case 64: e = launch_tile<T, O, 64>(wmap, xmap, g, st); break;
+      case 128: e = launch_tile<T, O, 128>(wmap, xmap, g, st); break;
+      default: e = launch_tile<T, O, 256>(wmap, xmap, g, st);
+    }
   }
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e;
@@ -847,8 +1017,8 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
-                   reinterpret_cast<uint32_t*>(ws + w.pairs), ws + w.low, nt, w.block,
-                   w.most_pairs, row_tiles, out_tiles};
+                   reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, w.most_blocks, row_tiles,
+                   out_tiles};
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (bf16)
