@@ -438,11 +438,17 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
           if (split > 1 && r % split != kpart) continue;
           float s[8] = {};
           if (split > 1) {
-            for (int32_t p = 0; p < split; ++p) {
-              const uint32_t from = shared_addr(&sums[0][r][col]);
-              const float4 f = peer_float4(from, p), h = peer_float4(from + 16, p);
-              s[0] += f.x; s[1] += f.y; s[2] += f.z; s[3] += f.w;
-              s[4] += h.x; s[5] += h.y; s[6] += h.z; s[7] += h.w;
+            const uint32_t from = shared_addr(&sums[0][r][col]);
+            float4 f[kMaxSplit], h[kMaxSplit];
+#pragma unroll
+            for (int p = 0; p < kMaxSplit; ++p) {
+              f[p] = p < split ? peer_float4(from, p) : float4{};
+              h[p] = p < split ? peer_float4(from + 16, p) : float4{};
+            }
+#pragma unroll
+            for (int p = 0; p < kMaxSplit; ++p) {
+              s[0] += f[p].x; s[1] += f[p].y; s[2] += f[p].z; s[3] += f[p].w;
+              s[4] += h[p].x; s[5] += h[p].y; s[6] += h[p].z; s[7] += h[p].w;
             }
           } else {
 #pragma unroll
@@ -489,10 +495,14 @@ constexpr uint32_t kEnd = 0;  // an empty step behind the last adapter of a tile
 struct ProjectShared {
   uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
   uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | items; kEnd
-  uint32_t item[kMaxStages][kMaxItems];  // B << 19 | S << 9 (their places / 128) | block << 5 | blocks
+  uint32_t item[kMaxStages][kMaxItems];  // its items, as in `plan`
   uint32_t tmem;
   uint32_t failed;
-  uint2 list[256];
+  // the items of the tile of rows, and the steps that they go in
+  uint32_t adapter[256];
+  uint32_t blocks[256];     // first block of S
+  uint32_t plan[256];       // loads B << 31 | B << 20 | S << 9 (places) | first block << 5 | blocks
+  uint16_t step[257];       // first item of each step
 };
 
 template <typename T, typename O, int NT>
@@ -544,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // --- loads ---------------------------------------------------------------
     if (!g.ids) pdl_wait();  // else what ran before the first kernel has completed
     bool waited = false;
-    int32_t listed = -1, items = 0;
+    int32_t listed = -1, nsteps = 0;
     int32_t stage = 0;
     uint32_t phase = 0;
     int32_t issued = 0;
@@ -557,90 +567,112 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (int32_t tile = first; tile < tiles && ok; tile += stride) {
       const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles;
-      if (lane == 0) {
-        for (int32_t s = s0; s < s1; ++s) {
-          if (!(ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) break;
+      for (int32_t s = s0; s < s1; ++s) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
+        if (!ok) break;
+        if (lane == 0) {
           const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
           bar_expect(bar, S::kWeightBytes + NT * kStepK * 2);
           load_box(at, &wmap, s * kStepK, outs * kTileN, bar);
           load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT, bar);
-          next();
         }
+        next();
       }
-      ok = __shfl_sync(kFull, ok, 0);
       if (!g.ids || !ok) continue;
       if (!waited) {
         pdl_wait();  // S is there
         waited = true;
       }
       if (listed != rows) {
-        items = min(g.count[rows], NT);
-        __syncwarp();
-        for (int32_t i = lane; i < items; i += 32)
-          sh.list[i] = g.items[static_cast<int64_t>(rows) * NT + i];
-        __syncwarp();
-        listed = rows;
-      }
-      if (lane == 0) {
         // A step takes as many items as fit: the ring is as long as the queue
         // of loads in front of HBM, so a step costs its share of that queue
-        // however little it carries (one adapter a step: 0.7 us each).
+        // however little it carries (one adapter a step: 0.7 us each). The
+        // plan is made once for a tile of rows; places are in units of 64
+        // bytes for each inner element of a step.
+        listed = rows;
+        const int32_t items = min(g.count[rows], NT);
         const int32_t p0 = items * part / split, p1 = items * (part + 1) / split;
-        for (int32_t c = 0; c < g.rank && ok; c += kRankStep) {
-          const int32_t rc = min(kRankStep, g.rank - c);
-          for (int32_t p = p0; p < p1;) {
-            if (!(ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) break;
-            const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
-            // first the sum of the bytes, then the copies
-            int32_t n = 0, used = 0, b_at = 0;
-            uint32_t last = ~0u;
-            for (; n < kMaxItems && p + n < p1; ++n) {
-              const uint2 item = sh.list[p + n];
-              const int32_t b_bytes = item.x == last ? 0 : rc * kTileN * 2;
-              const int32_t s_bytes = static_cast<int32_t>(item.y & 31u) * rc * 64;
-              if (used + b_bytes + s_bytes > S::kStageBytes) break;
-              if (b_bytes) b_at = used;
-              sh.item[stage][n] = static_cast<uint32_t>(b_at / 128) << 19 |
-                                  static_cast<uint32_t>((used + b_bytes) / 128) << 9 |
-                                  (item.y & 511u);
-              used += b_bytes + s_bytes;
-              last = item.x;
-            }
-            sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
-            bar_expect(bar, used);
-            last = ~0u;
-            used = 0;
-            for (int32_t i = 0; i < n; ++i) {
-              const uint2 item = sh.list[p + i];
-              if (item.x != last) {
-                last = item.x;
-                load_bulk(at + used,
-                          static_cast<const uint8_t*>(g.b) +
-                              ((static_cast<int64_t>(item.x) * g.out_tiles + outs) * g.rank + c) *
-                                  (kTileN * 2),
-                          rc * kTileN * 2, bar);
-                used += rc * kTileN * 2;
-              }
-              const int32_t s_bytes = static_cast<int32_t>(item.y & 31u) * rc * 64;
-              load_bulk(at + used,
-                        g.low +
-                            (static_cast<int64_t>(rows) * g.most_blocks + (item.y >> 9)) *
-                                (g.rank * 64) +
-                            static_cast<int32_t>(item.y & 31u) * c * 64,
-                        s_bytes, bar);
-              used += s_bytes;
-            }
-            next();
-            p += n;
-          }
+        __syncwarp();
+        for (int32_t i = p0 + lane; i < p1; i += 32) {
+          const uint2 item = g.items[static_cast<int64_t>(rows) * NT + i];
+          sh.adapter[i - p0] = item.x;
+          sh.blocks[i - p0] = item.y >> 9;
+          sh.plan[i - p0] = item.y & 511u;
         }
-        if (ok && (ok = bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1))) {
-          sh.shape[stage] = kEnd;
-          bar_arrive(shared_addr(&sh.full[stage]));
+        __syncwarp();
+        const int32_t room = S::kStageBytes / (64 * min(kRankStep, g.rank));
+        int32_t n = 0, used = 0, b_at = 0;
+        uint32_t last = ~0u;
+        nsteps = 0;
+        if (lane == 0) {
+          for (int32_t i = 0; i < p1 - p0; ++i) {
+            const uint32_t a = sh.adapter[i], item = sh.plan[i];
+            const int32_t wide = item & 31u;
+            if (i == 0 || n == kMaxItems || used + (a == last ? 0 : kTileN / 32) + wide > room) {
+              sh.step[nsteps++] = static_cast<uint16_t>(i);
+              n = used = 0;
+              last = ~0u;
+            }
+            const bool load = a != last;
+            if (load) {
+              b_at = used;
+              used += kTileN / 32;
+            }
+            sh.plan[i] = item | static_cast<uint32_t>(load) << 31 |
+                         static_cast<uint32_t>(b_at) << 20 | static_cast<uint32_t>(used) << 9;
+            used += wide;
+            last = a;
+            ++n;
+          }
+          sh.step[nsteps] = static_cast<uint16_t>(p1 - p0);
+        }
+        nsteps = __shfl_sync(kFull, nsteps, 0);
+        __syncwarp();
+      }
+      // each lane starts the copies of one item
+      for (int32_t c = 0; c < g.rank && ok; c += kRankStep) {
+        const int32_t rc = min(kRankStep, g.rank - c);
+        for (int32_t s = 0; s < nsteps; ++s) {
+          const int32_t i0 = sh.step[s], n = sh.step[s + 1] - i0;
+          const uint32_t at = ring + stage * S::kStageBytes;
+          const uint32_t item = lane < n ? sh.plan[i0 + lane] : 0, wide = item & 31u;
+          const bool load = item >> 31;
+          int32_t units = lane < n ? wide + (load ? kTileN / 32 : 0) : 0;
+#pragma unroll
+          for (int o = kMaxItems / 2; o > 0; o >>= 1) units += __shfl_xor_sync(kFull, units, o);
+          ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
+          if (!ok) break;
+          if (lane < n) sh.item[stage][lane] = item;
+          if (lane == 0) sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
+          __syncwarp();
+          const uint32_t bar = shared_addr(&sh.full[stage]);
+          if (lane == 0) bar_expect(bar, units * rc * 64);
+          __syncwarp();
+          if (lane < n) {
+            if (load)
+              load_bulk(at + ((item >> 20) & 2047u) * rc * 64,
+                        static_cast<const uint8_t*>(g.b) +
+                            ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles + outs) *
+                                 g.rank + c) * (kTileN * 2),
+                        rc * kTileN * 2, bar);
+            load_bulk(at + ((item >> 9) & 2047u) * rc * 64,
+                      g.low + (static_cast<int64_t>(rows) * g.most_blocks + sh.blocks[i0 + lane]) *
+                                  (g.rank * 64) + wide * c * 64,
+                      wide * rc * 64, bar);
+          }
           next();
         }
       }
-      ok = __shfl_sync(kFull, ok, 0);
+      if (ok) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
+        if (ok) {
+          if (lane == 0) {
+            sh.shape[stage] = kEnd;
+            bar_arrive(shared_addr(&sh.full[stage]));
+          }
+          next();
+        }
+      }
     }
     if (g.ids && !waited) pdl_wait();
     if (!ok && lane == 0) {
@@ -691,8 +723,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int32_t i = 0; i < n; ++i) {
               const uint32_t item = sh.item[stage][i], wide = item & 31u;
               const uint32_t to = d + ((item >> 5) & 15u) * kBlock;
-              const uint64_t b = desc_plain(at + (item >> 19) * 128, kTileN * 16);
-              const uint64_t low = desc_plain(at + ((item >> 9) & 1023u) * 128, wide * kBlock * 16);
+              const uint64_t b = desc_plain(at + ((item >> 20) & 2047u) * rc * 64, kTileN * 16);
+              const uint64_t low =
+                  desc_plain(at + ((item >> 9) & 2047u) * rc * 64, wide * kBlock * 16);
               const uint32_t idesc = instruction<T>(0) | (wide * (kBlock >> 3)) << 17;
               for (int32_t k = 0; k < 2 * rc; k += 16)  // the rounded values, then the rests
                 mma(to, b + (k < rc ? k : k - rc) * (kTileN * 2 / 16),
