@@ -17,10 +17,15 @@
 //
 // One cluster of CTAs works through one request, position after position, so
 // rows behind the first refused draft are never read. Each CTA scans a slice
-// of the row once, with a running maximum and sum; the slices' (m, argmax, s)
-// meet through distributed shared memory in a fixed order, so a result does
-// not depend on timing. The row that is replaced is scanned a second time
-// (from L2) with the noise and the draft's probabilities.
+// of the row once in 16-byte vectors, with a running maximum and sum, leaving
+// out vectors whose tokens are all rejected; the slices' (m, argmax, s) meet
+// through distributed shared memory in a fixed order, so a result does not
+// depend on timing. Behind the last draft the race runs in that same pass, on
+// x / T - log e, which needs neither m nor Z. A row whose draft was refused is
+// scanned a second time (from L2) with the noise and the draft's
+// probabilities. What a thread finds best is then scored again with full
+// precision, so that only scores within one thread are compared in fast
+// arithmetic.
 #include <algorithm>
 #include <climits>
 
@@ -30,9 +35,10 @@ namespace bpd {
 namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyArgs {
   const void* src;
@@ -75,21 +81,11 @@ struct Slice {
   float s;
 };
 
-// The two races over a slice: packed (score, lowest index) of max(p - q, 0) / e
-// and of p / e; 0 where nothing takes part.
-struct Race {
-  uint64_t left;
-  uint64_t all;
-};
-
 struct Shared {
   uint64_t warp_key[kVerifyWarps];
-  uint64_t warp_key2[kVerifyWarps];
   float warp_sum[kVerifyWarps];
-  Slice slice[2];  // by the position's parity: a neighbour may still read the other
-  Race race;
-  Slice row;       // the whole row's
-  Race winner;
+  Slice slice[2];   // by the position's parity: a neighbour may still read the other
+  uint64_t race[2]; // of two races in turn
   int32_t state[BPD_MAX_DRAFTS + 1];
 };
 
@@ -140,6 +136,41 @@ struct Allow {
   __device__ __forceinline__ bool has(int32_t t) const {
     return row ? ((__ldg(row + (t >> 5)) >> (t & 31)) & 1u) : any;
   }
+  // the bits of N tokens from t on, all of them inside the vocabulary
+  template <int N>
+  __device__ __forceinline__ uint32_t bits(int32_t t) const {
+    constexpr uint32_t all = (1u << N) - 1u;
+    if (!row) return any ? all : 0u;
+    const int32_t w = t >> 5, sh = t & 31;
+    const uint32_t lo = __ldg(row + w), hi = sh + N > 32 ? __ldg(row + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, sh) & all;
+  }
+};
+
+// A row of logits as 16-byte vectors: `head` tokens, `vecs` vectors, a tail.
+template <typename T>
+struct Row {
+  static constexpr int kEpv = Dt<T>::kPerVec;
+  using Bits = typename Dt<T>::Bits;
+  const Bits* p;
+  int32_t head, vecs, V;
+  __device__ Row(const void* row, int32_t V_) : p(static_cast<const Bits*>(row)), V(V_) {
+    const uintptr_t off = reinterpret_cast<uintptr_t>(row) & 15u;
+    head = min(V, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
+    vecs = (V - head) / kEpv;
+  }
+  __device__ __forceinline__ float at(int64_t t) const { return Dt<T>::to_float(p[t]); }
+  __device__ __forceinline__ int32_t token(int32_t vec) const { return head + vec * kEpv; }
+  __device__ __forceinline__ uint4 vec(int32_t j) const {
+    return __ldg(reinterpret_cast<const uint4*>(p + head) + j);
+  }
+  // the token outside the vectors that this thread looks at, or -1
+  __device__ __forceinline__ int32_t edge(bool first, bool last) const {
+    const int32_t i = threadIdx.x, tail = head + vecs * kEpv;
+    if (first && i < head) return i;
+    if (last && i >= 32 && i - 32 < V - tail) return tail + i - 32;
+    return -1;
+  }
 };
 
 // exp((x - m) / T) where x is not NaN and m the row's maximum: 1 at the
@@ -160,39 +191,197 @@ __device__ __forceinline__ float load_prob(const void* row, int32_t dtype, int64
   return load_logit<__half>(row, t);
 }
 
-// Maximum, its first index and the sum over tokens [t0, t1), by the whole CTA.
-template <typename T>
-__device__ Slice scan_slice(const void* row, const Allow& ok, int32_t t0, int32_t t1, float inv,
-                            Shared& sh) {
-  float m = -INFINITY, s = 0.0f;
-  int32_t idx = -1;
-  for (int32_t t = t0 + static_cast<int32_t>(threadIdx.x); t < t1; t += kVerifyThreads) {
-    if (!ok.has(t)) continue;
-    const float x = load_logit<T>(row, t);
-    if (!(x > -INFINITY)) continue;  // NaN counts as -inf
-    if (x > m) {
-      s = idx < 0 ? 1.0f : fmaf(s, expf((m - x) * inv), 1.0f);
-      m = x;
-      idx = t;
+// N consecutive values from p on, as fp32.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, bool aligned, float (&out)[N]) {
+  if (aligned) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i));
+      out[i] = f.x;
+      out[i + 1] = f.y;
+      out[i + 2] = f.z;
+      out[i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = __ldg(p + i);
+  }
+}
+
+// A row of the draft's probabilities (p == NULL: none).
+struct Given {
+  const void* p;
+  int32_t dtype;
+  bool aligned;  // its vectors begin where the logits' do, on 16 (8) bytes
+  template <int N>
+  __device__ __forceinline__ void load(int32_t t, float (&out)[N]) const {
+    if (dtype == BPD_F32) {
+      load_floats<N>(static_cast<const float*>(p) + t, aligned, out);
     } else {
-      s += weight(x, m, inv);
+      const uint16_t* h = static_cast<const uint16_t*>(p) + t;
+      uint32_t w[N / 2];
+      if (aligned) {
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 2) {
+          const uint2 u = __ldcs(reinterpret_cast<const uint2*>(h + 2 * i));
+          w[i] = u.x;
+          w[i + 1] = u.y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          w[i] = __ldg(h + 2 * i) | static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint16_t u = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+        out[i] = dtype == BPD_BF16 ? Dt<__nv_bfloat16>::to_float(u) : Dt<__half>::to_float(u);
+      }
     }
   }
-  const uint64_t mine = idx < 0 ? 0 : pack_arg(order_key(m), idx);
+};
+
+// The best of a thread in a race: what it needs to score it again.
+struct Best {
+  float score = -INFINITY, x = 0.0f, e = 1.0f;
+  int32_t idx = -1;
+};
+
+// The inverse of order_key.
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+__device__ __forceinline__ uint64_t block_max(uint64_t k, Shared& sh) {
   const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t k = warp_max_u64(mine);
+  k = warp_max_u64(k);
   if (lane == 0) sh.warp_key[warp] = k;
   __syncthreads();
-  k = sh.warp_key[lane < kVerifyWarps ? lane : 0];
-  k = warp_max_u64(k);
-  Slice out;
-  out.idx = k ? unpack_idx(k) : -1;
-  out.m = k ? load_logit<T>(row, out.idx) : -INFINITY;
-  s = idx < 0 ? 0.0f : s * weight(m, out.m, inv);
+  k = warp_max_u64(sh.warp_key[lane & (kVerifyWarps - 1)]);
+  return k;
+}
+// Between this and block_max there is a barrier in each call order used here.
+__device__ __forceinline__ float block_sum(float s, Shared& sh) {
+  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   s = warp_sum(s);
   if (lane == 0) sh.warp_sum[warp] = s;
   __syncthreads();
-  out.s = warp_sum(lane < kVerifyWarps ? sh.warp_sum[lane] : 0.0f);
+  return warp_sum(lane < kVerifyWarps ? sh.warp_sum[lane] : 0.0f);
+}
+
+// The sum of a slice whose maximum is m, by its definition: infinities share
+// the weight, NaN has none.
+template <typename T>
+__device__ __noinline__ float sum_by_definition(const Row<T> row, const Allow ok, int32_t j0,
+                                                int32_t j1, bool first, bool last, float m,
+                                                float inv) {
+  float s = 0.0f;
+  for (int32_t t = row.token(j0) + static_cast<int32_t>(threadIdx.x); t < row.token(j1);
+       t += kVerifyThreads)
+    if (ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
+  const int32_t t = row.edge(first, last);
+  if (t >= 0 && ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
+  return s;
+}
+
+// Maximum, its first index (where `first_index`) and the sum over the vectors
+// [j0, j1) and the edges of a row, by the whole CTA. With RACE, each thread's
+// best of x / T - log2(noise) besides.
+template <typename T, bool RACE>
+__device__ Slice scan_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1, bool first,
+                            bool last, float inv, bool first_index, const float* noise,
+                            bool noise_aligned, Best& best, Shared& sh) {
+  constexpr int kEpv = Row<T>::kEpv;
+  constexpr int kUnroll = RACE ? 2 : 4;
+  const float c = inv * kLog2e;
+  float m = -INFINITY, s = 0.0f;
+  int32_t idx = 0;
+  auto race = [&](float x, float e, int32_t t) {
+    const float score = fmaf(x, c, -__log2f(e));
+    if (score > best.score) {
+      best.score = score;
+      best.x = x;
+      best.e = e;
+      best.idx = t;
+    }
+  };
+  for (int32_t j = j0 + static_cast<int32_t>(threadIdx.x); j < j1; j += kUnroll * kVerifyThreads) {
+    uint32_t keep[kUnroll];
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = j + u * kVerifyThreads;
+      keep[u] = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      v[u] = uint4{};
+      if (keep[u]) v[u] = row.vec(j + u * kVerifyThreads);
+    }
+    float x[kUnroll][kEpv], top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < kEpv; ++i) {
+        const float f = Dt<T>::to_float(vec_get<T>(v[u], i));
+        x[u][i] = (keep[u] >> i) & 1u ? f : -INFINITY;
+        top = fmaxf(top, x[u][i]);
+      }
+    if (top > m) {
+      if (first_index) {
+#pragma unroll
+        for (int u = kUnroll - 1; u >= 0; --u)
+#pragma unroll
+          for (int i = kEpv - 1; i >= 0; --i)
+            if (x[u][i] == top) idx = row.token(j + u * kVerifyThreads) + i;
+      }
+      s *= exp2f((m - top) * c);
+      m = top;
+    }
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (keep[u]) {
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) s += exp2f((x[u][i] - m) * c);
+        }
+    }
+    if constexpr (RACE) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (keep[u]) {
+          const int32_t t = row.token(j + u * kVerifyThreads);
+          float e[kEpv];
+          load_floats<kEpv>(noise + t, noise_aligned, e);
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) race(x[u][i], e[i], t + i);
+        }
+    }
+  }
+  const int32_t t = row.edge(first, last);
+  if (t >= 0 && ok.has(t)) {
+    const float x = fmaxf(row.at(t), -INFINITY);
+    if (x > m || (x == m && m > -INFINITY && t < idx)) idx = t;
+    if (x > m) {
+      s = m > -INFINITY ? fmaf(s, exp2f((m - x) * c), 1.0f) : 1.0f;
+      m = x;
+    } else if (x > -INFINITY) {
+      s += exp2f((x - m) * c);
+    }
+    if constexpr (RACE) race(x, noise[t], t);
+  }
+  const uint64_t k =
+      block_max(m > -INFINITY ? pack_arg(order_key(m), first_index ? idx : 0) : 0, sh);
+  Slice out;
+  out.idx = k ? unpack_idx(k) : -1;
+  out.m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
+  out.s = block_sum(m > -INFINITY ? s * exp2f((m - out.m) * c) : 0.0f, sh);
+  // an infinite maximum, a NaN, or a temperature at either end of its range
+  if (k && !(out.s < INFINITY)) {
+    __syncthreads();
+    out.s = block_sum(sum_by_definition<T>(row, ok, j0, j1, first, last, out.m, inv), sh);
+  }
   return out;
 }
 
@@ -200,43 +389,101 @@ __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
   return pack_arg(__float_as_uint(score > 0.0f ? score : 0.0f), t);
 }
 
-// The two races over tokens [t0, t1). `given`: the draft's row of
-// probabilities, or NULL; `draft`: the token that takes no part (-1: none).
+// The race of max(p - q, 0) / noise over the vectors [j0, j1) and the edges of
+// a row, by the whole CTA: (score, lowest index), 0 where nothing takes part.
+// `draft`: a token that does not (-1: none).
 template <typename T>
-__device__ Race race_slice(const void* row, const Allow& ok, int32_t t0, int32_t t1, float inv,
-                           float m, float rz, const float* noise, const void* given,
-                           int32_t given_dtype, int32_t draft, Shared& sh) {
-  Race r{0, 0};
-  for (int32_t t = t0 + static_cast<int32_t>(threadIdx.x); t < t1; t += kVerifyThreads) {
-    if (!ok.has(t)) continue;
-    const float w = weight(fmaxf(load_logit<T>(row, t), -INFINITY), m, inv);
-    if (!(w > 0.0f)) continue;
-    const float p = w * rz, e = noise[t];
-    const uint64_t a = race_key(p / e, t);
-    r.all = a > r.all ? a : r.all;
-    float left = p;
-    if (given) left = p - load_prob(given, given_dtype, t);
-    if (left > 0.0f && t != draft) {
-      const uint64_t l = race_key(left / e, t);
-      r.left = l > r.left ? l : r.left;
+__device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
+                               bool first, bool last, float inv, float m, float rz,
+                               const float* noise, bool noise_aligned, const Given& given,
+                               int32_t draft, Shared& sh) {
+  constexpr int kEpv = Row<T>::kEpv;
+  const float c = inv * kLog2e;
+  // p - q with full precision, and its score
+  auto exact = [&](int32_t t) -> uint64_t {
+    if (t == draft || !ok.has(t)) return 0;
+    float left = weight(fmaxf(row.at(t), -INFINITY), m, inv) * rz;
+    if (given.p) left -= load_prob(given.p, given.dtype, t);
+    return left > 0.0f ? race_key(left / noise[t], t) : 0;
+  };
+  uint64_t mine = 0;
+  if (m < INFINITY && c < INFINITY) {
+    float best = -1.0f;
+    int32_t idx = -1;
+    constexpr int kUnroll = 2;
+    for (int32_t j = j0 + static_cast<int32_t>(threadIdx.x); j < j1;
+         j += kUnroll * kVerifyThreads) {
+      uint32_t keep[kUnroll];
+      uint4 v[kUnroll];
+      float e[kUnroll][kEpv], q[kUnroll][kEpv];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int32_t i = j + u * kVerifyThreads;
+        keep[u] = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int32_t i = j + u * kVerifyThreads, t = row.token(i);
+        v[u] = uint4{};
+#pragma unroll
+        for (int n = 0; n < kEpv; ++n) {
+          e[u][n] = 1.0f;
+          q[u][n] = 0.0f;
+        }
+        if (keep[u]) {
+          v[u] = row.vec(i);
+          load_floats<kEpv>(noise + t, noise_aligned, e[u]);
+          if (given.p) given.template load<kEpv>(t, q[u]);
+        }
+        if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
+          keep[u] &= ~(1u << (draft - t));
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (keep[u]) {
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) {
+            const float x = Dt<T>::to_float(vec_get<T>(v[u], i));
+            const float left = fmaf(exp2f((x - m) * c), rz, -q[u][i]);
+            const float score = fmaxf(__fdividef(left, e[u][i]), 0.0f);
+            if (((keep[u] >> i) & 1u) && left > 0.0f && score > best) {
+              best = score;
+              idx = row.token(j + u * kVerifyThreads) + i;
+            }
+          }
+        }
+    }
+    if (idx >= 0) mine = exact(idx);
+  } else {
+    for (int32_t t = row.token(j0) + static_cast<int32_t>(threadIdx.x); t < row.token(j1);
+         t += kVerifyThreads) {
+      const uint64_t k = exact(t);
+      mine = k > mine ? k : mine;
     }
   }
-  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  r.left = warp_max_u64(r.left);
-  r.all = warp_max_u64(r.all);
-  if (lane == 0) {
-    sh.warp_key[warp] = r.left;
-    sh.warp_key2[warp] = r.all;
+  const int32_t t = row.edge(first, last);
+  if (t >= 0) {
+    const uint64_t k = exact(t);
+    mine = k > mine ? k : mine;
   }
-  __syncthreads();
-  r.left = warp_max_u64(sh.warp_key[lane < kVerifyWarps ? lane : 0]);
-  r.all = warp_max_u64(sh.warp_key2[lane < kVerifyWarps ? lane : 0]);
-  __syncthreads();
-  return r;
+  return block_max(mine, sh);
+}
+
+// The largest of the cluster's keys; every CTA brings its own in `slot`.
+template <int C>
+__device__ __forceinline__ uint64_t cluster_max(uint64_t k, uint64_t& slot) {
+  if constexpr (C == 1) {
+    return k;
+  } else {
+    const int32_t lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) slot = k;
+    cluster_barrier<C>();
+    return warp_max_u64(peer_u64(peer_shared(&slot, lane < C ? lane : 0)));
+  }
 }
 
 template <typename T, int C>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 3) verify_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
   const uint32_t rank = C == 1 ? 0 : cluster_rank();
   const int32_t b = static_cast<int32_t>(blockIdx.x / C);
@@ -267,8 +514,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   const float heat = a.temperature ? a.temperature[b] : a.temperature_all;
   const bool greedy = !(heat > 0.0f);
   const float inv = greedy ? 1.0f : 1.0f / heat;
-  const int32_t per = ((V + C - 1) / C + 127) / 128 * 128;
-  const int32_t t0 = min(V, static_cast<int32_t>(rank) * per), t1 = min(V, t0 + per);
+  const bool head = rank == 0, tail = rank == C - 1;
   auto draft_at = [&](int32_t i) -> int64_t {
     const int64_t at = static_cast<int64_t>(b) * a.draft_stride + i;
     return a.drafts64 ? static_cast<const int64_t*>(a.drafts)[at]
@@ -279,31 +525,51 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
                ? -1
                : __ldg(a.tok_next + static_cast<int64_t>(s) * V + t);
   };
-  // the states along the drafts
+  // the states along the drafts, each one position ahead
   if (a.bits) {
     if (a.path) {
       for (int32_t i = tid; i <= len; i += kVerifyThreads)
         sh.state[i] = a.path[static_cast<int64_t>(b) * (K + 1) + i];
     } else if (tid == 0) {
-      int32_t s = a.pool[slot];
-      sh.state[0] = s;
-      for (int32_t i = 0; i < len; ++i) sh.state[i + 1] = s = step(s, draft_at(i));
+      sh.state[0] = a.pool[slot];
     }
   }
   __syncthreads();
 
+  const float* noise = a.noise + static_cast<int64_t>(b) * a.noise_stride;
   int32_t n = 0;
   int64_t token = -1;
   float logprob = 0.0f;
   for (;; ++n) {
-    const void* row = static_cast<const typename Dt<T>::Bits*>(a.src) + (first + n) * a.src_stride;
+    const Row<T> row(static_cast<const typename Dt<T>::Bits*>(a.src) + (first + n) * a.src_stride,
+                     V);
+    const int32_t per = (row.vecs + C - 1) / C;
+    const int32_t j0 = min(row.vecs, static_cast<int32_t>(rank) * per), j1 = min(row.vecs, j0 + per);
     Allow ok{nullptr, true};
     if (a.bits) {
       const int32_t s = sh.state[n];
       ok.any = false;
       if (s >= 0 && s < a.num_states) ok.row = a.bits + static_cast<int64_t>(s) * a.wstride;
     }
-    Slice r = scan_slice<T>(row, ok, t0, t1, inv, sh);
+    // what the decision needs comes while the row is scanned
+    const int64_t d = n < len ? draft_at(n) : -1;
+    const bool inside = d >= 0 && d < V;
+    float xd = -INFINITY, qd = 1.0f, uniform = 0.0f;
+    if (n < len) {
+      if (inside && ok.has(static_cast<int32_t>(d))) xd = fmaxf(row.at(d), -INFINITY);
+      if (!greedy) uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + n];
+      if (a.probs && inside)
+        qd = load_prob(a.probs, a.probs_dtype, (pfirst + n) * a.probs_stride + d);
+      if (a.bits && !a.path && tid == 0) sh.state[n + 1] = step(sh.state[n], d);
+    }
+    const bool noise_aligned =
+        (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
+    const bool race_now = n == len && !greedy;
+    Best best;
+    Slice r = race_now ? scan_slice<T, true>(row, ok, j0, j1, head, tail, inv, false, noise,
+                                             noise_aligned, best, sh)
+                       : scan_slice<T, false>(row, ok, j0, j1, head, tail, inv, greedy, noise,
+                                              noise_aligned, best, sh);
     if constexpr (C > 1) {
       Slice& own = sh.slice[n & 1];
       if (tid == 0) own = r;
@@ -313,29 +579,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       r.idx = lane < C ? static_cast<int32_t>(peer_u32(peer + 4)) : -1;
       r.s = __uint_as_float(peer_u32(peer + 8));
       const uint64_t k = warp_max_u64(r.idx < 0 ? 0 : pack_arg(order_key(r.m), r.idx));
-      const int32_t idx = k ? unpack_idx(k) : -1;
-      const float m = k ? load_logit<T>(row, idx) : -INFINITY;
+      const float m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
       r.s = warp_sum(r.idx < 0 ? 0.0f : r.s * weight(r.m, m, inv));
       r.m = m;
-      r.idx = idx;
+      r.idx = k ? unpack_idx(k) : -1;
     }
     if (r.idx < 0) break;  // nothing is allowed here
-    const int64_t d = n < len ? draft_at(n) : -1;
     if (n < len) {
-      bool accept;
-      float xd = -INFINITY;
-      if (d >= 0 && d < V && ok.has(static_cast<int32_t>(d)))
-        xd = fmaxf(load_logit<T>(row, d), -INFINITY);
-      if (greedy) {
-        accept = d == r.idx;
-      } else {
-        const float p = weight(xd, r.m, inv) / r.s;
-        const float q = a.probs && d >= 0 && d < V
-                            ? load_prob(a.probs, a.probs_dtype,
-                                        (pfirst + n) * a.probs_stride + d)
-                            : 1.0f;
-        accept = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + n] * q < p;
-      }
+      const bool accept = greedy ? d == r.idx : uniform * qd < weight(xd, r.m, inv) / r.s;
       if (accept) {
         if (rank == 0 && tid == 0) {
           tokens[n] = d;
@@ -347,26 +598,37 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     if (greedy) {
       token = r.idx;
     } else {
-      const void* given = nullptr;
-      if (n < len && a.probs) {
-        const int64_t at = (pfirst + n) * a.probs_stride;
-        given = static_cast<const char*>(a.probs) + at * (a.probs_dtype == BPD_F32 ? 4 : 2);
+      uint64_t won = 0;
+      if (race_now && r.m < INFINITY) {
+        const float w = best.idx >= 0 ? weight(best.x, r.m, inv) : 0.0f;
+        won = cluster_max<C>(
+            block_max(w > 0.0f ? race_key(w / best.e, best.idx) : 0, sh), sh.race[0]);
+      } else {
+        Given given{nullptr, a.probs_dtype, false};
+        if (n < len && a.probs) {
+          const int32_t size = a.probs_dtype == BPD_F32 ? 4 : 2;
+          const char* p =
+              static_cast<const char*>(a.probs) + (pfirst + n) * a.probs_stride * size;
+          given.p = p;
+          given.aligned =
+              (reinterpret_cast<uintptr_t>(p + row.head * size) & (size == 4 ? 15u : 7u)) == 0;
+        }
+        won = cluster_max<C>(
+            race_slice<T>(row, ok, j0, j1, head, tail, inv, r.m, 1.0f / r.s, noise, noise_aligned,
+                          given, n < len && !a.probs && inside ? static_cast<int32_t>(d) : -1, sh),
+            sh.race[0]);
       }
-      Race w = race_slice<T>(row, ok, t0, t1, inv, r.m, 1.0f / r.s,
-                             a.noise + static_cast<int64_t>(b) * a.noise_stride, given,
-                             a.probs_dtype,
-                             n < len && !a.probs && d >= 0 && d < V ? static_cast<int32_t>(d) : -1,
-                             sh);
-      if constexpr (C > 1) {
-        if (tid == 0) sh.race = w;
-        cluster_barrier<C>();
-        const uint32_t peer = peer_shared(&sh.race, lane < C ? lane : 0);
-        w.left = warp_max_u64(peer_u64(peer));
-        w.all = warp_max_u64(peer_u64(peer + 8));
+      if (!won) {  // nothing left of p - q: the race is over p
+        __syncthreads();
+        won = cluster_max<C>(
+            race_slice<T>(row, ok, j0, j1, head, tail, inv, r.m, 1.0f / r.s, noise, noise_aligned,
+                          Given{nullptr, 0, false}, -1, sh),
+            sh.race[1]);
       }
-      token = unpack_idx(w.left ? w.left : w.all);
+      if (!won) break;  // not for any noise above 0
+      token = unpack_idx(won);
     }
-    const float xt = load_logit<T>(row, token);
+    const float xt = row.at(token);
     logprob = (xt == r.m ? 0.0f : (xt - r.m) * inv) - logf(r.s);
     break;
   }
@@ -456,8 +718,12 @@ extern "C" bpd_status bpd_verify_drafts(
   cudaStream_t st = as_stream(stream);
   return with_dtype(src_dtype, what, [&](auto tag) {
     using T = decltype(tag);
-    const cudaError_t e = batch >= 4 * sm_count() ? launch_verify<T, 1>(a, st)
-                                                  : launch_verify<T, kMaxCluster>(a, st);
+    // enough CTAs to fill the SMs four times over, as far as a cluster reaches
+    const int64_t room = 4 * static_cast<int64_t>(sm_count());
+    const cudaError_t e = batch * 8ll <= room   ? launch_verify<T, 8>(a, st)
+                          : batch * 4ll <= room ? launch_verify<T, 4>(a, st)
+                          : batch * 2ll <= room ? launch_verify<T, 2>(a, st)
+                                                : launch_verify<T, 1>(a, st);
     return e == cudaSuccess ? BPD_OK : fail(BPD_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   });
 }
