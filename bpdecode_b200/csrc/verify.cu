@@ -71,6 +71,7 @@ struct VerifyArgs {
   float* logprobs;
   int32_t* next_out;
   int32_t write_back;
+  int32_t window;  // positions that are scanned before the cluster meets
 };
 
 // What a slice of a row comes to: its maximum, the first index that has it
@@ -81,11 +82,22 @@ struct Slice {
   float s;
 };
 
+// A position: what its decision needs, and what came of it.
+struct Position {
+  float xd, qd, uniform;  // the draft's logit (-inf: rejected) and probability
+  int32_t draft;          // -1: none, or no token of the vocabulary
+  float m, s;             // the whole row's
+  int32_t idx, accept;
+};
+
 struct Shared {
+  uint4 lanes[256];  // for each byte of allow bits, the 16-bit lanes that it keeps
   uint64_t warp_key[kVerifyWarps];
   float warp_sum[kVerifyWarps];
-  Slice slice[2];   // by the position's parity: a neighbour may still read the other
-  uint64_t race[2]; // of two races in turn
+  uint64_t race[2];  // of two races in turn
+  uint32_t bar;      // of a race: what no thread needs to look below
+  Slice slice[BPD_MAX_DRAFTS + 1];
+  Position position[BPD_MAX_DRAFTS + 1];
   int32_t state[BPD_MAX_DRAFTS + 1];
 };
 
@@ -127,6 +139,17 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
+}
+
+// The inverse of order_key.
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // A row's allow bits: every token (no grammar), a row of bits, or nothing.
@@ -242,16 +265,6 @@ struct Given {
   }
 };
 
-// The best of a thread in a race: what it needs to score it again.
-struct Best {
-  float score = -INFINITY, x = 0.0f, e = 1.0f;
-  int32_t idx = -1;
-};
-
-// The inverse of order_key.
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
-}
 
 __device__ __forceinline__ uint64_t block_max(uint64_t k, Shared& sh) {
   const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -285,98 +298,190 @@ __device__ __noinline__ float sum_by_definition(const Row<T> row, const Allow ok
   return s;
 }
 
+// `v` with -inf in the lanes that `keep` leaves out.
+template <typename T>
+__device__ __forceinline__ uint4 masked(const uint4& v, uint32_t keep, const Shared& sh) {
+  if constexpr (sizeof(typename Dt<T>::Bits) == 4) {
+    return make_uint4(keep & 1 ? v.x : 0xFF800000u, keep & 2 ? v.y : 0xFF800000u,
+                      keep & 4 ? v.z : 0xFF800000u, keep & 8 ? v.w : 0xFF800000u);
+  } else {
+    constexpr uint32_t kNone = std::is_same_v<T, __half> ? 0xFC00FC00u : 0xFF80FF80u;
+    const uint4 k = sh.lanes[keep];
+    return make_uint4((v.x & k.x) | (kNone & ~k.x), (v.y & k.y) | (kNone & ~k.y),
+                      (v.z & k.z) | (kNone & ~k.z), (v.w & k.w) | (kNone & ~k.w));
+  }
+}
+
+// The largest element of a vector; NaN only where there is nothing else.
+template <typename T>
+__device__ __forceinline__ float vec_top(const uint4& v) {
+  if constexpr (sizeof(typename Dt<T>::Bits) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                 fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else if constexpr (std::is_same_v<T, __half>) {
+    const __half2* p = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&m);
+    return fmaxf(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+}
+
+// A race's threads share a bar, the best score any of them has found so far:
+// with a bar of its own some lane of a warp nearly always has a new best to
+// look at (45 instructions for each element, against 11). A score has to be
+// over the bar less this much to be looked at, more than all roundings between
+// them, so the winner always is, whatever the order in which the bar rises.
+constexpr float kSlack = 1.0f - 3.0e-5f;
+constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is still compared
+
 // Maximum, its first index (where `first_index`) and the sum over the vectors
-// [j0, j1) and the edges of a row, by the whole CTA. With RACE, each thread's
-// best of x / T - log2(noise) besides.
+// [j0, j1) and the edges of a row, by the whole CTA. With RACE, this thread's
+// best of exp(x / T) / noise goes to `best`, too (-1: none); sh.bar is then
+// order_key(-inf) before the call.
+//
+// A thread's vectors are read one round ahead, their allow bits two rounds.
+// The sum is of exp2(x c - ref) with c = log2(e) / T and ref the rounded m c:
+// one fused multiply-add for each element; what the rounding left off is put
+// right once, at the end.
 template <typename T, bool RACE>
-__device__ Slice scan_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1, bool first,
-                            bool last, float inv, bool first_index, const float* noise,
-                            bool noise_aligned, Best& best, Shared& sh) {
+__device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, int32_t j0,
+                                            int32_t j1, bool first, bool last, float inv,
+                                            bool first_index, const float* noise,
+                                            bool noise_aligned, int32_t& best, Shared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
   constexpr int kUnroll = RACE ? 2 : 4;
+  constexpr int kStride = kUnroll * kVerifyThreads;
   const float c = inv * kLog2e;
-  float m = -INFINITY, s = 0.0f;
-  int32_t idx = 0;
-  auto race = [&](float x, float e, int32_t t) {
-    const float score = fmaf(x, c, -__log2f(e));
-    if (score > best.score) {
-      best.score = score;
-      best.x = x;
-      best.e = e;
-      best.idx = t;
-    }
-  };
-  for (int32_t j = j0 + static_cast<int32_t>(threadIdx.x); j < j1; j += kUnroll * kVerifyThreads) {
+  float m = -INFINITY, ref = 0.0f, s = 0.0f;
+  float score = -INFINITY;  // log2 of this thread's best in the race
+  int32_t idx = 0, from = 0;
+  best = -1;
+  struct Batch {
     uint32_t keep[kUnroll];
     uint4 v[kUnroll];
+    float e[RACE ? kUnroll : 1][kEpv];
+  };
+  auto bits = [&](int32_t j, uint32_t (&keep)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int32_t i = j + u * kVerifyThreads;
       keep[u] = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
     }
+  };
+  auto load = [&](int32_t j, const uint32_t (&keep)[kUnroll], Batch& b) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      v[u] = uint4{};
-      if (keep[u]) v[u] = row.vec(j + u * kVerifyThreads);
+      b.keep[u] = keep[u];
+      if (keep[u]) {
+        b.v[u] = row.vec(j + u * kVerifyThreads);
+        if constexpr (RACE)
+          load_floats<kEpv>(noise + row.token(j + u * kVerifyThreads), noise_aligned, b.e[u]);
+      }
     }
-    float x[kUnroll][kEpv], top = -INFINITY;
+  };
+  auto use = [&](int32_t j, Batch& b) {
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int i = 0; i < kEpv; ++i) {
-        const float f = Dt<T>::to_float(vec_get<T>(v[u], i));
-        x[u][i] = (keep[u] >> i) & 1u ? f : -INFINITY;
-        top = fmaxf(top, x[u][i]);
+      if (b.keep[u]) {
+        b.v[u] = masked<T>(b.v[u], b.keep[u], sh);
+        top = fmaxf(top, vec_top<T>(b.v[u]));
       }
     if (top > m) {
-      if (first_index) {
-#pragma unroll
-        for (int u = kUnroll - 1; u >= 0; --u)
-#pragma unroll
-          for (int i = kEpv - 1; i >= 0; --i)
-            if (x[u][i] == top) idx = row.token(j + u * kVerifyThreads) + i;
-      }
-      s *= exp2f((m - top) * c);
+      const float to = top * c;
+      s *= m > -INFINITY ? exp2_fast(ref - to) : 0.0f;
+      ref = to;
       m = top;
+      from = j;
     }
-    if (m > -INFINITY) {
+    if (!(m > -INFINITY)) return;
+    float bar = 0.0f;
+    if constexpr (RACE)
+      bar = exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - ref) * kSlack;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (keep[u]) {
+    for (int u = 0; u < kUnroll; ++u)
+      if (b.keep[u]) {
+        float w[kEpv];
 #pragma unroll
-          for (int i = 0; i < kEpv; ++i) s += exp2f((x[u][i] - m) * c);
+        for (int i = 0; i < kEpv; ++i) {
+          w[i] = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(b.v[u], i)), c, -ref));
+          s += w[i];
         }
+        if constexpr (RACE) {
+          float over = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) over = fmaxf(over, fmaf(-bar, b.e[u][i], w[i]));
+          if (over > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < kEpv; ++i) {
+              const float f = __log2f(w[i]) + ref - __log2f(b.e[u][i]);
+              if (f > score && w[i] > 0.0f) {
+                score = f;
+                best = row.token(j + u * kVerifyThreads) + i;
+              }
+            }
+            const float rise = fminf(score, ref + __log2f(kMostScore));
+            if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+          }
+        }
+      }
+  };
+  {
+    uint32_t ahead[kUnroll];
+    Batch now;
+    int32_t j = j0 + static_cast<int32_t>(threadIdx.x);
+    bits(j, ahead);
+    load(j, ahead, now);
+    bits(j + kStride, ahead);
+    for (; j < j1; j += kStride) {
+      Batch next;
+      load(j + kStride, ahead, next);
+      bits(j + 2 * kStride, ahead);
+      use(j, now);
+      now = next;
     }
-    if constexpr (RACE) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (keep[u]) {
-          const int32_t t = row.token(j + u * kVerifyThreads);
-          float e[kEpv];
-          load_floats<kEpv>(noise + t, noise_aligned, e);
-#pragma unroll
-          for (int i = 0; i < kEpv; ++i) race(x[u][i], e[i], t + i);
-        }
+  }
+  if (first_index && m > -INFINITY) {
+    // the first maximal token of the round that had it
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = from + u * kVerifyThreads;
+      const uint32_t keep = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
+      int32_t at = -1;
+      for (int n = kEpv - 1; n >= 0; --n)
+        if ((keep >> n) & 1u && row.at(row.token(i) + n) == m) at = row.token(i) + n;
+      if (at >= 0) {
+        idx = at;
+        break;
+      }
     }
   }
   const int32_t t = row.edge(first, last);
   if (t >= 0 && ok.has(t)) {
     const float x = fmaxf(row.at(t), -INFINITY);
-    if (x > m || (x == m && m > -INFINITY && t < idx)) idx = t;
-    if (x > m) {
-      s = m > -INFINITY ? fmaf(s, exp2f((m - x) * c), 1.0f) : 1.0f;
-      m = x;
-    } else if (x > -INFINITY) {
-      s += exp2f((x - m) * c);
+    if (x > -INFINITY) {
+      if (x > m || (x == m && t < idx)) idx = t;
+      if (x > m) {
+        const float to = x * c;
+        s *= m > -INFINITY ? exp2_fast(ref - to) : 0.0f;
+        ref = to;
+        m = x;
+      }
+      const float w = exp2_fast(fmaf(x, c, -ref));
+      s += w;
+      if (RACE && __log2f(w) + ref - __log2f(noise[t]) > score) best = t;
     }
-    if constexpr (RACE) race(x, noise[t], t);
   }
+  s *= exp2_fast(-fmaf(m, c, -ref));  // from ref to m c
   const uint64_t k =
       block_max(m > -INFINITY ? pack_arg(order_key(m), first_index ? idx : 0) : 0, sh);
   Slice out;
   out.idx = k ? unpack_idx(k) : -1;
   out.m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
-  out.s = block_sum(m > -INFINITY ? s * exp2f((m - out.m) * c) : 0.0f, sh);
+  out.s = block_sum(m > -INFINITY ? s * exp2_fast((m - out.m) * c) : 0.0f, sh);
   // an infinite maximum, a NaN, or a temperature at either end of its range
   if (k && !(out.s < INFINITY)) {
     __syncthreads();
@@ -390,7 +495,8 @@ __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
 }
 
 // The race of max(p - q, 0) / noise over the vectors [j0, j1) and the edges of
-// a row, by the whole CTA: (score, lowest index), 0 where nothing takes part.
+// a row, by the whole CTA: (score, lowest index), 0 where nothing takes part;
+// sh.bar is 0 before the call.
 // `draft`: a token that does not (-1: none).
 template <typename T>
 __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
@@ -410,48 +516,58 @@ __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, i
   if (m < INFINITY && c < INFINITY) {
     float best = -1.0f;
     int32_t idx = -1;
-    constexpr int kUnroll = 2;
-    for (int32_t j = j0 + static_cast<int32_t>(threadIdx.x); j < j1;
-         j += kUnroll * kVerifyThreads) {
-      uint32_t keep[kUnroll];
-      uint4 v[kUnroll];
-      float e[kUnroll][kEpv], q[kUnroll][kEpv];
+    const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
+    constexpr int kStride = kVerifyThreads;
+    uint32_t keep = 0, ahead = 0;
+    uint4 v{}, v2{};
+    float e[kEpv] = {}, q[kEpv] = {}, e2[kEpv] = {}, q2[kEpv] = {};
+    auto bits = [&](int32_t i) { return i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u; };
+    auto load = [&](int32_t i, uint32_t k, uint4& vv, float(&ee)[kEpv], float(&qq)[kEpv]) {
+      if (!k) return;
+      vv = row.vec(i);
+      load_floats<kEpv>(noise + row.token(i), noise_aligned, ee);
+      if (given.p) given.template load<kEpv>(row.token(i), qq);
+    };
+    int32_t j = j0 + static_cast<int32_t>(threadIdx.x);
+    keep = bits(j);
+    load(j, keep, v, e, q);
+    ahead = bits(j + kStride);
+    for (; j < j1; j += kStride) {
+      load(j + kStride, ahead, v2, e2, q2);
+      const uint32_t behind = bits(j + 2 * kStride);
+      const int32_t t = row.token(j);
+      if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
+        keep &= ~(1u << (draft - t));
+      if (keep) {
+        const uint4 x = masked<T>(v, keep, sh);
+        const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+        float left[kEpv], over = 0.0f;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int32_t i = j + u * kVerifyThreads;
-        keep[u] = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int32_t i = j + u * kVerifyThreads, t = row.token(i);
-        v[u] = uint4{};
-#pragma unroll
-        for (int n = 0; n < kEpv; ++n) {
-          e[u][n] = 1.0f;
-          q[u][n] = 0.0f;
+        for (int i = 0; i < kEpv; ++i) {
+          const float w = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
+          left[i] = fmaf(w, fix, -q[i]);
+          over = fmaxf(over, fmaf(-bar, e[i], left[i]));
         }
-        if (keep[u]) {
-          v[u] = row.vec(i);
-          load_floats<kEpv>(noise + t, noise_aligned, e[u]);
-          if (given.p) given.template load<kEpv>(t, q[u]);
-        }
-        if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
-          keep[u] &= ~(1u << (draft - t));
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (keep[u]) {
+        if (over > 0.0f) {
 #pragma unroll
           for (int i = 0; i < kEpv; ++i) {
-            const float x = Dt<T>::to_float(vec_get<T>(v[u], i));
-            const float left = fmaf(exp2f((x - m) * c), rz, -q[u][i]);
-            const float score = fmaxf(__fdividef(left, e[u][i]), 0.0f);
-            if (((keep[u] >> i) & 1u) && left > 0.0f && score > best) {
-              best = score;
-              idx = row.token(j + u * kVerifyThreads) + i;
+            const float f = fmaxf(__fdividef(left[i], e[i]), 0.0f);
+            if (left[i] > 0.0f && f > best) {
+              best = f;
+              idx = t + i;
             }
           }
+          if (best > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(best, kMostScore)));
         }
+      }
+      keep = ahead;
+      ahead = behind;
+      v = v2;
+#pragma unroll
+      for (int i = 0; i < kEpv; ++i) {
+        e[i] = e2[i];
+        q[i] = q2[i];
+      }
     }
     if (idx >= 0) mine = exact(idx);
   } else {
@@ -483,7 +599,7 @@ __device__ __forceinline__ uint64_t cluster_max(uint64_t k, uint64_t& slot) {
 }
 
 template <typename T, int C>
-__global__ void __launch_bounds__(kVerifyThreads, 3) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
   const uint32_t rank = C == 1 ? 0 : cluster_rank();
   const int32_t b = static_cast<int32_t>(blockIdx.x / C);
@@ -534,103 +650,156 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_kernel(const VerifyA
       sh.state[0] = a.pool[slot];
     }
   }
+  if (tid == 0) sh.bar = order_key(-INFINITY);
+  if (sizeof(typename Dt<T>::Bits) == 2) {
+    auto two = [&](uint32_t k) { return (k & 1 ? 0xFFFFu : 0u) | (k & 2 ? 0xFFFF0000u : 0u); };
+    for (uint32_t k = tid; k < 256; k += kVerifyThreads)
+      sh.lanes[k] = make_uint4(two(k), two(k >> 2), two(k >> 4), two(k >> 6));
+  }
   __syncthreads();
 
   const float* noise = a.noise + static_cast<int64_t>(b) * a.noise_stride;
-  int32_t n = 0;
-  int64_t token = -1;
-  float logprob = 0.0f;
-  for (;; ++n) {
-    const Row<T> row(static_cast<const typename Dt<T>::Bits*>(a.src) + (first + n) * a.src_stride,
-                     V);
-    const int32_t per = (row.vecs + C - 1) / C;
-    const int32_t j0 = min(row.vecs, static_cast<int32_t>(rank) * per), j1 = min(row.vecs, j0 + per);
+  auto row_of = [&](int32_t i) {
+    return Row<T>(
+        static_cast<const typename Dt<T>::Bits*>(a.src) + (first + i) * a.src_stride, V);
+  };
+  auto allow_of = [&](int32_t i) {
     Allow ok{nullptr, true};
     if (a.bits) {
-      const int32_t s = sh.state[n];
+      const int32_t s = sh.state[i];
       ok.any = false;
       if (s >= 0 && s < a.num_states) ok.row = a.bits + static_cast<int64_t>(s) * a.wstride;
     }
-    // what the decision needs comes while the row is scanned
-    const int64_t d = n < len ? draft_at(n) : -1;
-    const bool inside = d >= 0 && d < V;
-    float xd = -INFINITY, qd = 1.0f, uniform = 0.0f;
-    if (n < len) {
-      if (inside && ok.has(static_cast<int32_t>(d))) xd = fmaxf(row.at(d), -INFINITY);
-      if (!greedy) uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + n];
-      if (a.probs && inside)
-        qd = load_prob(a.probs, a.probs_dtype, (pfirst + n) * a.probs_stride + d);
-      if (a.bits && !a.path && tid == 0) sh.state[n + 1] = step(sh.state[n], d);
+    return ok;
+  };
+  auto part_of = [&](const Row<T>& row, int32_t& j0, int32_t& j1) {
+    const int32_t per = (row.vecs + C - 1) / C;
+    j0 = min(row.vecs, static_cast<int32_t>(rank) * per);
+    j1 = min(row.vecs, j0 + per);
+  };
+  auto noise_fits = [&](const Row<T>& row) {
+    return (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
+  };
+  int32_t best = -1;  // of the last row's race
+  int32_t n = 0;      // the first position that is not an accepted draft
+  for (int32_t begin = 0;; begin += a.window) {
+    const int32_t end = min(begin + a.window, len + 1);
+    for (int32_t i = begin; i < end; ++i) {
+      const Row<T> row = row_of(i);
+      const Allow ok = allow_of(i);
+      int32_t j0, j1;
+      part_of(row, j0, j1);
+      // what the decision needs comes while the row is scanned
+      const int64_t d = i < len ? draft_at(i) : -1;
+      const bool inside = d >= 0 && d < V;
+      float xd = -INFINITY, qd = 1.0f, uniform = 0.0f;
+      int32_t next = -1;
+      if (i < len) {
+        if (inside && ok.has(static_cast<int32_t>(d))) xd = fmaxf(row.at(d), -INFINITY);
+        if (!greedy) uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + i];
+        if (a.probs && inside)
+          qd = load_prob(a.probs, a.probs_dtype, (pfirst + i) * a.probs_stride + d);
+        if (a.bits && !a.path) next = step(sh.state[i], d);
+      }
+      const Slice r =
+          i == len && !greedy
+              ? scan_slice<T, true>(row, ok, j0, j1, head, tail, inv, false, noise,
+                                    noise_fits(row), best, sh)
+              : scan_slice<T, false>(row, ok, j0, j1, head, tail, inv, greedy, noise, false, best,
+                                     sh);
+      if (tid == 0) {
+        sh.slice[i] = r;
+        Position& p = sh.position[i];
+        p.xd = xd;
+        p.qd = qd;
+        p.uniform = uniform;
+        p.draft = inside ? static_cast<int32_t>(d) : -1;
+        if (i < len && a.bits && !a.path) sh.state[i + 1] = next;
+      }
+      __syncthreads();
     }
-    const bool noise_aligned =
-        (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
-    const bool race_now = n == len && !greedy;
-    Best best;
-    Slice r = race_now ? scan_slice<T, true>(row, ok, j0, j1, head, tail, inv, false, noise,
-                                             noise_aligned, best, sh)
-                       : scan_slice<T, false>(row, ok, j0, j1, head, tail, inv, greedy, noise,
-                                              noise_aligned, best, sh);
-    if constexpr (C > 1) {
-      Slice& own = sh.slice[n & 1];
-      if (tid == 0) own = r;
-      cluster_barrier<C>();
-      const uint32_t peer = peer_shared(&own, lane < C ? lane : 0);
-      r.m = __uint_as_float(peer_u32(peer));
-      r.idx = lane < C ? static_cast<int32_t>(peer_u32(peer + 4)) : -1;
-      r.s = __uint_as_float(peer_u32(peer + 8));
-      const uint64_t k = warp_max_u64(r.idx < 0 ? 0 : pack_arg(order_key(r.m), r.idx));
-      const float m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
-      r.s = warp_sum(r.idx < 0 ? 0.0f : r.s * weight(r.m, m, inv));
-      r.m = m;
-      r.idx = k ? unpack_idx(k) : -1;
-    }
-    if (r.idx < 0) break;  // nothing is allowed here
-    if (n < len) {
-      const bool accept = greedy ? d == r.idx : uniform * qd < weight(xd, r.m, inv) / r.s;
-      if (accept) {
-        if (rank == 0 && tid == 0) {
-          tokens[n] = d;
-          logprobs[n] = (xd == r.m ? 0.0f : (xd - r.m) * inv) - logf(r.s);
-        }
-        continue;
+    cluster_barrier<C>();
+    // a warp puts a position's slices together and decides on it
+    for (int32_t i = begin + (tid >> 5); i < end; i += kVerifyWarps) {
+      Position& p = sh.position[i];
+      Slice r;
+      const uint32_t peer = C > 1 ? peer_shared(&sh.slice[i], lane < C ? lane : 0) : 0;
+      if constexpr (C > 1) {
+        r.m = __uint_as_float(peer_u32(peer));
+        r.idx = lane < C ? static_cast<int32_t>(peer_u32(peer + 4)) : -1;
+        r.s = __uint_as_float(peer_u32(peer + 8));
+        const uint64_t k = warp_max_u64(r.idx < 0 ? 0 : pack_arg(order_key(r.m), r.idx));
+        const float m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
+        r.s = warp_sum(r.idx < 0 ? 0.0f : r.s * weight(r.m, m, inv));
+        r.m = m;
+        r.idx = k ? unpack_idx(k) : -1;
+      } else {
+        r = sh.slice[i];
+      }
+      if (lane == 0) {
+        p.m = r.m;
+        p.s = r.s;
+        p.idx = r.idx;
+        p.accept = i < len && r.idx >= 0 &&
+                   (greedy ? p.draft == r.idx
+                           : p.uniform * p.qd < weight(p.xd, r.m, inv) / r.s);
       }
     }
+    __syncthreads();
+    for (n = begin; n < end && sh.position[n].accept; ++n) {
+      if (rank == 0 && tid == 0) {
+        const Position& p = sh.position[n];
+        tokens[n] = p.draft;
+        logprobs[n] = (p.xd == p.m ? 0.0f : (p.xd - p.m) * inv) - logf(p.s);
+      }
+    }
+    if (n < end) break;
+  }
+  const Position p = sh.position[n];
+  int64_t token = -1;
+  float logprob = 0.0f;
+  if (p.idx >= 0) {  // else nothing is allowed here
+    const Row<T> row = row_of(n);
     if (greedy) {
-      token = r.idx;
+      token = p.idx;
     } else {
+      const Allow ok = allow_of(n);
+      int32_t j0, j1;
+      part_of(row, j0, j1);
       uint64_t won = 0;
-      if (race_now && r.m < INFINITY) {
-        const float w = best.idx >= 0 ? weight(best.x, r.m, inv) : 0.0f;
-        won = cluster_max<C>(
-            block_max(w > 0.0f ? race_key(w / best.e, best.idx) : 0, sh), sh.race[0]);
+      if (tid == 0) sh.bar = 0;
+      __syncthreads();
+      if (n == len && p.m < INFINITY) {
+        const float w = best >= 0 ? weight(row.at(best), p.m, inv) : 0.0f;
+        won = block_max(w > 0.0f ? race_key(w / noise[best], best) : 0, sh);
       } else {
         Given given{nullptr, a.probs_dtype, false};
         if (n < len && a.probs) {
           const int32_t size = a.probs_dtype == BPD_F32 ? 4 : 2;
-          const char* p =
-              static_cast<const char*>(a.probs) + (pfirst + n) * a.probs_stride * size;
-          given.p = p;
+          const char* q = static_cast<const char*>(a.probs) + (pfirst + n) * a.probs_stride * size;
+          given.p = q;
           given.aligned =
-              (reinterpret_cast<uintptr_t>(p + row.head * size) & (size == 4 ? 15u : 7u)) == 0;
+              (reinterpret_cast<uintptr_t>(q + row.head * size) & (size == 4 ? 15u : 7u)) == 0;
         }
-        won = cluster_max<C>(
-            race_slice<T>(row, ok, j0, j1, head, tail, inv, r.m, 1.0f / r.s, noise, noise_aligned,
-                          given, n < len && !a.probs && inside ? static_cast<int32_t>(d) : -1, sh),
-            sh.race[0]);
+        won = race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
+                            noise_fits(row), given, n < len && !a.probs ? p.draft : -1, sh);
       }
+      won = cluster_max<C>(won, sh.race[0]);
       if (!won) {  // nothing left of p - q: the race is over p
         __syncthreads();
+        if (tid == 0) sh.bar = 0;
+        __syncthreads();
         won = cluster_max<C>(
-            race_slice<T>(row, ok, j0, j1, head, tail, inv, r.m, 1.0f / r.s, noise, noise_aligned,
-                          Given{nullptr, 0, false}, -1, sh),
+            race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
+                          noise_fits(row), Given{nullptr, 0, false}, -1, sh),
             sh.race[1]);
       }
-      if (!won) break;  // not for any noise above 0
-      token = unpack_idx(won);
+      if (won) token = unpack_idx(won);
     }
-    const float xt = row.at(token);
-    logprob = (xt == r.m ? 0.0f : (xt - r.m) * inv) - logf(r.s);
-    break;
+    if (token >= 0) {
+      const float xt = row.at(token);
+      logprob = (xt == p.m ? 0.0f : (xt - p.m) * inv) - logf(p.s);
+    }
   }
   if (rank == 0) {
     for (int32_t i = n + tid; i <= K; i += kVerifyThreads) {
@@ -714,10 +883,15 @@ extern "C" bpd_status bpd_verify_drafts(
                uniform_stride, noise, noise_stride, temperature, temperature_all, batch,
                max_drafts, vocab_size, state_pool, slots, path, allow_bits, words_stride,
                allow_bits ? tok_next : nullptr, num_states, tokens_out, counts_out, logprobs_out,
-               next_out, write_back};
+               next_out, write_back, 1};
   cudaStream_t st = as_stream(stream);
   return with_dtype(src_dtype, what, [&](auto tag) {
     using T = decltype(tag);
+    // Positions are scanned ahead of the decisions where all rows are few
+    // enough to be read in less time than the cluster takes to meet.
+    const int64_t rows_bytes = static_cast<int64_t>(batch) * (max_drafts + 1) * vocab_size *
+                               static_cast<int64_t>(sizeof(typename Dt<T>::Bits));
+    a.window = rows_bytes <= (100ll << 20) ? max_drafts + 1 : 1;
     // enough CTAs to fill the SMs four times over, as far as a cluster reaches
     const int64_t room = 4 * static_cast<int64_t>(sm_count());
     const cudaError_t e = batch * 8ll <= room   ? launch_verify<T, 8>(a, st)
