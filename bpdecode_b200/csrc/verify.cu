@@ -27,6 +27,7 @@
 // precision, so that only scores within one thread are compared in fast
 // arithmetic.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -38,6 +39,13 @@ constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kMaxCluster = 8;
+// Bytes of shared memory for each thread's loads on their way: eight vectors of
+// logits, or four with their noise, or two with noise and probabilities.
+constexpr int kRingBytes = 192;
+#ifndef LB
+#define LB 4
+#endif
+constexpr int kCtasPerSm = LB;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyArgs {
@@ -184,9 +192,7 @@ struct Row {
   }
   __device__ __forceinline__ float at(int64_t t) const { return Dt<T>::to_float(p[t]); }
   __device__ __forceinline__ int32_t token(int32_t vec) const { return head + vec * kEpv; }
-  __device__ __forceinline__ uint4 vec(int32_t j) const {
-    return __ldg(reinterpret_cast<const uint4*>(p + head) + j);
-  }
+  __device__ __forceinline__ const Bits* vec_at(int32_t j) const { return p + token(j); }
   // the token outside the vectors that this thread looks at, or -1
   __device__ __forceinline__ int32_t edge(bool first, bool last) const {
     const int32_t i = threadIdx.x, tail = head + vecs * kEpv;
@@ -214,21 +220,51 @@ __device__ __forceinline__ float load_prob(const void* row, int32_t dtype, int64
   return load_logit<__half>(row, t);
 }
 
-// N consecutive values from p on, as fp32.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ uint4 shared_vec(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+// This thread's places in the ring: 16 bytes beside its neighbours'.
+constexpr uint32_t kPlane = kVerifyThreads * 16;
+
+// N consecutive floats from p on, to the planes from `dst` on.
 template <int N>
-__device__ __forceinline__ void load_floats(const float* p, bool aligned, float (&out)[N]) {
+__device__ __forceinline__ void copy_floats(uint32_t dst, const float* p, bool aligned) {
   if (aligned) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i));
-      out[i] = f.x;
-      out[i + 1] = f.y;
-      out[i + 2] = f.z;
-      out[i + 3] = f.w;
-    }
+    for (int i = 0; i < N; i += 4) copy_async<16>(dst + i / 4 * kPlane, p + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = __ldg(p + i);
+    for (int i = 0; i < N; ++i) copy_async<4>(dst + i / 4 * kPlane + i % 4 * 4, p + i);
+  }
+}
+template <int N>
+__device__ __forceinline__ void read_floats(uint32_t src, float (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint4 v = shared_vec(src + i / 4 * kPlane);
+    out[i] = __uint_as_float(v.x);
+    out[i + 1] = __uint_as_float(v.y);
+    out[i + 2] = __uint_as_float(v.z);
+    out[i + 3] = __uint_as_float(v.w);
   }
 }
 
@@ -236,35 +272,94 @@ __device__ __forceinline__ void load_floats(const float* p, bool aligned, float 
 struct Given {
   const void* p;
   int32_t dtype;
-  bool aligned;  // its vectors begin where the logits' do, on 16 (8) bytes
+  bool aligned;  // its vectors begin where the logits' do, on as many bytes as a copy has
+  // N probabilities from token t on, on their way to the planes from dst on
+  // (fp32: always; 16 bits: where aligned)
   template <int N>
-  __device__ __forceinline__ void load(int32_t t, float (&out)[N]) const {
+  __device__ __forceinline__ void copy(uint32_t dst, int32_t t) const {
+    if (!p) return;
+    if (dtype == BPD_F32)
+      copy_floats<N>(dst, static_cast<const float*>(p) + t, aligned);
+    else if (aligned)
+      copy_async<N * 2>(dst, static_cast<const uint16_t*>(p) + t);
+  }
+  template <int N>
+  __device__ __forceinline__ void read(uint32_t src, int32_t t, float (&out)[N]) const {
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[i] = 0.0f;
+      return;
+    }
     if (dtype == BPD_F32) {
-      load_floats<N>(static_cast<const float*>(p) + t, aligned, out);
+      read_floats<N>(src, out);
+      return;
+    }
+    uint32_t w[N / 2];
+    if (aligned) {
+      const uint4 v = shared_vec(src);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) w[i] = vec_word(v, i);
     } else {
       const uint16_t* h = static_cast<const uint16_t*>(p) + t;
-      uint32_t w[N / 2];
-      if (aligned) {
 #pragma unroll
-        for (int i = 0; i < N / 2; i += 2) {
-          const uint2 u = __ldcs(reinterpret_cast<const uint2*>(h + 2 * i));
-          w[i] = u.x;
-          w[i + 1] = u.y;
-        }
-      } else {
+      for (int i = 0; i < N / 2; ++i)
+        w[i] = __ldg(h + 2 * i) | static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16;
+    }
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-          w[i] = __ldg(h + 2 * i) | static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16;
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint16_t u = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
-        out[i] = dtype == BPD_BF16 ? Dt<__nv_bfloat16>::to_float(u) : Dt<__half>::to_float(u);
-      }
+    for (int i = 0; i < N; ++i) {
+      const uint16_t u = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+      out[i] = dtype == BPD_BF16 ? Dt<__nv_bfloat16>::to_float(u) : Dt<__half>::to_float(u);
     }
   }
 };
 
+// Streams the vectors [j0, j1) of a row through the CTA, DEPTH of them on
+// their way for each thread at any time: start(slot, vector) begins the copies
+// of a vector that keeps a token, use(slot, vector, keep) takes it. Registers
+// hold none of what is on its way (kept in registers, two rounds ahead, the
+// same loop ran at a third of the rate). Allow bits are read DEPTH + 2 rounds
+// ahead of their use; a thread reads what it copied itself, so there is no
+// barrier.
+template <typename T, int DEPTH, typename Start, typename Use>
+__device__ __forceinline__ void stream(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
+                                       Start&& start, Use&& use) {
+  constexpr int kEpv = Row<T>::kEpv;
+  const int32_t rounds = (j1 - j0 + kVerifyThreads - 1) / kVerifyThreads;
+  const int32_t mine = j0 + static_cast<int32_t>(threadIdx.x);
+  auto bits = [&](int32_t r) -> uint32_t {
+    const int32_t j = mine + r * kVerifyThreads;
+    return r < rounds && j < j1 ? ok.template bits<kEpv>(row.token(j)) : 0u;
+  };
+  uint64_t keeps = 0;  // 8 bits for each slot, the next one lowest
+  {
+    uint32_t k[DEPTH];
+#pragma unroll
+    for (int r = 0; r < DEPTH; ++r) k[r] = bits(r);
+#pragma unroll
+    for (int r = 0; r < DEPTH; ++r) {
+      if (k[r]) start(r, mine + r * kVerifyThreads);
+      copy_commit();
+      keeps |= static_cast<uint64_t>(k[r]) << (8 * r);
+    }
+  }
+  auto turn = [&](int32_t r, uint32_t& ahead) {
+    copy_wait<DEPTH - 1>();
+    const int32_t slot = r & (DEPTH - 1), j = mine + r * kVerifyThreads;
+    const uint32_t keep = static_cast<uint32_t>(keeps) & 255u;
+    if (keep) use(slot, j, keep);
+    if (ahead) start(slot, j + DEPTH * kVerifyThreads);
+    copy_commit();
+    keeps = keeps >> 8 | static_cast<uint64_t>(ahead) << (8 * (DEPTH - 1));
+    ahead = bits(r + DEPTH + 2);
+  };
+  // two in turn: a copy from one to the other would wait for its load
+  uint32_t even = bits(DEPTH), odd = bits(DEPTH + 1);
+  for (int32_t r = 0; r < rounds; r += 2) {
+    turn(r, even);
+    if (r + 1 < rounds) turn(r + 1, odd);
+  }
+  copy_wait<0>();
+}
 
 __device__ __forceinline__ uint64_t block_max(uint64_t k, Shared& sh) {
   const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -343,7 +438,6 @@ constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is st
 // best of exp(x / T) / noise goes to `best`, too (-1: none); sh.bar is then
 // order_key(-inf) before the call.
 //
-// A thread's vectors are read one round ahead, their allow bits two rounds.
 // The sum is of exp2(x c - ref) with c = log2(e) / T and ref the rounded m c:
 // one fused multiply-add for each element; what the rounding left off is put
 // right once, at the end.
@@ -351,46 +445,24 @@ template <typename T, bool RACE>
 __device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, int32_t j0,
                                             int32_t j1, bool first, bool last, float inv,
                                             bool first_index, const float* noise,
-                                            bool noise_aligned, int32_t& best, Shared& sh) {
+                                            bool noise_aligned, int32_t& best, uint32_t ring, Shared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
-  constexpr int kUnroll = RACE ? 2 : 4;
-  constexpr int kStride = kUnroll * kVerifyThreads;
   const float c = inv * kLog2e;
   float m = -INFINITY, ref = 0.0f, s = 0.0f;
   float score = -INFINITY;  // log2 of this thread's best in the race
   int32_t idx = 0, from = 0;
   best = -1;
-  struct Batch {
-    uint32_t keep[kUnroll];
-    uint4 v[kUnroll];
-    float e[RACE ? kUnroll : 1][kEpv];
+  constexpr int kDepth = RACE ? 4 : 8;
+  constexpr uint32_t kSlot = (RACE ? 1 + kEpv / 4 : 1) * kPlane;
+  static_assert(kDepth * kSlot <= kRingBytes * kVerifyThreads, "the ring holds every slot");
+  auto start = [&](int32_t slot, int32_t j) {
+    copy_async<16>(ring + slot * kSlot, row.vec_at(j));
+    if constexpr (RACE)
+      copy_floats<kEpv>(ring + slot * kSlot + kPlane, noise + row.token(j), noise_aligned);
   };
-  auto bits = [&](int32_t j, uint32_t (&keep)[kUnroll]) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int32_t i = j + u * kVerifyThreads;
-      keep[u] = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
-    }
-  };
-  auto load = [&](int32_t j, const uint32_t (&keep)[kUnroll], Batch& b) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      b.keep[u] = keep[u];
-      if (keep[u]) {
-        b.v[u] = row.vec(j + u * kVerifyThreads);
-        if constexpr (RACE)
-          load_floats<kEpv>(noise + row.token(j + u * kVerifyThreads), noise_aligned, b.e[u]);
-      }
-    }
-  };
-  auto use = [&](int32_t j, Batch& b) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (b.keep[u]) {
-        b.v[u] = masked<T>(b.v[u], b.keep[u], sh);
-        top = fmaxf(top, vec_top<T>(b.v[u]));
-      }
+  auto use = [&](int32_t slot, int32_t j, uint32_t keep) {
+    const uint4 v = masked<T>(shared_vec(ring + slot * kSlot), keep, sh);
+    const float top = vec_top<T>(v);
     if (top > m) {
       const float to = top * c;
       s *= m > -INFINITY ? exp2_fast(ref - to) : 0.0f;
@@ -399,65 +471,39 @@ __device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, 
       from = j;
     }
     if (!(m > -INFINITY)) return;
-    float bar = 0.0f;
-    if constexpr (RACE)
-      bar = exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - ref) * kSlack;
+    float w[kEpv];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (b.keep[u]) {
-        float w[kEpv];
+    for (int i = 0; i < kEpv; ++i) {
+      w[i] = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(v, i)), c, -ref));
+      s += w[i];
+    }
+    if constexpr (RACE) {
+      const float bar =
+          exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - ref) * kSlack;
+      float e[kEpv], over = 0.0f;
+      read_floats<kEpv>(ring + slot * kSlot + kPlane, e);
+#pragma unroll
+      for (int i = 0; i < kEpv; ++i) over = fmaxf(over, fmaf(-bar, e[i], w[i]));
+      if (over > 0.0f) {
 #pragma unroll
         for (int i = 0; i < kEpv; ++i) {
-          w[i] = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(b.v[u], i)), c, -ref));
-          s += w[i];
-        }
-        if constexpr (RACE) {
-          float over = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kEpv; ++i) over = fmaxf(over, fmaf(-bar, b.e[u][i], w[i]));
-          if (over > 0.0f) {
-#pragma unroll
-            for (int i = 0; i < kEpv; ++i) {
-              const float f = __log2f(w[i]) + ref - __log2f(b.e[u][i]);
-              if (f > score && w[i] > 0.0f) {
-                score = f;
-                best = row.token(j + u * kVerifyThreads) + i;
-              }
-            }
-            const float rise = fminf(score, ref + __log2f(kMostScore));
-            if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+          const float f = __log2f(w[i]) + ref - __log2f(e[i]);
+          if (f > score && w[i] > 0.0f) {
+            score = f;
+            best = row.token(j) + i;
           }
         }
+        const float rise = fminf(score, ref + __log2f(kMostScore));
+        if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
       }
+    }
   };
-  {
-    uint32_t ahead[kUnroll];
-    Batch now;
-    int32_t j = j0 + static_cast<int32_t>(threadIdx.x);
-    bits(j, ahead);
-    load(j, ahead, now);
-    bits(j + kStride, ahead);
-    for (; j < j1; j += kStride) {
-      Batch next;
-      load(j + kStride, ahead, next);
-      bits(j + 2 * kStride, ahead);
-      use(j, now);
-      now = next;
-    }
-  }
+  stream<T, kDepth>(row, ok, j0, j1, start, use);
   if (first_index && m > -INFINITY) {
-    // the first maximal token of the round that had it
-    for (int u = 0; u < kUnroll; ++u) {
-      const int32_t i = from + u * kVerifyThreads;
-      const uint32_t keep = i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u;
-      int32_t at = -1;
-      for (int n = kEpv - 1; n >= 0; --n)
-        if ((keep >> n) & 1u && row.at(row.token(i) + n) == m) at = row.token(i) + n;
-      if (at >= 0) {
-        idx = at;
-        break;
-      }
-    }
+    // the first maximal token of the vector that had it
+    const uint32_t keep = ok.template bits<kEpv>(row.token(from));
+    for (int i = kEpv - 1; i >= 0; --i)
+      if ((keep >> i) & 1u && row.at(row.token(from) + i) == m) idx = row.token(from) + i;
   }
   const int32_t t = row.edge(first, last);
   if (t >= 0 && ok.has(t)) {
@@ -502,7 +548,7 @@ template <typename T>
 __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
                                bool first, bool last, float inv, float m, float rz,
                                const float* noise, bool noise_aligned, const Given& given,
-                               int32_t draft, Shared& sh) {
+                               int32_t draft, uint32_t ring, Shared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
   const float c = inv * kLog2e;
   // p - q with full precision, and its score
@@ -517,58 +563,43 @@ __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, i
     float best = -1.0f;
     int32_t idx = -1;
     const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
-    constexpr int kStride = kVerifyThreads;
-    uint32_t keep = 0, ahead = 0;
-    uint4 v{}, v2{};
-    float e[kEpv] = {}, q[kEpv] = {}, e2[kEpv] = {}, q2[kEpv] = {};
-    auto bits = [&](int32_t i) { return i < j1 ? ok.template bits<kEpv>(row.token(i)) : 0u; };
-    auto load = [&](int32_t i, uint32_t k, uint4& vv, float(&ee)[kEpv], float(&qq)[kEpv]) {
-      if (!k) return;
-      vv = row.vec(i);
-      load_floats<kEpv>(noise + row.token(i), noise_aligned, ee);
-      if (given.p) given.template load<kEpv>(row.token(i), qq);
+    constexpr int kDepth = 2;
+    constexpr uint32_t kNoise = kPlane, kGiven = kPlane * (1 + kEpv / 4),
+                       kSlot = kPlane * (1 + kEpv / 2);
+    static_assert(kDepth * kSlot <= kRingBytes * kVerifyThreads, "the ring holds every slot");
+    auto start = [&](int32_t slot, int32_t j) {
+      copy_async<16>(ring + slot * kSlot, row.vec_at(j));
+      copy_floats<kEpv>(ring + slot * kSlot + kNoise, noise + row.token(j), noise_aligned);
+      given.template copy<kEpv>(ring + slot * kSlot + kGiven, row.token(j));
     };
-    int32_t j = j0 + static_cast<int32_t>(threadIdx.x);
-    keep = bits(j);
-    load(j, keep, v, e, q);
-    ahead = bits(j + kStride);
-    for (; j < j1; j += kStride) {
-      load(j + kStride, ahead, v2, e2, q2);
-      const uint32_t behind = bits(j + 2 * kStride);
+    auto use = [&](int32_t slot, int32_t j, uint32_t keep) {
       const int32_t t = row.token(j);
       if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
         keep &= ~(1u << (draft - t));
-      if (keep) {
-        const uint4 x = masked<T>(v, keep, sh);
-        const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
-        float left[kEpv], over = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kEpv; ++i) {
-          const float w = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
-          left[i] = fmaf(w, fix, -q[i]);
-          over = fmaxf(over, fmaf(-bar, e[i], left[i]));
-        }
-        if (over > 0.0f) {
-#pragma unroll
-          for (int i = 0; i < kEpv; ++i) {
-            const float f = fmaxf(__fdividef(left[i], e[i]), 0.0f);
-            if (left[i] > 0.0f && f > best) {
-              best = f;
-              idx = t + i;
-            }
-          }
-          if (best > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(best, kMostScore)));
-        }
-      }
-      keep = ahead;
-      ahead = behind;
-      v = v2;
+      const uint4 x = masked<T>(shared_vec(ring + slot * kSlot), keep, sh);
+      const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+      float left[kEpv], e[kEpv], over = 0.0f;
+      given.template read<kEpv>(ring + slot * kSlot + kGiven, t, left);
+      read_floats<kEpv>(ring + slot * kSlot + kNoise, e);
 #pragma unroll
       for (int i = 0; i < kEpv; ++i) {
-        e[i] = e2[i];
-        q[i] = q2[i];
+        const float w = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
+        left[i] = fmaf(w, fix, -left[i]);
+        over = fmaxf(over, fmaf(-bar, e[i], left[i]));
       }
-    }
+      if (over > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < kEpv; ++i) {
+          const float f = fmaxf(__fdividef(left[i], e[i]), 0.0f);
+          if (left[i] > 0.0f && f > best) {
+            best = f;
+            idx = t + i;
+          }
+        }
+        if (best > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(best, kMostScore)));
+      }
+    };
+    stream<T, kDepth>(row, ok, j0, j1, start, use);
     if (idx >= 0) mine = exact(idx);
   } else {
     for (int32_t t = row.token(j0) + static_cast<int32_t>(threadIdx.x); t < row.token(j1);
@@ -599,8 +630,11 @@ __device__ __forceinline__ uint64_t cluster_max(uint64_t k, uint64_t& slot) {
 }
 
 template <typename T, int C>
-__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(const VerifyArgs a) {
+  extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
+  const uint32_t ring =
+      static_cast<uint32_t>(__cvta_generic_to_shared(dynamic)) + threadIdx.x * 16;
   const uint32_t rank = C == 1 ? 0 : cluster_rank();
   const int32_t b = static_cast<int32_t>(blockIdx.x / C);
   const int32_t tid = threadIdx.x, lane = tid & 31;
@@ -704,9 +738,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
       const Slice r =
           i == len && !greedy
               ? scan_slice<T, true>(row, ok, j0, j1, head, tail, inv, false, noise,
-                                    noise_fits(row), best, sh)
+                                    noise_fits(row), best, ring, sh)
               : scan_slice<T, false>(row, ok, j0, j1, head, tail, inv, greedy, noise, false, best,
-                                     sh);
+                                     ring, sh);
       if (tid == 0) {
         sh.slice[i] = r;
         Position& p = sh.position[i];
@@ -779,10 +813,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
           const char* q = static_cast<const char*>(a.probs) + (pfirst + n) * a.probs_stride * size;
           given.p = q;
           given.aligned =
-              (reinterpret_cast<uintptr_t>(q + row.head * size) & (size == 4 ? 15u : 7u)) == 0;
+              reinterpret_cast<uintptr_t>(q + row.head * size) % min(16, Row<T>::kEpv * size) == 0;
         }
         won = race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
-                            noise_fits(row), given, n < len && !a.probs ? p.draft : -1, sh);
+                            noise_fits(row), given, n < len && !a.probs ? p.draft : -1, ring, sh);
       }
       won = cluster_max<C>(won, sh.race[0]);
       if (!won) {  // nothing left of p - q: the race is over p
@@ -791,7 +825,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
         __syncthreads();
         won = cluster_max<C>(
             race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
-                          noise_fits(row), Given{nullptr, 0, false}, -1, sh),
+                          noise_fits(row), Given{nullptr, 0, false}, -1, ring, sh),
             sh.race[1]);
       }
       if (won) token = unpack_idx(won);
@@ -820,9 +854,19 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
 
 template <typename T, int C>
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st) {
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev].load(std::memory_order_relaxed))) {
+    e = cudaFuncSetAttribute(verify_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kRingBytes * kVerifyThreads);
+    if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * C);
   cfg.blockDim = dim3(kVerifyThreads);
+  cfg.dynamicSmemBytes = kRingBytes * kVerifyThreads;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -833,7 +877,7 @@ cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T, C>, a);
+  e = cudaLaunchKernelEx(&cfg, verify_kernel<T, C>, a);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e;
 }
@@ -893,7 +937,7 @@ extern "C" bpd_status bpd_verify_drafts(
                                static_cast<int64_t>(sizeof(typename Dt<T>::Bits));
     a.window = rows_bytes <= (100ll << 20) ? max_drafts + 1 : 1;
     // enough CTAs to fill the SMs four times over, as far as a cluster reaches
-    const int64_t room = 4 * static_cast<int64_t>(sm_count());
+    const int64_t room = kCtasPerSm * static_cast<int64_t>(sm_count());
     const cudaError_t e = batch * 8ll <= room   ? launch_verify<T, 8>(a, st)
                           : batch * 4ll <= room ? launch_verify<T, 4>(a, st)
                           : batch * 2ll <= room ? launch_verify<T, 2>(a, st)
