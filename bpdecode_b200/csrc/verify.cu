@@ -313,50 +313,74 @@ struct Given {
   }
 };
 
-// Streams the vectors [j0, j1) of a row through the CTA, DEPTH of them on
+// A warp's share of a row: every `step`-th block of 128 vectors from `first` on.
+struct Share {
+  int32_t first, step;
+  bool head, tail;  // whether this CTA looks at the tokens before, behind the vectors
+};
+constexpr int kRounds = 4;  // of a warp in a block, a vector for each lane
+
+// Streams a warp's share of a row through shared memory, DEPTH vectors on
 // their way for each thread at any time: start(slot, vector) begins the copies
-// of a vector that keeps a token, use(slot, vector, keep) takes it. Registers
+// of a vector that keeps a token, use(slot, vector, keep) takes it (also where
+// none is kept and nothing was copied). Registers
 // hold none of what is on its way (kept in registers, two rounds ahead, the
-// same loop ran at a third of the rate). Allow bits are read DEPTH + 2 rounds
-// ahead of their use; a thread reads what it copied itself, so there is no
-// barrier.
+// same loop ran at a third of the rate). A lane reads 32 allow bits of a block,
+// a block ahead of the copies, and the others take theirs from it. A thread
+// reads what it copied itself, so there is no barrier.
 template <typename T, int DEPTH, typename Start, typename Use>
-__device__ __forceinline__ void stream(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
+__device__ __forceinline__ void stream(const Row<T>& row, const Allow& ok, const Share& share,
                                        Start&& start, Use&& use) {
   constexpr int kEpv = Row<T>::kEpv;
-  const int32_t rounds = (j1 - j0 + kVerifyThreads - 1) / kVerifyThreads;
-  const int32_t mine = j0 + static_cast<int32_t>(threadIdx.x);
-  auto bits = [&](int32_t r) -> uint32_t {
-    const int32_t j = mine + r * kVerifyThreads;
-    return r < rounds && j < j1 ? ok.template bits<kEpv>(row.token(j)) : 0u;
+  constexpr int kLanes = 32 / kEpv;       // vectors, and lanes, of a word of bits
+  constexpr int kAhead = DEPTH / kRounds; // whole blocks that a copy is ahead
+  constexpr uint32_t kAllBits = (1u << kEpv) - 1u;
+  static_assert(DEPTH == 2 || DEPTH % kRounds == 0, "copies run two rounds or whole blocks ahead");
+  const int32_t lane = threadIdx.x & 31;
+  const int32_t blocks = (row.vecs + 127) / 128;
+  const int32_t words = (row.V + 31) / 32, shift = row.head & 31;
+  auto bits = [&](int32_t b) -> uint32_t {
+    if (b >= blocks) return 0u;
+    if (!ok.row) return ok.any ? ~0u : 0u;
+    const int32_t w = (row.head >> 5) + b * (4 * kEpv) + (lane & (4 * kEpv - 1));
+    const uint32_t lo = w < words ? __ldg(ok.row + w) : 0u;
+    const uint32_t hi = shift && w + 1 < words ? __ldg(ok.row + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, shift);
   };
-  uint64_t keeps = 0;  // 8 bits for each slot, the next one lowest
-  {
-    uint32_t k[DEPTH];
+  auto keep_of = [&](uint32_t word, int32_t j, int32_t q) -> uint32_t {
+    const uint32_t w = __shfl_sync(kFull, word, q * kEpv + lane / kLanes);
+    return j < row.vecs ? (w >> (lane % kLanes * kEpv)) & kAllBits : 0u;
+  };
+  // words[i]: the bits of the i-th block from the one in use on
+  uint32_t word[kAhead + 2];
 #pragma unroll
-    for (int r = 0; r < DEPTH; ++r) k[r] = bits(r);
+  for (int i = 0; i < kAhead + 2; ++i) word[i] = bits(share.first + i * share.step);
+  int32_t b = share.first;
 #pragma unroll
-    for (int r = 0; r < DEPTH; ++r) {
-      if (k[r]) start(r, mine + r * kVerifyThreads);
-      copy_commit();
-      keeps |= static_cast<uint64_t>(k[r]) << (8 * r);
-    }
-  }
-  auto turn = [&](int32_t r, uint32_t& ahead) {
-    copy_wait<DEPTH - 1>();
-    const int32_t slot = r & (DEPTH - 1), j = mine + r * kVerifyThreads;
-    const uint32_t keep = static_cast<uint32_t>(keeps) & 255u;
-    if (keep) use(slot, j, keep);
-    if (ahead) start(slot, j + DEPTH * kVerifyThreads);
+  for (int r = 0; r < DEPTH; ++r) {
+    const int32_t j = (b + r / kRounds * share.step) * 128 + r % kRounds * 32 + lane;
+    if (keep_of(word[r / kRounds], j, r % kRounds)) start(r, j);
     copy_commit();
-    keeps = keeps >> 8 | static_cast<uint64_t>(ahead) << (8 * (DEPTH - 1));
-    ahead = bits(r + DEPTH + 2);
-  };
-  // two in turn: a copy from one to the other would wait for its load
-  uint32_t even = bits(DEPTH), odd = bits(DEPTH + 1);
-  for (int32_t r = 0; r < rounds; r += 2) {
-    turn(r, even);
-    if (r + 1 < rounds) turn(r + 1, odd);
+  }
+  int32_t slot0 = 0;
+  for (; b < blocks; b += share.step) {
+    const uint32_t behind = bits(b + (kAhead + 2) * share.step);
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
+      const int32_t slot = DEPTH > kRounds ? slot0 + q : q & (DEPTH - 1);
+      copy_wait<DEPTH - 1>();
+      const int32_t j = b * 128 + q * 32 + lane;
+      use(slot, j, keep_of(word[0], j, q));
+      constexpr int kOver = DEPTH % kRounds;
+      const int next = kAhead + (q + kOver) / kRounds, nq = (q + kOver) % kRounds;
+      const int32_t nj = (b + next * share.step) * 128 + nq * 32 + lane;
+      if (keep_of(word[next], nj, nq)) start(slot, nj);
+      copy_commit();
+    }
+    if (DEPTH > kRounds) slot0 = (slot0 + kRounds) & (DEPTH - 1);
+#pragma unroll
+    for (int i = 0; i <= kAhead; ++i) word[i] = word[i + 1];
+    word[kAhead + 1] = behind;
   }
   copy_wait<0>();
 }
@@ -378,18 +402,27 @@ __device__ __forceinline__ float block_sum(float s, Shared& sh) {
   return warp_sum(lane < kVerifyWarps ? sh.warp_sum[lane] : 0.0f);
 }
 
+// Calls f for each token of this thread's share, one by one.
+template <typename T, typename F>
+__device__ __forceinline__ void each_token(const Row<T>& row, const Share& share, F&& f) {
+  constexpr int kTokens = 128 * Row<T>::kEpv;
+  const int32_t end = row.token(row.vecs);
+  for (int32_t b = share.first; b * 128 < row.vecs; b += share.step)
+    for (int32_t i = threadIdx.x & 31; i < kTokens && row.token(b * 128) + i < end; i += 32)
+      f(row.token(b * 128) + i);
+  const int32_t t = row.edge(share.head, share.tail);
+  if (t >= 0) f(t);
+}
+
 // The sum of a slice whose maximum is m, by its definition: infinities share
 // the weight, NaN has none.
 template <typename T>
-__device__ __noinline__ float sum_by_definition(const Row<T> row, const Allow ok, int32_t j0,
-                                                int32_t j1, bool first, bool last, float m,
-                                                float inv) {
+__device__ __noinline__ float sum_by_definition(const Row<T> row, const Allow ok, const Share share,
+                                                float m, float inv) {
   float s = 0.0f;
-  for (int32_t t = row.token(j0) + static_cast<int32_t>(threadIdx.x); t < row.token(j1);
-       t += kVerifyThreads)
+  each_token(row, share, [&](int32_t t) {
     if (ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
-  const int32_t t = row.edge(first, last);
-  if (t >= 0 && ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
+  });
   return s;
 }
 
@@ -433,8 +466,8 @@ __device__ __forceinline__ float vec_top(const uint4& v) {
 constexpr float kSlack = 1.0f - 3.0e-5f;
 constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is still compared
 
-// Maximum, its first index (where `first_index`) and the sum over the vectors
-// [j0, j1) and the edges of a row, by the whole CTA. With RACE, this thread's
+// Maximum, its first index (where `first_index`) and the sum over the CTA's
+// share of a row. With RACE, this thread's
 // best of exp(x / T) / noise goes to `best`, too (-1: none); sh.bar is then
 // order_key(-inf) before the call.
 //
@@ -442,9 +475,9 @@ constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is st
 // one fused multiply-add for each element; what the rounding left off is put
 // right once, at the end.
 template <typename T, bool RACE>
-__device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, int32_t j0,
-                                            int32_t j1, bool first, bool last, float inv,
-                                            bool first_index, const float* noise,
+__device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok,
+                                            const Share& share, float inv, bool first_index,
+                                            const float* noise,
                                             bool noise_aligned, int32_t& best, uint32_t ring, Shared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
   const float c = inv * kLog2e;
@@ -470,8 +503,7 @@ __device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, 
       m = top;
       from = j;
     }
-    if (!(m > -INFINITY)) return;
-    float w[kEpv];
+    float w[kEpv];  // ref is 0 as long as there is nothing but -inf: weights of 0
 #pragma unroll
     for (int i = 0; i < kEpv; ++i) {
       w[i] = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(v, i)), c, -ref));
@@ -498,14 +530,14 @@ __device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, 
       }
     }
   };
-  stream<T, kDepth>(row, ok, j0, j1, start, use);
+  stream<T, kDepth>(row, ok, share, start, use);
   if (first_index && m > -INFINITY) {
     // the first maximal token of the vector that had it
     const uint32_t keep = ok.template bits<kEpv>(row.token(from));
     for (int i = kEpv - 1; i >= 0; --i)
       if ((keep >> i) & 1u && row.at(row.token(from) + i) == m) idx = row.token(from) + i;
   }
-  const int32_t t = row.edge(first, last);
+  const int32_t t = row.edge(share.head, share.tail);
   if (t >= 0 && ok.has(t)) {
     const float x = fmaxf(row.at(t), -INFINITY);
     if (x > -INFINITY) {
@@ -531,7 +563,7 @@ __device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok, 
   // an infinite maximum, a NaN, or a temperature at either end of its range
   if (k && !(out.s < INFINITY)) {
     __syncthreads();
-    out.s = block_sum(sum_by_definition<T>(row, ok, j0, j1, first, last, out.m, inv), sh);
+    out.s = block_sum(sum_by_definition<T>(row, ok, share, out.m, inv), sh);
   }
   return out;
 }
@@ -540,15 +572,13 @@ __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
   return pack_arg(__float_as_uint(score > 0.0f ? score : 0.0f), t);
 }
 
-// The race of max(p - q, 0) / noise over the vectors [j0, j1) and the edges of
-// a row, by the whole CTA: (score, lowest index), 0 where nothing takes part;
-// sh.bar is 0 before the call.
-// `draft`: a token that does not (-1: none).
+// The race of max(p - q, 0) / noise over the CTA's share of a row: (score,
+// lowest index), 0 where nothing takes part; sh.bar is 0 before the call.
+// `draft`: a token that takes no part (-1: none).
 template <typename T>
-__device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, int32_t j1,
-                               bool first, bool last, float inv, float m, float rz,
-                               const float* noise, bool noise_aligned, const Given& given,
-                               int32_t draft, uint32_t ring, Shared& sh) {
+__device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, const Share& share, float inv,
+                               float m, float rz, const float* noise, bool noise_aligned,
+                               const Given& given, int32_t draft, uint32_t ring, Shared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
   const float c = inv * kLog2e;
   // p - q with full precision, and its score
@@ -573,6 +603,7 @@ __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, i
       given.template copy<kEpv>(ring + slot * kSlot + kGiven, row.token(j));
     };
     auto use = [&](int32_t slot, int32_t j, uint32_t keep) {
+      if (!keep) return;  // nothing was copied
       const int32_t t = row.token(j);
       if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
         keep &= ~(1u << (draft - t));
@@ -599,19 +630,18 @@ __device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, int32_t j0, i
         if (best > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(best, kMostScore)));
       }
     };
-    stream<T, kDepth>(row, ok, j0, j1, start, use);
+    stream<T, kDepth>(row, ok, share, start, use);
     if (idx >= 0) mine = exact(idx);
-  } else {
-    for (int32_t t = row.token(j0) + static_cast<int32_t>(threadIdx.x); t < row.token(j1);
-         t += kVerifyThreads) {
+    const int32_t t = row.edge(share.head, share.tail);
+    if (t >= 0) {
       const uint64_t k = exact(t);
       mine = k > mine ? k : mine;
     }
-  }
-  const int32_t t = row.edge(first, last);
-  if (t >= 0) {
-    const uint64_t k = exact(t);
-    mine = k > mine ? k : mine;
+  } else {
+    each_token(row, share, [&](int32_t t) {
+      const uint64_t k = exact(t);
+      mine = k > mine ? k : mine;
+    });
   }
   return block_max(mine, sh);
 }
@@ -664,7 +694,8 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
   const float heat = a.temperature ? a.temperature[b] : a.temperature_all;
   const bool greedy = !(heat > 0.0f);
   const float inv = greedy ? 1.0f : 1.0f / heat;
-  const bool head = rank == 0, tail = rank == C - 1;
+  const Share share{static_cast<int32_t>(rank) * kVerifyWarps + (tid >> 5), C * kVerifyWarps,
+                    rank == 0, rank == C - 1};
   auto draft_at = [&](int32_t i) -> int64_t {
     const int64_t at = static_cast<int64_t>(b) * a.draft_stride + i;
     return a.drafts64 ? static_cast<const int64_t*>(a.drafts)[at]
@@ -706,11 +737,6 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
     }
     return ok;
   };
-  auto part_of = [&](const Row<T>& row, int32_t& j0, int32_t& j1) {
-    const int32_t per = (row.vecs + C - 1) / C;
-    j0 = min(row.vecs, static_cast<int32_t>(rank) * per);
-    j1 = min(row.vecs, j0 + per);
-  };
   auto noise_fits = [&](const Row<T>& row) {
     return (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   };
@@ -721,8 +747,6 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
     for (int32_t i = begin; i < end; ++i) {
       const Row<T> row = row_of(i);
       const Allow ok = allow_of(i);
-      int32_t j0, j1;
-      part_of(row, j0, j1);
       // what the decision needs comes while the row is scanned
       const int64_t d = i < len ? draft_at(i) : -1;
       const bool inside = d >= 0 && d < V;
@@ -737,9 +761,9 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
       }
       const Slice r =
           i == len && !greedy
-              ? scan_slice<T, true>(row, ok, j0, j1, head, tail, inv, false, noise,
+              ? scan_slice<T, true>(row, ok, share, inv, false, noise,
                                     noise_fits(row), best, ring, sh)
-              : scan_slice<T, false>(row, ok, j0, j1, head, tail, inv, greedy, noise, false, best,
+              : scan_slice<T, false>(row, ok, share, inv, greedy, noise, false, best,
                                      ring, sh);
       if (tid == 0) {
         sh.slice[i] = r;
@@ -798,8 +822,6 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
       token = p.idx;
     } else {
       const Allow ok = allow_of(n);
-      int32_t j0, j1;
-      part_of(row, j0, j1);
       uint64_t won = 0;
       if (tid == 0) sh.bar = 0;
       __syncthreads();
@@ -815,7 +837,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
           given.aligned =
               reinterpret_cast<uintptr_t>(q + row.head * size) % min(16, Row<T>::kEpv * size) == 0;
         }
-        won = race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
+        won = race_slice<T>(row, ok, share, inv, p.m, 1.0f / p.s, noise,
                             noise_fits(row), given, n < len && !a.probs ? p.draft : -1, ring, sh);
       }
       won = cluster_max<C>(won, sh.race[0]);
@@ -824,7 +846,7 @@ __global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(cons
         if (tid == 0) sh.bar = 0;
         __syncthreads();
         won = cluster_max<C>(
-            race_slice<T>(row, ok, j0, j1, head, tail, inv, p.m, 1.0f / p.s, noise,
+            race_slice<T>(row, ok, share, inv, p.m, 1.0f / p.s, noise,
                           noise_fits(row), Given{nullptr, 0, false}, -1, ring, sh),
             sh.race[1]);
       }
