@@ -79,7 +79,8 @@ _SIGNATURES: dict[str, tuple[object, list]] = {
                                 _I32, _P, _I32, _P, _I32, _I64, _P, _P]),
     "bpd_verify_drafts": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I32, _I64, _P, _P, _I32, _I64,
                                  _I64, _P, _P, _I64, _P, _I64, _P, _F, _I32, _I32, _I32, _P, _P,
-                                 _P, _P, _I32, _P, _I32, _P, _P, _P, _P, _I32, _P]),
+                                 _P, _P, _I32, _P, _I32, _P, _P, _P, _P, _I32, _P, _P]),
+    "bpd_verify_workspace_bytes": (_S, [_I32, _I32]),
     "bpd_serving_turnover": (_I32, [_I32, C.c_uint64, _P, _F, _F, _F, _I32, _I32, _P, _P, _P, _P,
                                     _P, _P, _P, _P, _P, _P, _P]),
     "bpd_serving_gather_tokens": (_I32, [_I32, _P, _P, _P, _P, _P, _P, _P]),

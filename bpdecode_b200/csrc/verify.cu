@@ -15,19 +15,23 @@
 // greedy: d_i is accepted iff it is the first maximal token, which also
 // replaces it.
 //
-// One cluster of CTAs works through one request, position after position, so
-// rows behind the first refused draft are never read. Each CTA scans a slice
-// of the row once in 16-byte vectors, with a running maximum and sum, leaving
-// out vectors whose tokens are all rejected; the slices' (m, argmax, s) meet
-// through distributed shared memory in a fixed order, so a result does not
-// depend on timing. Behind the last draft the race runs in that same pass, on
-// x / T - log e, which needs neither m nor Z. A row whose draft was refused is
-// scanned a second time (from L2) with the noise and the draft's
-// probabilities. What a thread finds best is then scored again with full
-// precision, so that only scores within one thread are compared in fast
-// arithmetic.
+// Up to three launches. walk_kernel: the states along the drafts, and what the
+// decisions need besides the rows. scan_kernel: the drafts' rows, one CTA for a
+// chunk of a row, in one pass with a running maximum and sum. The CTA of a row
+// that finishes last puts the chunks together and decides; CTAs are ordered by
+// position, and those of a row behind a refused draft leave at once, so in a
+// large batch few of these rows are read. last_kernel: the row that decides
+// the last token. Behind the last draft it is scanned and raced in one pass, on
+// w / e, which needs no Z; a row whose draft was refused is passed over a
+// second time, with the noise and the draft's probabilities. No CTA waits for
+// another.
+//
+// All are bound by HBM; few requests by the loads that depend on one another
+// (state, allow bits, logits). What a thread finds best in a race is scored
+// again with full precision, so only scores within one thread are compared in
+// fast arithmetic. Nothing depends on the order in which CTAs run: chunks meet
+// in a fixed order, and a race takes the maximum of (score, lowest index).
 #include <algorithm>
-#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -36,16 +40,17 @@ namespace bpd {
 namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
-constexpr int kVerifyThreads = 256;
-constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kMaxCluster = 8;
-// Bytes of shared memory for each thread's loads on their way: eight vectors of
-// logits, or four with their noise, or two with noise and probabilities.
-constexpr int kRingBytes = 192;
-#ifndef LB
-#define LB 4
+constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
+constexpr int kMaxChunks = 32;  // of a row
+#ifndef SC
+#define SC 5
+#define LC 4
+#define CW 8
+#define LW 8
+#define RV 2
 #endif
-constexpr int kCtasPerSm = LB;
+constexpr int kScanCtas = SC, kLastCtas = LC;  // on an SM
+constexpr int kRaceVecs = RV;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyArgs {
@@ -79,75 +84,42 @@ struct VerifyArgs {
   float* logprobs;
   int32_t* next_out;
   int32_t write_back;
-  int32_t window;  // positions that are scanned before the cluster meets
 };
 
-// What a slice of a row comes to: its maximum, the first index that has it
-// (-1: nothing allowed), and the sum of exp((x - m) / T).
-struct Slice {
-  float m;
-  int32_t idx;
-  float s;
-};
-
-// A position: what its decision needs, and what came of it.
+// What walk_kernel leaves for a position: its state, the draft (-1: none, or
+// no token of the vocabulary) with its logit (-inf: rejected) and probability,
+// and the uniform number.
 struct Position {
-  float xd, qd, uniform;  // the draft's logit (-inf: rejected) and probability
-  int32_t draft;          // -1: none, or no token of the vocabulary
-  float m, s;             // the whole row's
-  int32_t idx, accept;
+  int32_t state, draft;
+  float xd, qd, uniform;
+  uint32_t arrived;  // chunks of the row that are done
+  // the whole row: maximum, its first index (-1: nothing is allowed) and sum
+  float m, s;
+  int32_t idx;
 };
 
-struct Shared {
-  uint4 lanes[256];  // for each byte of allow bits, the 16-bit lanes that it keeps
-  uint64_t warp_key[kVerifyWarps];
-  float warp_sum[kVerifyWarps];
-  uint64_t race[2];  // of two races in turn
-  uint32_t bar;      // of a race: what no thread needs to look below
-  Slice slice[BPD_MAX_DRAFTS + 1];
-  Position position[BPD_MAX_DRAFTS + 1];
-  int32_t state[BPD_MAX_DRAFTS + 1];
+// A chunk of a row: maximum, its first index, the sum of exp((x - m) / T); and
+// its best in the race.
+struct Part {
+  float m, s;
+  int32_t idx;
+  int32_t best;
+  float x, e;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
+struct Request {
+  int32_t len;       // -1: idle
+  int32_t end;       // the first position that is not an accepted draft
+  uint32_t arrived;  // chunks of its row that are done
+  uint32_t pad;
+  unsigned long long race;  // its winner so far
+};
 
-// A barrier over the cluster's threads (over the CTA's where it has one CTA).
-template <int C>
-__device__ __forceinline__ void cluster_barrier() {
-  if constexpr (C == 1) {
-    __syncthreads();
-  } else {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-  }
-}
-
-// The address of `p` (this CTA's shared memory) in the cluster's CTA `rank`.
-__device__ __forceinline__ uint32_t peer_shared(const void* p, uint32_t rank) {
-  uint32_t a;
-  const uint32_t own = static_cast<uint32_t>(__cvta_generic_to_shared(p));
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(own), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ uint32_t peer_u32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint64_t peer_u64(uint32_t a) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  return v;
-}
+struct Workspace {
+  Request* request;    // [batch]
+  Position* position;  // [batch, K + 1]
+  Part* part;          // [batch, K + 1, kMaxChunks]
+};
 
 // The inverse of order_key.
 __device__ __forceinline__ float key_value(uint32_t k) {
@@ -160,45 +132,137 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two fp32 values, one instruction for both.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ void split(const Pair& p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
 // A row's allow bits: every token (no grammar), a row of bits, or nothing.
 struct Allow {
   const uint32_t* row;  // NULL: see `any`
   bool any;
+  __device__ __forceinline__ Allow(const VerifyArgs& a, int32_t state) : row(nullptr), any(!a.bits) {
+    if (a.bits && state >= 0 && state < a.num_states)
+      row = a.bits + static_cast<int64_t>(state) * a.wstride;
+  }
   __device__ __forceinline__ bool has(int32_t t) const {
     return row ? ((__ldg(row + (t >> 5)) >> (t & 31)) & 1u) : any;
   }
-  // the bits of N tokens from t on, all of them inside the vocabulary
-  template <int N>
-  __device__ __forceinline__ uint32_t bits(int32_t t) const {
-    constexpr uint32_t all = (1u << N) - 1u;
-    if (!row) return any ? all : 0u;
-    const int32_t w = t >> 5, sh = t & 31;
-    const uint32_t lo = __ldg(row + w), hi = sh + N > 32 ? __ldg(row + w + 1) : 0u;
-    return __funnelshift_r(lo, hi, sh) & all;
-  }
 };
 
-// A row of logits as 16-byte vectors: `head` tokens, `vecs` vectors, a tail.
+// A row of logits as 16-byte vectors: `head` tokens, `vecs` vectors, a tail;
+// in blocks of 128 vectors, four for each lane of a warp.
 template <typename T>
 struct Row {
   static constexpr int kEpv = Dt<T>::kPerVec;
   using Bits = typename Dt<T>::Bits;
   const Bits* p;
-  int32_t head, vecs, V;
-  __device__ Row(const void* row, int32_t V_) : p(static_cast<const Bits*>(row)), V(V_) {
-    const uintptr_t off = reinterpret_cast<uintptr_t>(row) & 15u;
-    head = min(V, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
-    vecs = (V - head) / kEpv;
+  int32_t head, vecs;
+  __device__ Row(const VerifyArgs& a, int64_t row)
+      : p(static_cast<const Bits*>(a.src) + row * a.src_stride) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    head = min(a.V, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
+    vecs = (a.V - head) / kEpv;
   }
   __device__ __forceinline__ float at(int64_t t) const { return Dt<T>::to_float(p[t]); }
   __device__ __forceinline__ int32_t token(int32_t vec) const { return head + vec * kEpv; }
-  __device__ __forceinline__ const Bits* vec_at(int32_t j) const { return p + token(j); }
-  // the token outside the vectors that this thread looks at, or -1
-  __device__ __forceinline__ int32_t edge(bool first, bool last) const {
-    const int32_t i = threadIdx.x, tail = head + vecs * kEpv;
-    if (first && i < head) return i;
-    if (last && i >= 32 && i - 32 < V - tail) return tail + i - 32;
-    return -1;
+  __device__ __forceinline__ uint4 vec(int32_t j) const {
+    return __ldg(reinterpret_cast<const uint4*>(p + head) + j);
+  }
+  // Brings block b to L2, if a fair share of its vectors keep a token, and its
+  // noise: in 128-byte lines, a lane for each.
+  __device__ __forceinline__ void warm(int32_t b, uint32_t word, const float* noise) const {
+    uint32_t marks = word | word >> 1 | word >> 2 | word >> 3;
+    if (kEpv == 8) marks |= marks >> 4;
+    const uint32_t mine = threadIdx.x & 31u, words = 4 * kEpv;
+    const uint32_t kept = __reduce_add_sync(
+        kFull, mine < words ? __popc(marks & (kEpv == 8 ? 0x01010101u : 0x11111111u)) : 0);
+    if (kept < 32) return;
+    const int32_t j = b * 128;
+    const uint8_t* at = reinterpret_cast<const uint8_t*>(p + token(j)) + mine * 128;
+    if (mine < 16 && static_cast<int32_t>(mine) * 8 < vecs - j)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+    if (noise) {
+      const int32_t t = token(j) + static_cast<int32_t>(mine) * 32;
+      if (mine < words && t < token(vecs)) asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + t));
+    }
+  }
+  // the blocks [first, end) of chunk c of n
+  __device__ __forceinline__ void chunk(int32_t c, int32_t n, int32_t& first, int32_t& end) const {
+    const int32_t blocks = (vecs + 127) / 128;
+    first = static_cast<int32_t>(static_cast<int64_t>(blocks) * c / n);
+    end = static_cast<int32_t>(static_cast<int64_t>(blocks) * (c + 1) / n);
+  }
+  // This lane's 32 (or 16) allow bits of block b: lane l has word l, of 32
+  // tokens; 0 behind the vectors.
+  __device__ __forceinline__ uint32_t bits(const Allow& ok, int32_t b, int32_t V) const {
+    constexpr int kLanes = 32 / kEpv;  // vectors of a word
+    const int32_t l = threadIdx.x & (4 * kEpv - 1);
+    const int32_t have = vecs - b * 128 - l * kLanes;  // vectors from here on
+    if (have <= 0) return 0u;
+    uint32_t w = ok.any ? ~0u : 0u;
+    if (ok.row) {
+      const int32_t at = (head >> 5) + b * (4 * kEpv) + l, shift = head & 31;
+      const uint32_t lo = __ldg(ok.row + at);
+      const uint32_t hi = shift && at + 1 < (V + 31) / 32 ? __ldg(ok.row + at + 1) : 0u;
+      w = __funnelshift_r(lo, hi, shift);
+    }
+    return have < kLanes ? w & ((1u << have * kEpv) - 1u) : w;
+  }
+  // From the lanes' words, the bits of this lane's vector q of four.
+  __device__ __forceinline__ static uint32_t keep(uint32_t word, int32_t q) {
+    constexpr int kLanes = 32 / kEpv;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t w = __shfl_sync(kFull, word, q * kEpv + lane / kLanes);
+    return (w >> (lane % kLanes * kEpv)) & ((1u << kEpv) - 1u);
+  }
+  // Calls f for the tokens around the vectors, by one warp of the first and
+  // last chunk.
+  template <typename F>
+  __device__ __forceinline__ void edges(int32_t c, int32_t n, int32_t V, F&& f) const {
+    const int32_t i = threadIdx.x, tail = token(vecs);
+    if (c == 0 && i < head) f(i);
+    if (c == n - 1 && i >= 32 && i - 32 < V - tail) f(tail + i - 32);
+  }
+  // Calls f for each token of this thread's share of chunk c, one by one.
+  template <typename F>
+  __device__ __forceinline__ void each(int32_t c, int32_t n, int32_t V, F&& f) const {
+    int32_t first, end;
+    chunk(c, n, first, end);
+    const int32_t last = min(token(vecs), token(end * 128));
+    for (int32_t t = token(first * 128) + static_cast<int32_t>(threadIdx.x); t < last;
+         t += kScanThreads)
+      f(t);
+    edges(c, n, V, f);
   }
 };
 
@@ -209,98 +273,62 @@ __device__ __forceinline__ float weight(float x, float m, float inv) {
   return x > -INFINITY ? expf((x - m) * inv) : 0.0f;
 }
 
-template <typename T>
-__device__ __forceinline__ float load_logit(const void* row, int64_t t) {
-  return Dt<T>::to_float(static_cast<const typename Dt<T>::Bits*>(row)[t]);
-}
-
 __device__ __forceinline__ float load_prob(const void* row, int32_t dtype, int64_t t) {
   if (dtype == BPD_F32) return static_cast<const float*>(row)[t];
-  if (dtype == BPD_BF16) return load_logit<__nv_bfloat16>(row, t);
-  return load_logit<__half>(row, t);
+  const uint16_t u = static_cast<const uint16_t*>(row)[t];
+  return dtype == BPD_BF16 ? Dt<__nv_bfloat16>::to_float(u) : Dt<__half>::to_float(u);
 }
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-__device__ __forceinline__ uint4 shared_vec(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
-}
-
-// This thread's places in the ring: 16 bytes beside its neighbours'.
-constexpr uint32_t kPlane = kVerifyThreads * 16;
-
-// N consecutive floats from p on, to the planes from `dst` on.
+// N consecutive floats from p on.
 template <int N>
-__device__ __forceinline__ void copy_floats(uint32_t dst, const float* p, bool aligned) {
+__device__ __forceinline__ void load_floats(const float* p, bool aligned, float (&out)[N]) {
   if (aligned) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) copy_async<16>(dst + i / 4 * kPlane, p + i);
+    for (int i = 0; i < N; i += 4) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i));
+      out[i] = f.x;
+      out[i + 1] = f.y;
+      out[i + 2] = f.z;
+      out[i + 3] = f.w;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) copy_async<4>(dst + i / 4 * kPlane + i % 4 * 4, p + i);
-  }
-}
-template <int N>
-__device__ __forceinline__ void read_floats(uint32_t src, float (&out)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const uint4 v = shared_vec(src + i / 4 * kPlane);
-    out[i] = __uint_as_float(v.x);
-    out[i + 1] = __uint_as_float(v.y);
-    out[i + 2] = __uint_as_float(v.z);
-    out[i + 3] = __uint_as_float(v.w);
+    for (int i = 0; i < N; ++i) out[i] = __ldg(p + i);
   }
 }
 
 // A row of the draft's probabilities (p == NULL: none).
 struct Given {
-  const void* p;
+  const uint8_t* p;
   int32_t dtype;
-  bool aligned;  // its vectors begin where the logits' do, on as many bytes as a copy has
-  // N probabilities from token t on, on their way to the planes from dst on
-  // (fp32: always; 16 bits: where aligned)
+  __device__ __forceinline__ int32_t size() const { return dtype == BPD_F32 ? 4 : 2; }
+  // whether N from token t on can be read as whole vectors
   template <int N>
-  __device__ __forceinline__ void copy(uint32_t dst, int32_t t) const {
-    if (!p) return;
-    if (dtype == BPD_F32)
-      copy_floats<N>(dst, static_cast<const float*>(p) + t, aligned);
-    else if (aligned)
-      copy_async<N * 2>(dst, static_cast<const uint16_t*>(p) + t);
+  __device__ __forceinline__ bool fits(int32_t t) const {
+    return reinterpret_cast<uintptr_t>(p + t * static_cast<int64_t>(size())) %
+               min(16, N * size()) == 0;
   }
   template <int N>
-  __device__ __forceinline__ void read(uint32_t src, int32_t t, float (&out)[N]) const {
-    if (!p) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) out[i] = 0.0f;
-      return;
-    }
+  __device__ __forceinline__ void load(int32_t t, bool aligned, float (&out)[N]) const {
     if (dtype == BPD_F32) {
-      read_floats<N>(src, out);
+      load_floats<N>(reinterpret_cast<const float*>(p) + t, aligned, out);
       return;
     }
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + t;
     uint32_t w[N / 2];
     if (aligned) {
-      const uint4 v = shared_vec(src);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) w[i] = vec_word(v, i);
+      if constexpr (N == 8) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(h));
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+      } else {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2*>(h));
+        w[0] = v.x;
+        w[1] = v.y;
+      }
     } else {
-      const uint16_t* h = static_cast<const uint16_t*>(p) + t;
 #pragma unroll
       for (int i = 0; i < N / 2; ++i)
         w[i] = __ldg(h + 2 * i) | static_cast<uint32_t>(__ldg(h + 2 * i + 1)) << 16;
@@ -313,134 +341,50 @@ struct Given {
   }
 };
 
-// A warp's share of a row: every `step`-th block of 128 vectors from `first` on.
-struct Share {
-  int32_t first, step;
-  bool head, tail;  // whether this CTA looks at the tokens before, behind the vectors
+// For each byte of allow bits, the 16-bit lanes of a vector that it keeps.
+struct Lanes {
+  uint4 of[256];
+  __device__ __forceinline__ void fill() {
+    auto two = [](uint32_t k) { return (k & 1 ? 0xFFFFu : 0u) | (k & 2 ? 0xFFFF0000u : 0u); };
+    for (uint32_t k = threadIdx.x; k < 256; k += kScanThreads)
+      of[k] = make_uint4(two(k), two(k >> 2), two(k >> 4), two(k >> 6));
+  }
 };
-constexpr int kRounds = 4;  // of a warp in a block, a vector for each lane
-
-// Streams a warp's share of a row through shared memory, DEPTH vectors on
-// their way for each thread at any time: start(slot, vector) begins the copies
-// of a vector that keeps a token, use(slot, vector, keep) takes it (also where
-// none is kept and nothing was copied). Registers
-// hold none of what is on its way (kept in registers, two rounds ahead, the
-// same loop ran at a third of the rate). A lane reads 32 allow bits of a block,
-// a block ahead of the copies, and the others take theirs from it. A thread
-// reads what it copied itself, so there is no barrier.
-template <typename T, int DEPTH, typename Start, typename Use>
-__device__ __forceinline__ void stream(const Row<T>& row, const Allow& ok, const Share& share,
-                                       Start&& start, Use&& use) {
-  constexpr int kEpv = Row<T>::kEpv;
-  constexpr int kLanes = 32 / kEpv;       // vectors, and lanes, of a word of bits
-  constexpr int kAhead = DEPTH / kRounds; // whole blocks that a copy is ahead
-  constexpr uint32_t kAllBits = (1u << kEpv) - 1u;
-  static_assert(DEPTH == 2 || DEPTH % kRounds == 0, "copies run two rounds or whole blocks ahead");
-  const int32_t lane = threadIdx.x & 31;
-  const int32_t blocks = (row.vecs + 127) / 128;
-  const int32_t words = (row.V + 31) / 32, shift = row.head & 31;
-  auto bits = [&](int32_t b) -> uint32_t {
-    if (b >= blocks) return 0u;
-    if (!ok.row) return ok.any ? ~0u : 0u;
-    const int32_t w = (row.head >> 5) + b * (4 * kEpv) + (lane & (4 * kEpv - 1));
-    const uint32_t lo = w < words ? __ldg(ok.row + w) : 0u;
-    const uint32_t hi = shift && w + 1 < words ? __ldg(ok.row + w + 1) : 0u;
-    return __funnelshift_r(lo, hi, shift);
-  };
-  auto keep_of = [&](uint32_t word, int32_t j, int32_t q) -> uint32_t {
-    const uint32_t w = __shfl_sync(kFull, word, q * kEpv + lane / kLanes);
-    return j < row.vecs ? (w >> (lane % kLanes * kEpv)) & kAllBits : 0u;
-  };
-  // words[i]: the bits of the i-th block from the one in use on
-  uint32_t word[kAhead + 2];
-#pragma unroll
-  for (int i = 0; i < kAhead + 2; ++i) word[i] = bits(share.first + i * share.step);
-  int32_t b = share.first;
-#pragma unroll
-  for (int r = 0; r < DEPTH; ++r) {
-    const int32_t j = (b + r / kRounds * share.step) * 128 + r % kRounds * 32 + lane;
-    if (keep_of(word[r / kRounds], j, r % kRounds)) start(r, j);
-    copy_commit();
-  }
-  int32_t slot0 = 0;
-  for (; b < blocks; b += share.step) {
-    const uint32_t behind = bits(b + (kAhead + 2) * share.step);
-#pragma unroll
-    for (int q = 0; q < kRounds; ++q) {
-      const int32_t slot = DEPTH > kRounds ? slot0 + q : q & (DEPTH - 1);
-      copy_wait<DEPTH - 1>();
-      const int32_t j = b * 128 + q * 32 + lane;
-      use(slot, j, keep_of(word[0], j, q));
-      constexpr int kOver = DEPTH % kRounds;
-      const int next = kAhead + (q + kOver) / kRounds, nq = (q + kOver) % kRounds;
-      const int32_t nj = (b + next * share.step) * 128 + nq * 32 + lane;
-      if (keep_of(word[next], nj, nq)) start(slot, nj);
-      copy_commit();
-    }
-    if (DEPTH > kRounds) slot0 = (slot0 + kRounds) & (DEPTH - 1);
-#pragma unroll
-    for (int i = 0; i <= kAhead; ++i) word[i] = word[i + 1];
-    word[kAhead + 1] = behind;
-  }
-  copy_wait<0>();
-}
-
-__device__ __forceinline__ uint64_t block_max(uint64_t k, Shared& sh) {
-  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  k = warp_max_u64(k);
-  if (lane == 0) sh.warp_key[warp] = k;
-  __syncthreads();
-  k = warp_max_u64(sh.warp_key[lane & (kVerifyWarps - 1)]);
-  return k;
-}
-// Between this and block_max there is a barrier in each call order used here.
-__device__ __forceinline__ float block_sum(float s, Shared& sh) {
-  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  s = warp_sum(s);
-  if (lane == 0) sh.warp_sum[warp] = s;
-  __syncthreads();
-  return warp_sum(lane < kVerifyWarps ? sh.warp_sum[lane] : 0.0f);
-}
-
-// Calls f for each token of this thread's share, one by one.
-template <typename T, typename F>
-__device__ __forceinline__ void each_token(const Row<T>& row, const Share& share, F&& f) {
-  constexpr int kTokens = 128 * Row<T>::kEpv;
-  const int32_t end = row.token(row.vecs);
-  for (int32_t b = share.first; b * 128 < row.vecs; b += share.step)
-    for (int32_t i = threadIdx.x & 31; i < kTokens && row.token(b * 128) + i < end; i += 32)
-      f(row.token(b * 128) + i);
-  const int32_t t = row.edge(share.head, share.tail);
-  if (t >= 0) f(t);
-}
-
-// The sum of a slice whose maximum is m, by its definition: infinities share
-// the weight, NaN has none.
-template <typename T>
-__device__ __noinline__ float sum_by_definition(const Row<T> row, const Allow ok, const Share share,
-                                                float m, float inv) {
-  float s = 0.0f;
-  each_token(row, share, [&](int32_t t) {
-    if (ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
-  });
-  return s;
-}
 
 // `v` with -inf in the lanes that `keep` leaves out.
 template <typename T>
-__device__ __forceinline__ uint4 masked(const uint4& v, uint32_t keep, const Shared& sh) {
+__device__ __forceinline__ uint4 masked(const uint4& v, uint32_t keep, const Lanes& lanes) {
   if constexpr (sizeof(typename Dt<T>::Bits) == 4) {
     return make_uint4(keep & 1 ? v.x : 0xFF800000u, keep & 2 ? v.y : 0xFF800000u,
                       keep & 4 ? v.z : 0xFF800000u, keep & 8 ? v.w : 0xFF800000u);
   } else {
     constexpr uint32_t kNone = std::is_same_v<T, __half> ? 0xFC00FC00u : 0xFF80FF80u;
-    const uint4 k = sh.lanes[keep];
+    const uint4 k = lanes.of[keep];
     return make_uint4((v.x & k.x) | (kNone & ~k.x), (v.y & k.y) | (kNone & ~k.y),
                       (v.z & k.z) | (kNone & ~k.z), (v.w & k.w) | (kNone & ~k.w));
   }
 }
 
-// The largest element of a vector; NaN only where there is nothing else.
+// The larger of each of two vectors' elements, and the largest of a vector's;
+// NaN only where there is nothing else.
+template <typename T>
+__device__ __forceinline__ uint4 vec_max2(const uint4& a, const uint4& b) {
+  uint4 r;
+  if constexpr (sizeof(typename Dt<T>::Bits) == 4) {
+    r.x = __float_as_uint(fmaxf(__uint_as_float(a.x), __uint_as_float(b.x)));
+    r.y = __float_as_uint(fmaxf(__uint_as_float(a.y), __uint_as_float(b.y)));
+    r.z = __float_as_uint(fmaxf(__uint_as_float(a.z), __uint_as_float(b.z)));
+    r.w = __float_as_uint(fmaxf(__uint_as_float(a.w), __uint_as_float(b.w)));
+  } else {
+    using Two = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const Two* p = reinterpret_cast<const Two*>(&a);
+    const Two* q = reinterpret_cast<const Two*>(&b);
+    Two* o = reinterpret_cast<Two*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __hmax2(p[i], q[i]);
+  }
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ float vec_top(const uint4& v) {
   if constexpr (sizeof(typename Dt<T>::Bits) == 4) {
@@ -460,454 +404,602 @@ __device__ __forceinline__ float vec_top(const uint4& v) {
 
 // A race's threads share a bar, the best score any of them has found so far:
 // with a bar of its own some lane of a warp nearly always has a new best to
-// look at (45 instructions for each element, against 11). A score has to be
-// over the bar less this much to be looked at, more than all roundings between
-// them, so the winner always is, whatever the order in which the bar rises.
+// look at. A score has to be over the bar less this much to be looked at, more
+// than all roundings between them, so the winner always is, whatever the order
+// in which the bar rises.
 constexpr float kSlack = 1.0f - 3.0e-5f;
 constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is still compared
-
-// Maximum, its first index (where `first_index`) and the sum over the CTA's
-// share of a row. With RACE, this thread's
-// best of exp(x / T) / noise goes to `best`, too (-1: none); sh.bar is then
-// order_key(-inf) before the call.
-//
-// The sum is of exp2(x c - ref) with c = log2(e) / T and ref the rounded m c:
-// one fused multiply-add for each element; what the rounding left off is put
-// right once, at the end.
-template <typename T, bool RACE>
-__device__ __forceinline__ Slice scan_slice(const Row<T>& row, const Allow& ok,
-                                            const Share& share, float inv, bool first_index,
-                                            const float* noise,
-                                            bool noise_aligned, int32_t& best, uint32_t ring, Shared& sh) {
-  constexpr int kEpv = Row<T>::kEpv;
-  const float c = inv * kLog2e;
-  float m = -INFINITY, ref = 0.0f, s = 0.0f;
-  float score = -INFINITY;  // log2 of this thread's best in the race
-  int32_t idx = 0, from = 0;
-  best = -1;
-  constexpr int kDepth = RACE ? 4 : 8;
-  constexpr uint32_t kSlot = (RACE ? 1 + kEpv / 4 : 1) * kPlane;
-  static_assert(kDepth * kSlot <= kRingBytes * kVerifyThreads, "the ring holds every slot");
-  auto start = [&](int32_t slot, int32_t j) {
-    copy_async<16>(ring + slot * kSlot, row.vec_at(j));
-    if constexpr (RACE)
-      copy_floats<kEpv>(ring + slot * kSlot + kPlane, noise + row.token(j), noise_aligned);
-  };
-  auto use = [&](int32_t slot, int32_t j, uint32_t keep) {
-    const uint4 v = masked<T>(shared_vec(ring + slot * kSlot), keep, sh);
-    const float top = vec_top<T>(v);
-    if (top > m) {
-      const float to = top * c;
-      s *= m > -INFINITY ? exp2_fast(ref - to) : 0.0f;
-      ref = to;
-      m = top;
-      from = j;
-    }
-    float w[kEpv];  // ref is 0 as long as there is nothing but -inf: weights of 0
-#pragma unroll
-    for (int i = 0; i < kEpv; ++i) {
-      w[i] = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(v, i)), c, -ref));
-      s += w[i];
-    }
-    if constexpr (RACE) {
-      const float bar =
-          exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - ref) * kSlack;
-      float e[kEpv], over = 0.0f;
-      read_floats<kEpv>(ring + slot * kSlot + kPlane, e);
-#pragma unroll
-      for (int i = 0; i < kEpv; ++i) over = fmaxf(over, fmaf(-bar, e[i], w[i]));
-      if (over > 0.0f) {
-#pragma unroll
-        for (int i = 0; i < kEpv; ++i) {
-          const float f = __log2f(w[i]) + ref - __log2f(e[i]);
-          if (f > score && w[i] > 0.0f) {
-            score = f;
-            best = row.token(j) + i;
-          }
-        }
-        const float rise = fminf(score, ref + __log2f(kMostScore));
-        if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
-      }
-    }
-  };
-  stream<T, kDepth>(row, ok, share, start, use);
-  if (first_index && m > -INFINITY) {
-    // the first maximal token of the vector that had it
-    const uint32_t keep = ok.template bits<kEpv>(row.token(from));
-    for (int i = kEpv - 1; i >= 0; --i)
-      if ((keep >> i) & 1u && row.at(row.token(from) + i) == m) idx = row.token(from) + i;
-  }
-  const int32_t t = row.edge(share.head, share.tail);
-  if (t >= 0 && ok.has(t)) {
-    const float x = fmaxf(row.at(t), -INFINITY);
-    if (x > -INFINITY) {
-      if (x > m || (x == m && t < idx)) idx = t;
-      if (x > m) {
-        const float to = x * c;
-        s *= m > -INFINITY ? exp2_fast(ref - to) : 0.0f;
-        ref = to;
-        m = x;
-      }
-      const float w = exp2_fast(fmaf(x, c, -ref));
-      s += w;
-      if (RACE && __log2f(w) + ref - __log2f(noise[t]) > score) best = t;
-    }
-  }
-  s *= exp2_fast(-fmaf(m, c, -ref));  // from ref to m c
-  const uint64_t k =
-      block_max(m > -INFINITY ? pack_arg(order_key(m), first_index ? idx : 0) : 0, sh);
-  Slice out;
-  out.idx = k ? unpack_idx(k) : -1;
-  out.m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
-  out.s = block_sum(m > -INFINITY ? s * exp2_fast((m - out.m) * c) : 0.0f, sh);
-  // an infinite maximum, a NaN, or a temperature at either end of its range
-  if (k && !(out.s < INFINITY)) {
-    __syncthreads();
-    out.s = block_sum(sum_by_definition<T>(row, ok, share, out.m, inv), sh);
-  }
-  return out;
-}
 
 __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
   return pack_arg(__float_as_uint(score > 0.0f ? score : 0.0f), t);
 }
 
-// The race of max(p - q, 0) / noise over the CTA's share of a row: (score,
-// lowest index), 0 where nothing takes part; sh.bar is 0 before the call.
-// `draft`: a token that takes no part (-1: none).
+__device__ __forceinline__ uint64_t block_max(uint64_t k, uint64_t* warps) {
+  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  k = warp_max_u64(k);
+  if (lane == 0) warps[warp] = k;
+  __syncthreads();
+  return warp_max_u64(warps[lane & (kScanWarps - 1)]);
+}
+
+__device__ __forceinline__ int32_t step(const VerifyArgs& a, int32_t s, int64_t t) {
+  return (s < 0 || s >= a.num_states || t < 0 || t >= a.V)
+             ? -1
+             : __ldg(a.tok_next + static_cast<int64_t>(s) * a.V + t);
+}
+
+__device__ __forceinline__ int64_t first_row(const VerifyArgs& a, int32_t b) {
+  return a.src_rows ? a.src_rows[b] : static_cast<int64_t>(b) * (a.K + 1);
+}
+__device__ __forceinline__ int64_t first_prob(const VerifyArgs& a, int32_t b) {
+  return a.prob_rows ? a.prob_rows[b] : static_cast<int64_t>(b) * a.K;
+}
+__device__ __forceinline__ float heat_of(const VerifyArgs& a, int32_t b) {
+  return a.temperature ? a.temperature[b] : a.temperature_all;
+}
+
+// ---------------------------------------------------------------------------
+// One warp for a request, a lane for each position.
+
 template <typename T>
-__device__ uint64_t race_slice(const Row<T>& row, const Allow& ok, const Share& share, float inv,
-                               float m, float rz, const float* noise, bool noise_aligned,
-                               const Given& given, int32_t draft, uint32_t ring, Shared& sh) {
+__global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Workspace w) {
+  pdl_trigger();
+  pdl_wait();
+  const int32_t b = static_cast<int32_t>(blockIdx.x * 4 + (threadIdx.x >> 5));
+  const int32_t lane = threadIdx.x & 31, K = a.K;
+  if (b >= a.batch) return;
+  const int32_t len = a.lens ? a.lens[b] : K;
+  const int64_t first = first_row(a, b), pfirst = first_prob(a, b);
+  const int64_t slot = a.slots ? a.slots[b] : b;
+  const bool idle = len < 0 || len > K || first < 0 || first > a.src_total - 1 - len ||
+                    (a.probs && len > 0 && (pfirst < 0 || pfirst > a.probs_total - len));
+  if (lane == 0) w.request[b] = Request{idle ? -1 : len, len, 0, 0, 0};
+  if (idle) {
+    if (lane <= K) {
+      a.tokens[static_cast<int64_t>(b) * (K + 1) + lane] = -1;
+      a.logprobs[static_cast<int64_t>(b) * (K + 1) + lane] = 0.0f;
+    }
+    if (lane == 0) {
+      a.counts[b] = 0;
+      if (a.next_out) a.next_out[b] = a.pool[slot];
+    }
+    return;
+  }
+  Position p{-1, -1, -INFINITY, 1.0f, 0.0f, 0, -INFINITY, 0.0f, -1};
+  if (lane < len) {
+    const int64_t at = static_cast<int64_t>(b) * a.draft_stride + lane;
+    const int64_t d = a.drafts64 ? static_cast<const int64_t*>(a.drafts)[at]
+                                 : static_cast<const int32_t*>(a.drafts)[at];
+    if (d >= 0 && d < a.V) p.draft = static_cast<int32_t>(d);
+    if (heat_of(a, b) > 0.0f) p.uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + lane];
+    if (a.probs && p.draft >= 0)
+      p.qd = load_prob(a.probs, a.probs_dtype, (pfirst + lane) * a.probs_stride + p.draft);
+  }
+  if (a.bits) {
+    if (a.path) {
+      if (lane <= len) p.state = a.path[static_cast<int64_t>(b) * (K + 1) + lane];
+    } else {
+      int32_t s = a.pool[slot];
+      for (int32_t i = 0; i <= len; ++i) {
+        if (lane == i) p.state = s;
+        s = i < len ? step(a, s, __shfl_sync(kFull, p.draft, i)) : -1;
+      }
+    }
+  }
+  if (p.draft >= 0 && Allow(a, p.state).has(p.draft))
+    p.xd = fmaxf(Row<T>(a, first + lane).at(p.draft), -INFINITY);
+  if (lane <= len) w.position[static_cast<int64_t>(b) * (K + 1) + lane] = p;
+}
+
+// ---------------------------------------------------------------------------
+// What a thread keeps of a row that it scans: the maximum m and the sum of
+// exp2(x c - ref) with c = log2(e) / T. ref is not the maximum but some value
+// within kReach of it (of the logits), so that it hardly ever changes; a term
+// is one multiply-add, one exponential and one addition.
+struct Scan {
+  static constexpr float kReach = 16.0f;
+  float m = -INFINITY, ref = 0.0f, limit = -INFINITY, s = 0.0f;
+  int32_t from = -1;         // the block that has m (-1: none)
+  float score = -INFINITY;   // the race: log2 of this thread's best
+  float bar = 0.0f;          // what it has to pass, times -1
+  int32_t best = -1;
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (top > limit) {  // the first value, or one far above it
+      const float to = top * c;
+      s *= limit > -INFINITY ? exp2_fast(ref - to) : 0.0f;
+      ref = to;
+      limit = top + kReach * fminf(1.0f / c, 3.0e38f);
+    }
+  }
+};
+
+struct ScanShared {
+  Lanes lanes;
+  uint64_t warps[kScanWarps];
+  float sums[kScanWarps];
+  uint32_t bar;
+  int32_t last;
+};
+
+// Looks at four vectors of each lane, `word` their allow bits. kRace: with the
+// noise, two at a time for the registers' sake.
+template <typename T, bool RACE>
+__device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_t word, float c,
+                                           const float* noise, bool noise_fits, Scan& k,
+                                           ScanShared& sh) {
+  constexpr int kEpv = Row<T>::kEpv;
+  constexpr int kAtOnce = RACE ? kRaceVecs : 4;
+  const int32_t j0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
+#pragma unroll
+  for (int q0 = 0; q0 < 4; q0 += kAtOnce) {
+    uint32_t keep[kAtOnce];
+    uint4 v[kAtOnce];
+    float e[RACE ? kAtOnce : 1][kEpv];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      keep[q] = Row<T>::keep(word, q0 + q);
+      v[q] = uint4{};
+      if (keep[q]) v[q] = row.vec(j0 + (q0 + q) * 32);
+      if constexpr (RACE) {
+        if (keep[q]) {
+          load_floats<kEpv>(noise + row.token(j0 + (q0 + q) * 32), noise_fits, e[q]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) e[q][i] = 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) v[q] = masked<T>(v[q], keep[q], sh.lanes);
+    uint4 larger = v[0];
+    if constexpr (kAtOnce == 2) larger = vec_max2<T>(v[0], v[1]);
+    if constexpr (kAtOnce == 4)
+      larger = vec_max2<T>(vec_max2<T>(v[0], v[1]), vec_max2<T>(v[2], v[3]));
+    const float top = vec_top<T>(larger);
+    if (top > k.m) {
+      k.from = b;
+      k.m = top;
+    }
+    k.raise(top, c);
+    if constexpr (RACE)
+      k.bar = exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - k.ref) * -kSlack;
+    // ref is 0 as long as there is nothing but -inf: weights of 0
+    const Pair c2 = pair_of(c, c), low = pair_of(-k.ref, -k.ref);
+    const Pair bar2 = pair_of(k.bar, k.bar);
+    Pair s = pair_of(0.0f, 0.0f);
+    float w[RACE ? kAtOnce : 1][kEpv], over = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+      for (int i = 0; i < kEpv; i += 2) {
+        float lo, hi;
+        split(fma2(pair_of(Dt<T>::to_float(vec_get<T>(v[q], i)),
+                           Dt<T>::to_float(vec_get<T>(v[q], i + 1))), c2, low), lo, hi);
+        lo = exp2_fast(lo);
+        hi = exp2_fast(hi);
+        const Pair both = pair_of(lo, hi);
+        s = add2(s, both);
+        if constexpr (RACE) {
+          w[q][i] = lo;
+          w[q][i + 1] = hi;
+          split(fma2(bar2, pair_of(e[q][i], e[q][i + 1]), both), lo, hi);
+          over = fmaxf(over, fmaxf(lo, hi));
+        }
+      }
+    float lo, hi;
+    split(s, lo, hi);
+    k.s += lo + hi;
+    if constexpr (RACE) {
+      if (over > 0.0f) {
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) {
+            const float f = __log2f(w[q][i]) + k.ref - __log2f(e[q][i]);
+            if (f > k.score && w[q][i] > 0.0f) {
+              k.score = f;
+              k.best = row.token(j0 + (q0 + q) * 32) + i;
+            }
+          }
+        const float rise = fminf(k.score, k.ref + __log2f(kMostScore));
+        if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+      }
+    }
+  }
+}
+
+// Calls f(block, allow bits) for this warp's blocks of a chunk, with the next
+// one's bits and lines on their way.
+template <typename T, typename F>
+__device__ __forceinline__ void each_block(const Row<T>& row, const Allow& ok, int32_t chunk,
+                                           int32_t chunks, int32_t V, const float* noise, F&& f) {
+  int32_t first, end;
+  row.chunk(chunk, chunks, first, end);
+  int32_t b = first + static_cast<int32_t>(threadIdx.x >> 5);
+  uint32_t word = b < end ? row.bits(ok, b, V) : 0u;
+  uint32_t next = b + kScanWarps < end ? row.bits(ok, b + kScanWarps, V) : 0u;
+  for (; b < end; b += kScanWarps) {
+    const uint32_t behind =
+        b + 2 * kScanWarps < end ? row.bits(ok, b + 2 * kScanWarps, V) : 0u;
+    if (b + kScanWarps < end) row.warm(b + kScanWarps, next, noise);
+    if (__any_sync(kFull, word != 0)) f(b, word);
+    word = next;
+    next = behind;
+  }
+}
+
+// A chunk of a row, by the whole CTA; all of it in the thread that the return
+// value is true for. RACE: with the race of exp(x / T) / noise.
+template <typename T, bool RACE>
+__device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, int32_t chunk,
+                                           int32_t chunks, int32_t V, float inv, bool greedy,
+                                           const float* noise, ScanShared& sh, Part& part) {
   constexpr int kEpv = Row<T>::kEpv;
   const float c = inv * kLog2e;
-  // p - q with full precision, and its score
+  const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool noise_fits =
+      RACE && (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
+  Scan k;
+  int32_t idx = INT_MAX;
+  each_block(row, ok, chunk, chunks, V, RACE ? noise : nullptr, [&](int32_t b, uint32_t word) {
+    scan_block<T, RACE>(row, b, word, c, noise, noise_fits, k, sh);
+  });
+  row.edges(chunk, chunks, V, [&](int32_t t) {
+    const float x = ok.has(t) ? fmaxf(row.at(t), -INFINITY) : -INFINITY;
+    if (!(x > -INFINITY)) return;
+    k.raise(x, c);
+    if (x > k.m) {
+      k.m = x;
+      k.from = -1;
+      idx = t;
+    } else if (x == k.m) {
+      idx = t;
+    }
+    const float f = exp2_fast(fmaf(x, c, -k.ref));
+    k.s += f;
+    if (RACE && __log2f(f) + k.ref - __log2f(noise[t]) > k.score) k.best = t;
+  });
+  // the chunk's maximum, and where it is first
+  float m = warp_max(k.m);
+  if (lane == 0) sh.sums[warp] = m;
+  __syncthreads();
+  m = warp_max(sh.sums[lane & (kScanWarps - 1)]);
+  uint64_t won = 0;
+  part = Part{m, 0.0f, m > -INFINITY ? 0 : -1, -1, 0.0f, 1.0f};
+  if (greedy && k.m == m && m > -INFINITY) {
+    if (k.from >= 0) {
+      // the first one in this lane's vectors of the block
+      for (int q = 3; q >= 0; --q) {
+        const int32_t j = k.from * 128 + q * 32 + lane;
+        if (j >= row.vecs) continue;
+        for (int n = kEpv - 1; n >= 0; --n) {
+          const int32_t t = row.token(j) + n;
+          if (ok.has(t) && row.at(t) == m) idx = min(idx, t);
+        }
+      }
+    }
+    if (idx != INT_MAX) won = pack_arg(1u, idx);
+  }
+  // its best in the race, with full precision
+  if (RACE && k.best >= 0) {
+    part.x = row.at(k.best);
+    part.e = noise[k.best];
+    const float f = weight(part.x, m, inv);
+    if (f > 0.0f) won = race_key(f / part.e, k.best);
+  }
+  const uint64_t mine = won;
+  won = block_max(won, sh.warps);
+  float s = warp_sum(k.m > -INFINITY ? k.s * exp2_fast(fmaf(-m, c, k.ref)) : 0.0f);
+  if (lane == 0) sh.sums[warp] = s;
+  __syncthreads();
+  s = warp_sum(lane < kScanWarps ? sh.sums[lane] : 0.0f);
+  // an infinite maximum, a NaN, or a temperature at either end of its range
+  if (m > -INFINITY && !(s < INFINITY)) {
+    s = 0.0f;
+    row.each(chunk, chunks, V, [&](int32_t t) {
+      if (ok.has(t)) s += weight(fmaxf(row.at(t), -INFINITY), m, inv);
+    });
+    s = warp_sum(s);
+    __syncthreads();
+    if (lane == 0) sh.sums[warp] = s;
+    __syncthreads();
+    s = warp_sum(lane < kScanWarps ? sh.sums[lane] : 0.0f);
+  }
+  part.s = s;
+  if (greedy && won) part.idx = unpack_idx(won);
+  if (RACE && won) part.best = unpack_idx(won);
+  // the winner knows its logit and noise
+  return RACE && won ? mine == won : tid == 0;
+}
+
+// All chunks of a row put together by one warp, a lane for each; `best`: of
+// the race (-1: none).
+__device__ __forceinline__ Part join(const Part* parts, int32_t chunks, float inv) {
+  const int32_t lane = threadIdx.x & 31;
+  Part p{-INFINITY, 0.0f, -1, -1, 0.0f, 1.0f};
+  if (lane < chunks) {
+    const volatile Part* v = parts + lane;
+    p.m = v->m;
+    p.s = v->s;
+    p.idx = v->idx;
+    p.best = v->best;
+    p.x = v->x;
+    p.e = v->e;
+  }
+  const uint64_t top = warp_max_u64(p.idx < 0 ? 0 : pack_arg(order_key(p.m), p.idx));
+  const float m = top ? key_value(static_cast<uint32_t>(top >> 32)) : -INFINITY;
+  const float s = warp_sum(p.idx < 0 ? 0.0f : p.s * weight(p.m, m, inv));
+  const float f = p.best >= 0 ? weight(p.x, m, inv) : 0.0f;
+  const uint64_t best = warp_max_u64(f > 0.0f ? race_key(f / p.e, p.best) : 0);
+  return Part{m, s, top ? unpack_idx(top) : -1, best ? unpack_idx(best) : -1, 0.0f, 1.0f};
+}
+
+// The drafts' rows.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, kScanCtas)
+    scan_kernel(const VerifyArgs a, const Workspace w, const int32_t chunks) {
+  __shared__ ScanShared sh;
+  const int32_t K = a.K;
+  const int32_t chunk = static_cast<int32_t>(blockIdx.x % chunks);
+  const int32_t b = static_cast<int32_t>(blockIdx.x / chunks % a.batch);
+  const int32_t i = static_cast<int32_t>(blockIdx.x / chunks / a.batch);  // early ones first
+  if (sizeof(typename Dt<T>::Bits) == 2) sh.lanes.fill();
+  pdl_trigger();
+  pdl_wait();
+  Position& pos = w.position[static_cast<int64_t>(b) * (K + 1) + i];
+  const int32_t len = w.request[b].len, state = pos.state;
+  const float heat = heat_of(a, b);
+  // one thread looks, since another CTA may be writing
+  if (threadIdx.x == 0) sh.last = *const_cast<volatile int32_t*>(&w.request[b].end) < i;
+  __syncthreads();
+  if (i >= len || sh.last) return;  // no such row, or one behind a refused draft
+  const bool greedy = !(heat > 0.0f);
+  const float inv = greedy ? 1.0f : 1.0f / heat;
+  Part* parts = w.part + (static_cast<int64_t>(b) * (K + 1) + i) * kMaxChunks;
+  Part part;
+  if (scan_chunk<T, false>(Row<T>(a, first_row(a, b) + i), Allow(a, state), chunk, chunks, a.V, inv,
+                           greedy, nullptr, sh, part)) {
+    parts[chunk] = part;
+    __threadfence();
+    sh.last = atomicAdd(&pos.arrived, 1u) == static_cast<uint32_t>(chunks) - 1;
+  }
+  __syncthreads();
+  if (!sh.last || threadIdx.x >= 32) return;
+  __threadfence();
+  const Part all = join(parts, chunks, inv);
+  if (threadIdx.x == 0) {
+    pos.m = all.m;
+    pos.s = all.s;
+    pos.idx = all.idx;
+    const bool accept = all.idx >= 0 && (greedy ? pos.draft == all.idx
+                                                : pos.uniform * pos.qd <
+                                                      weight(pos.xd, all.m, inv) / all.s);
+    if (!accept) atomicMin(&w.request[b].end, i);
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+// The best max(p - q, 0) / noise of chunk `chunk` of `chunks` of a row, with
+// p = exp((x - m) / T) / s: (score, lowest index), 0 where nothing takes part.
+// `without`: a token that takes no part (-1: none). By the whole CTA.
+template <typename T>
+__device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& ok, int32_t chunk,
+                                               int32_t chunks, int32_t V, float inv, float m,
+                                               float s, const float* noise, const Given& given,
+                                               int32_t without, ScanShared& sh) {
+  constexpr int kEpv = Row<T>::kEpv;
+  const float c = inv * kLog2e, rz = 1.0f / s;
   auto exact = [&](int32_t t) -> uint64_t {
-    if (t == draft || !ok.has(t)) return 0;
+    if (t == without || !ok.has(t)) return 0;
     float left = weight(fmaxf(row.at(t), -INFINITY), m, inv) * rz;
     if (given.p) left -= load_prob(given.p, given.dtype, t);
     return left > 0.0f ? race_key(left / noise[t], t) : 0;
   };
-  uint64_t mine = 0;
-  if (m < INFINITY && c < INFINITY) {
-    float best = -1.0f;
-    int32_t idx = -1;
-    const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
-    constexpr int kDepth = 2;
-    constexpr uint32_t kNoise = kPlane, kGiven = kPlane * (1 + kEpv / 4),
-                       kSlot = kPlane * (1 + kEpv / 2);
-    static_assert(kDepth * kSlot <= kRingBytes * kVerifyThreads, "the ring holds every slot");
-    auto start = [&](int32_t slot, int32_t j) {
-      copy_async<16>(ring + slot * kSlot, row.vec_at(j));
-      copy_floats<kEpv>(ring + slot * kSlot + kNoise, noise + row.token(j), noise_aligned);
-      given.template copy<kEpv>(ring + slot * kSlot + kGiven, row.token(j));
-    };
-    auto use = [&](int32_t slot, int32_t j, uint32_t keep) {
-      if (!keep) return;  // nothing was copied
-      const int32_t t = row.token(j);
-      if (static_cast<uint32_t>(draft - t) < static_cast<uint32_t>(kEpv))
-        keep &= ~(1u << (draft - t));
-      const uint4 x = masked<T>(shared_vec(ring + slot * kSlot), keep, sh);
-      const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
-      float left[kEpv], e[kEpv], over = 0.0f;
-      given.template read<kEpv>(ring + slot * kSlot + kGiven, t, left);
-      read_floats<kEpv>(ring + slot * kSlot + kNoise, e);
+  uint64_t won = 0;
+  auto offer = [&](int32_t t) {
+    const uint64_t k = exact(t);
+    won = k > won ? k : won;
+  };
+  __syncthreads();
+  if (threadIdx.x == 0) sh.bar = 0;
+  __syncthreads();
+  if (!(m < INFINITY && c < INFINITY)) {
+    row.each(chunk, chunks, V, offer);
+    return block_max(won, sh.warps);
+  }
+  float top = -1.0f;
+  int32_t idx = -1;
+  const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
+  const bool noise_fits = (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
+  const bool given_fits = given.p && given.template fits<kEpv>(row.head);
+  each_block(row, ok, chunk, chunks, V, noise, [&](int32_t at, uint32_t word) {
+      const int32_t j0 = at * 128 + static_cast<int32_t>(threadIdx.x & 31);
 #pragma unroll
-      for (int i = 0; i < kEpv; ++i) {
-        const float w = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
-        left[i] = fmaf(w, fix, -left[i]);
-        over = fmaxf(over, fmaf(-bar, e[i], left[i]));
-      }
-      if (over > 0.0f) {
+      for (int q0 = 0; q0 < 4; q0 += 2) {
+        uint32_t keep[2];
+        uint4 v[2];
+        float e[2][kEpv], left[2][kEpv];
 #pragma unroll
-        for (int i = 0; i < kEpv; ++i) {
-          const float f = fmaxf(__fdividef(left[i], e[i]), 0.0f);
-          if (left[i] > 0.0f && f > best) {
-            best = f;
-            idx = t + i;
+        for (int q = 0; q < 2; ++q) {
+          keep[q] = Row<T>::keep(word, q0 + q);
+          const int32_t j = j0 + (q0 + q) * 32, t = row.token(j);
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) left[q][i] = 0.0f;
+          if (keep[q]) {
+            v[q] = row.vec(j);
+            load_floats<kEpv>(noise + t, noise_fits, e[q]);
+            if (given.p) given.load<kEpv>(t, given_fits, left[q]);
+            if (static_cast<uint32_t>(without - t) < static_cast<uint32_t>(kEpv))
+              keep[q] &= ~(1u << (without - t));
           }
         }
-        if (best > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(best, kMostScore)));
+        const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (!keep[q]) continue;
+          const uint4 x = masked<T>(v[q], keep[q], sh.lanes);
+          float over = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i) {
+            const float f = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
+            left[q][i] = fmaf(f, fix, -left[q][i]);
+            over = fmaxf(over, (keep[q] >> i) & 1u ? fmaf(-bar, e[q][i], left[q][i]) : 0.0f);
+          }
+          if (over > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < kEpv; ++i) {
+              const float f = fmaxf(__fdividef(left[q][i], e[q][i]), 0.0f);
+              if ((keep[q] >> i) & 1u && left[q][i] > 0.0f && f > top) {
+                top = f;
+                idx = row.token(j0 + (q0 + q) * 32) + i;
+              }
+            }
+            if (top > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(top, kMostScore)));
+          }
+        }
       }
-    };
-    stream<T, kDepth>(row, ok, share, start, use);
-    if (idx >= 0) mine = exact(idx);
-    const int32_t t = row.edge(share.head, share.tail);
-    if (t >= 0) {
-      const uint64_t k = exact(t);
-      mine = k > mine ? k : mine;
-    }
-  } else {
-    each_token(row, share, [&](int32_t t) {
-      const uint64_t k = exact(t);
-      mine = k > mine ? k : mine;
-    });
-  }
-  return block_max(mine, sh);
+  });
+  if (idx >= 0) offer(idx);
+  row.edges(chunk, chunks, V, offer);
+  return block_max(won, sh.warps);
 }
 
-// The largest of the cluster's keys; every CTA brings its own in `slot`.
-template <int C>
-__device__ __forceinline__ uint64_t cluster_max(uint64_t k, uint64_t& slot) {
-  if constexpr (C == 1) {
-    return k;
-  } else {
-    const int32_t lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) slot = k;
-    cluster_barrier<C>();
-    return warp_max_u64(peer_u64(peer_shared(&slot, lane < C ? lane : 0)));
-  }
-}
-
-template <typename T, int C>
-__global__ void __launch_bounds__(kVerifyThreads, kCtasPerSm) verify_kernel(const VerifyArgs a) {
-  extern __shared__ __align__(16) uint8_t dynamic[];
-  __shared__ Shared sh;
-  const uint32_t ring =
-      static_cast<uint32_t>(__cvta_generic_to_shared(dynamic)) + threadIdx.x * 16;
-  const uint32_t rank = C == 1 ? 0 : cluster_rank();
-  const int32_t b = static_cast<int32_t>(blockIdx.x / C);
-  const int32_t tid = threadIdx.x, lane = tid & 31;
-  const int32_t K = a.K, V = a.V;
+// The row behind a request's accepted drafts, and the results.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, kLastCtas)
+    last_kernel(const VerifyArgs a, const Workspace w, const int32_t chunks) {
+  __shared__ ScanShared sh;
+  const int32_t chunk = static_cast<int32_t>(blockIdx.x % chunks);
+  const int32_t b = static_cast<int32_t>(blockIdx.x / chunks);
+  const int32_t tid = threadIdx.x, lane = tid & 31, K = a.K, V = a.V;
+  if (sizeof(typename Dt<T>::Bits) == 2) sh.lanes.fill();
+  if (tid == 0) sh.bar = order_key(-INFINITY);
+  pdl_trigger();
   pdl_wait();
-  const int32_t len = a.lens ? a.lens[b] : K;
-  const int64_t first = a.src_rows ? a.src_rows[b] : static_cast<int64_t>(b) * (K + 1);
-  const int64_t pfirst = a.prob_rows ? a.prob_rows[b] : static_cast<int64_t>(b) * K;
-  const int64_t slot = a.slots ? a.slots[b] : b;
-  const bool idle = len < 0 || len > K || first < 0 || first > a.src_total - 1 - len ||
-                    (a.probs && len > 0 && (pfirst < 0 || pfirst > a.probs_total - len));
-  int64_t* tokens = a.tokens + static_cast<int64_t>(b) * (K + 1);
-  float* logprobs = a.logprobs + static_cast<int64_t>(b) * (K + 1);
-  if (idle) {  // the same for every CTA of the cluster
-    if (rank == 0) {
-      for (int32_t i = tid; i <= K; i += kVerifyThreads) {
-        tokens[i] = -1;
-        logprobs[i] = 0.0f;
-      }
-      if (tid == 0) {
-        a.counts[b] = 0;
-        if (a.next_out) a.next_out[b] = a.pool[slot];
-      }
-    }
-    return;
-  }
-  const float heat = a.temperature ? a.temperature[b] : a.temperature_all;
+  Request& request = w.request[b];
+  const int32_t len = request.len, n = request.end;
+  if (len < 0) return;
+  const float heat = heat_of(a, b);
   const bool greedy = !(heat > 0.0f);
   const float inv = greedy ? 1.0f : 1.0f / heat;
-  const Share share{static_cast<int32_t>(rank) * kVerifyWarps + (tid >> 5), C * kVerifyWarps,
-                    rank == 0, rank == C - 1};
-  auto draft_at = [&](int32_t i) -> int64_t {
-    const int64_t at = static_cast<int64_t>(b) * a.draft_stride + i;
-    return a.drafts64 ? static_cast<const int64_t*>(a.drafts)[at]
-                      : static_cast<const int32_t*>(a.drafts)[at];
-  };
-  auto step = [&](int32_t s, int64_t t) -> int32_t {
-    return (s < 0 || s >= a.num_states || t < 0 || t >= V)
-               ? -1
-               : __ldg(a.tok_next + static_cast<int64_t>(s) * V + t);
-  };
-  // the states along the drafts, each one position ahead
-  if (a.bits) {
-    if (a.path) {
-      for (int32_t i = tid; i <= len; i += kVerifyThreads)
-        sh.state[i] = a.path[static_cast<int64_t>(b) * (K + 1) + i];
-    } else if (tid == 0) {
-      sh.state[0] = a.pool[slot];
-    }
-  }
-  if (tid == 0) sh.bar = order_key(-INFINITY);
-  if (sizeof(typename Dt<T>::Bits) == 2) {
-    auto two = [&](uint32_t k) { return (k & 1 ? 0xFFFFu : 0u) | (k & 2 ? 0xFFFF0000u : 0u); };
-    for (uint32_t k = tid; k < 256; k += kVerifyThreads)
-      sh.lanes[k] = make_uint4(two(k), two(k >> 2), two(k >> 4), two(k >> 6));
-  }
-  __syncthreads();
-
+  const Position* positions = w.position + static_cast<int64_t>(b) * (K + 1);
+  Position p = positions[n];
+  const Row<T> row(a, first_row(a, b) + n);
+  const Allow ok(a, p.state);
   const float* noise = a.noise + static_cast<int64_t>(b) * a.noise_stride;
-  auto row_of = [&](int32_t i) {
-    return Row<T>(
-        static_cast<const typename Dt<T>::Bits*>(a.src) + (first + i) * a.src_stride, V);
-  };
-  auto allow_of = [&](int32_t i) {
-    Allow ok{nullptr, true};
-    if (a.bits) {
-      const int32_t s = sh.state[i];
-      ok.any = false;
-      if (s >= 0 && s < a.num_states) ok.row = a.bits + static_cast<int64_t>(s) * a.wstride;
-    }
-    return ok;
-  };
-  auto noise_fits = [&](const Row<T>& row) {
-    return (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
-  };
-  int32_t best = -1;  // of the last row's race
-  int32_t n = 0;      // the first position that is not an accepted draft
-  for (int32_t begin = 0;; begin += a.window) {
-    const int32_t end = min(begin + a.window, len + 1);
-    for (int32_t i = begin; i < end; ++i) {
-      const Row<T> row = row_of(i);
-      const Allow ok = allow_of(i);
-      // what the decision needs comes while the row is scanned
-      const int64_t d = i < len ? draft_at(i) : -1;
-      const bool inside = d >= 0 && d < V;
-      float xd = -INFINITY, qd = 1.0f, uniform = 0.0f;
-      int32_t next = -1;
-      if (i < len) {
-        if (inside && ok.has(static_cast<int32_t>(d))) xd = fmaxf(row.at(d), -INFINITY);
-        if (!greedy) uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + i];
-        if (a.probs && inside)
-          qd = load_prob(a.probs, a.probs_dtype, (pfirst + i) * a.probs_stride + d);
-        if (a.bits && !a.path) next = step(sh.state[i], d);
-      }
-      const Slice r =
-          i == len && !greedy
-              ? scan_slice<T, true>(row, ok, share, inv, false, noise,
-                                    noise_fits(row), best, ring, sh)
-              : scan_slice<T, false>(row, ok, share, inv, greedy, noise, false, best,
-                                     ring, sh);
-      if (tid == 0) {
-        sh.slice[i] = r;
-        Position& p = sh.position[i];
-        p.xd = xd;
-        p.qd = qd;
-        p.uniform = uniform;
-        p.draft = inside ? static_cast<int32_t>(d) : -1;
-        if (i < len && a.bits && !a.path) sh.state[i + 1] = next;
-      }
-      __syncthreads();
-    }
-    cluster_barrier<C>();
-    // a warp puts a position's slices together and decides on it
-    for (int32_t i = begin + (tid >> 5); i < end; i += kVerifyWarps) {
-      Position& p = sh.position[i];
-      Slice r;
-      const uint32_t peer = C > 1 ? peer_shared(&sh.slice[i], lane < C ? lane : 0) : 0;
-      if constexpr (C > 1) {
-        r.m = __uint_as_float(peer_u32(peer));
-        r.idx = lane < C ? static_cast<int32_t>(peer_u32(peer + 4)) : -1;
-        r.s = __uint_as_float(peer_u32(peer + 8));
-        const uint64_t k = warp_max_u64(r.idx < 0 ? 0 : pack_arg(order_key(r.m), r.idx));
-        const float m = k ? key_value(static_cast<uint32_t>(k >> 32)) : -INFINITY;
-        r.s = warp_sum(r.idx < 0 ? 0.0f : r.s * weight(r.m, m, inv));
-        r.m = m;
-        r.idx = k ? unpack_idx(k) : -1;
-      } else {
-        r = sh.slice[i];
-      }
-      if (lane == 0) {
-        p.m = r.m;
-        p.s = r.s;
-        p.idx = r.idx;
-        p.accept = i < len && r.idx >= 0 &&
-                   (greedy ? p.draft == r.idx
-                           : p.uniform * p.qd < weight(p.xd, r.m, inv) / r.s);
-      }
+  __syncthreads();
+  int64_t token = -1;
+  bool open = false;  // the race is still to be run, over p
+  if (n == len) {
+    Part* parts = w.part + (static_cast<int64_t>(b) * (K + 1) + n) * kMaxChunks;
+    Part part;
+    if (greedy ? scan_chunk<T, false>(row, ok, chunk, chunks, V, inv, true, nullptr, sh, part)
+               : scan_chunk<T, true>(row, ok, chunk, chunks, V, inv, false, noise, sh, part)) {
+      parts[chunk] = part;
+      __threadfence();
+      sh.last = atomicAdd(&request.arrived, 1u) == static_cast<uint32_t>(chunks) - 1;
     }
     __syncthreads();
-    for (n = begin; n < end && sh.position[n].accept; ++n) {
-      if (rank == 0 && tid == 0) {
-        const Position& p = sh.position[n];
-        tokens[n] = p.draft;
-        logprobs[n] = (p.xd == p.m ? 0.0f : (p.xd - p.m) * inv) - logf(p.s);
-      }
-    }
-    if (n < end) break;
-  }
-  const Position p = sh.position[n];
-  int64_t token = -1;
-  float logprob = 0.0f;
-  if (p.idx >= 0) {  // else nothing is allowed here
-    const Row<T> row = row_of(n);
-    if (greedy) {
-      token = p.idx;
-    } else {
-      const Allow ok = allow_of(n);
-      uint64_t won = 0;
-      if (tid == 0) sh.bar = 0;
-      __syncthreads();
-      if (n == len && p.m < INFINITY) {
-        const float w = best >= 0 ? weight(row.at(best), p.m, inv) : 0.0f;
-        won = block_max(w > 0.0f ? race_key(w / noise[best], best) : 0, sh);
-      } else {
-        Given given{nullptr, a.probs_dtype, false};
-        if (n < len && a.probs) {
-          const int32_t size = a.probs_dtype == BPD_F32 ? 4 : 2;
-          const char* q = static_cast<const char*>(a.probs) + (pfirst + n) * a.probs_stride * size;
-          given.p = q;
-          given.aligned =
-              reinterpret_cast<uintptr_t>(q + row.head * size) % min(16, Row<T>::kEpv * size) == 0;
-        }
-        won = race_slice<T>(row, ok, share, inv, p.m, 1.0f / p.s, noise,
-                            noise_fits(row), given, n < len && !a.probs ? p.draft : -1, ring, sh);
-      }
-      won = cluster_max<C>(won, sh.race[0]);
-      if (!won) {  // nothing left of p - q: the race is over p
-        __syncthreads();
-        if (tid == 0) sh.bar = 0;
-        __syncthreads();
-        won = cluster_max<C>(
-            race_slice<T>(row, ok, share, inv, p.m, 1.0f / p.s, noise,
-                          noise_fits(row), Given{nullptr, 0, false}, -1, ring, sh),
-            sh.race[1]);
-      }
-      if (won) token = unpack_idx(won);
-    }
-    if (token >= 0) {
-      const float xt = row.at(token);
-      logprob = (xt == p.m ? 0.0f : (xt - p.m) * inv) - logf(p.s);
-    }
-  }
-  if (rank == 0) {
-    for (int32_t i = n + tid; i <= K; i += kVerifyThreads) {
-      tokens[i] = i == n ? token : -1;
-      logprobs[i] = i == n ? logprob : 0.0f;
-    }
+    if (!sh.last) return;
+    __threadfence();
+    part = join(parts, chunks, inv);  // by each warp alike
+    p.m = part.m;
+    p.s = part.s;
+    p.idx = part.idx;
+    if (p.idx >= 0) token = greedy ? p.idx : part.best;
+    open = !greedy && p.idx >= 0 && (part.best < 0 || !(p.m < INFINITY));
+  } else if (greedy || p.idx < 0) {
+    if (chunk != 0) return;
+    token = p.idx;
+  } else {
+    Given given{nullptr, a.probs_dtype};
+    if (a.probs)
+      given.p = static_cast<const uint8_t*>(a.probs) +
+                (first_prob(a, b) + n) * a.probs_stride * given.size();
+    uint64_t won = race_chunk<T>(row, ok, chunk, chunks, V, inv, p.m, p.s, noise, given,
+                                 a.probs ? -1 : p.draft, sh);
     if (tid == 0) {
-      a.counts[b] = n + (token >= 0);
-      if (a.tok_next) {
-        const int32_t next = token < 0 ? -1 : step(sh.state[n], token);
-        if (a.next_out) a.next_out[b] = next;
-        if (a.write_back) a.pool[slot] = next;
-      }
+      if (won) atomicMax(&request.race, static_cast<unsigned long long>(won));
+      __threadfence();
+      sh.last = atomicAdd(&request.arrived, 1u) == static_cast<uint32_t>(chunks) - 1;
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    won = *const_cast<volatile unsigned long long*>(&request.race);
+    if (won)
+      token = unpack_idx(won);
+    else
+      open = true;  // nothing left of p - q
+  }
+  if (open) {
+    const uint64_t won =
+        race_chunk<T>(row, ok, 0, 1, V, inv, p.m, p.s, noise, Given{nullptr, 0}, -1, sh);
+    token = won ? unpack_idx(won) : -1;
+  }
+  if (tid >= 32) return;
+  // a lane for each position
+  const int64_t out = static_cast<int64_t>(b) * (K + 1) + lane;
+  if (lane <= K) {
+    int64_t t = -1;
+    float logprob = 0.0f;
+    if (lane < n) {
+      const Position& mine = positions[lane];
+      t = mine.draft;
+      logprob = (mine.xd == mine.m ? 0.0f : (mine.xd - mine.m) * inv) - logf(mine.s);
+    } else if (lane == n && token >= 0) {
+      const float x = row.at(token);
+      t = token;
+      logprob = (x == p.m ? 0.0f : (x - p.m) * inv) - logf(p.s);
+    }
+    a.tokens[out] = t;
+    a.logprobs[out] = logprob;
+  }
+  if (lane == 0) {
+    a.counts[b] = n + (token >= 0);
+    if (a.tok_next) {
+      const int32_t next = token < 0 ? -1 : step(a, p.state, token);
+      if (a.next_out) a.next_out[b] = next;
+      if (a.write_back) a.pool[a.slots ? a.slots[b] : b] = next;
     }
   }
-  cluster_barrier<C>();  // nobody leaves while a neighbour may read its shared memory
 }
 
-template <typename T, int C>
-cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st) {
-  static std::atomic<bool> ready[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev >= 64 || !ready[dev].load(std::memory_order_relaxed))) {
-    e = cudaFuncSetAttribute(verify_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kRingBytes * kVerifyThreads);
-    if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+// ---------------------------------------------------------------------------
+
+// Chunks of a row: enough CTAs to fill the SMs a few times over, none with
+// less than eight blocks of 128 vectors (one for each warp).
+int32_t chunks_of(int64_t rows, int32_t vocab, int32_t vec, int32_t waves) {
+  const int64_t want = (static_cast<int64_t>(sm_count()) * waves + rows - 1) / std::max<int64_t>(rows, 1);
+  const int64_t most = (static_cast<int64_t>(vocab) / vec + 1023) / 1024;
+  return static_cast<int32_t>(std::max<int64_t>(1, std::min({want, most, int64_t{kMaxChunks}})));
+}
+
+size_t lay_out(int32_t batch, int32_t max_drafts, void* base, Workspace* w) {
+  const size_t rows = static_cast<size_t>(batch) * (max_drafts + 1);
+  const size_t position = align256(batch * sizeof(Request));
+  const size_t part = position + align256(rows * sizeof(Position));
+  if (w) {
+    uint8_t* p = static_cast<uint8_t*>(base);
+    w->request = reinterpret_cast<Request*>(p);
+    w->position = reinterpret_cast<Position*>(p + position);
+    w->part = reinterpret_cast<Part*>(p + part);
   }
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * C);
-  cfg.blockDim = dim3(kVerifyThreads);
-  cfg.dynamicSmemBytes = kRingBytes * kVerifyThreads;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = BPD_PDL ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = C;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = C > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, verify_kernel<T, C>, a);
-  if (e != cudaSuccess) (void)cudaGetLastError();
-  return e;
+  return part;
 }
 
 }  // namespace
 }  // namespace bpd
 
 using namespace bpd;
+
+extern "C" size_t bpd_verify_workspace_bytes(int32_t batch, int32_t max_drafts) {
+  batch = std::max(batch, 1);
+  max_drafts = std::max(max_drafts, 0);
+  return lay_out(batch, max_drafts, nullptr, nullptr) +
+         align256(static_cast<size_t>(batch) * (max_drafts + 1) * kMaxChunks * sizeof(Part));
+}
 
 extern "C" bpd_status bpd_verify_drafts(
     const void* src, int32_t src_dtype, int64_t src_stride, int64_t src_total,
@@ -918,15 +1010,15 @@ extern "C" bpd_status bpd_verify_drafts(
     int32_t batch, int32_t max_drafts, int32_t vocab_size, int32_t* state_pool,
     const int64_t* slots, const int32_t* path, const uint32_t* allow_bits, int32_t words_stride,
     const int32_t* tok_next, int32_t num_states, int64_t* tokens_out, int32_t* counts_out,
-    float* logprobs_out, int32_t* next_out, int32_t write_back, void* stream) {
+    float* logprobs_out, int32_t* next_out, int32_t write_back, void* workspace, void* stream) {
   const char* what = "bpd_verify_drafts";
   BPD_REQUIRE(batch >= 0 && vocab_size > 0 && max_drafts >= 0 && src_total >= 0,
               "%s: bad sizes", what);
   if (max_drafts > BPD_MAX_DRAFTS)
     return fail(BPD_ERR_CAPACITY, "%s: more than %d drafts", what, BPD_MAX_DRAFTS);
-  if (batch > INT_MAX / kMaxCluster) return fail(BPD_ERR_CAPACITY, "%s: batch too large", what);
   if (batch == 0) return BPD_OK;
-  BPD_REQUIRE(src && tokens_out && counts_out && logprobs_out, "%s: null pointer", what);
+  BPD_REQUIRE(src && tokens_out && counts_out && logprobs_out && workspace, "%s: null pointer", what);
+  BPD_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", what);
   BPD_REQUIRE(src_stride >= vocab_size, "%s: row stride < vocab", what);
   BPD_REQUIRE(max_drafts == 0 || (drafts && draft_stride >= max_drafts),
               "%s: drafts missing, or their row stride < max_drafts", what);
@@ -944,26 +1036,29 @@ extern "C" bpd_status bpd_verify_drafts(
               "%s: a grammar needs state_pool and tok_next, or path", what);
   BPD_REQUIRE((!next_out && !write_back) || (state_pool && tok_next && allow_bits),
               "%s: next states need state_pool, allow_bits and tok_next", what);
-  VerifyArgs a{src, src_stride, src_total, src_rows, drafts, draft_stride, drafts_int64,
-               draft_lens, probs, probs_dtype, probs_stride, probs_total, prob_rows, uniforms,
-               uniform_stride, noise, noise_stride, temperature, temperature_all, batch,
-               max_drafts, vocab_size, state_pool, slots, path, allow_bits, words_stride,
-               allow_bits ? tok_next : nullptr, num_states, tokens_out, counts_out, logprobs_out,
-               next_out, write_back, 1};
+  const VerifyArgs a{src, src_stride, src_total, src_rows, drafts, draft_stride, drafts_int64,
+                     draft_lens, probs, probs_dtype, probs_stride, probs_total, prob_rows,
+                     uniforms, uniform_stride, noise, noise_stride, temperature, temperature_all,
+                     batch, max_drafts, vocab_size, state_pool, slots, path, allow_bits,
+                     words_stride, allow_bits ? tok_next : nullptr, num_states, tokens_out,
+                     counts_out, logprobs_out, next_out, write_back};
   cudaStream_t st = as_stream(stream);
   return with_dtype(src_dtype, what, [&](auto tag) {
     using T = decltype(tag);
-    // Positions are scanned ahead of the decisions where all rows are few
-    // enough to be read in less time than the cluster takes to meet.
-    const int64_t rows_bytes = static_cast<int64_t>(batch) * (max_drafts + 1) * vocab_size *
-                               static_cast<int64_t>(sizeof(typename Dt<T>::Bits));
-    a.window = rows_bytes <= (100ll << 20) ? max_drafts + 1 : 1;
-    // enough CTAs to fill the SMs four times over, as far as a cluster reaches
-    const int64_t room = kCtasPerSm * static_cast<int64_t>(sm_count());
-    const cudaError_t e = batch * 8ll <= room   ? launch_verify<T, 8>(a, st)
-                          : batch * 4ll <= room ? launch_verify<T, 4>(a, st)
-                          : batch * 2ll <= room ? launch_verify<T, 2>(a, st)
-                                                : launch_verify<T, 1>(a, st);
+    const int64_t rows = static_cast<int64_t>(batch) * max_drafts;
+    Workspace w{};
+    lay_out(batch, max_drafts, workspace, &w);
+    const int32_t chunks = chunks_of(rows, vocab_size, Dt<T>::kPerVec, CW);
+    const int32_t lasts = chunks_of(batch, vocab_size, Dt<T>::kPerVec, LW);
+    if (std::max(rows * chunks, static_cast<int64_t>(batch) * lasts) > INT_MAX)
+      return fail(BPD_ERR_CAPACITY, "%s: batch too large", what);
+    cudaError_t e = launch_pdl(walk_kernel<T>, dim3((batch + 3) / 4), dim3(128), 0, st, a, w);
+    if (e == cudaSuccess && max_drafts)
+      e = launch_pdl(scan_kernel<T>, dim3(static_cast<unsigned>(rows * chunks)),
+                     dim3(kScanThreads), 0, st, a, w, chunks);
+    if (e == cudaSuccess)
+      e = launch_pdl(last_kernel<T>, dim3(static_cast<unsigned>(batch) * lasts),
+                     dim3(kScanThreads), 0, st, a, w, lasts);
     return e == cudaSuccess ? BPD_OK : fail(BPD_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   });
 }

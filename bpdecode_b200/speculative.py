@@ -111,6 +111,7 @@ def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, 
     counts = torch.empty(B, dtype=torch.int32, device=dev)
     logprobs = torch.empty((B, K + 1), dtype=torch.float32, device=dev)
     L = _capi.lib()
+    work = torch.empty(L.bpd_verify_workspace_bytes(B, K), dtype=torch.uint8, device=dev)
     with on_device(dev):
         L.check(L.bpd_verify_drafts(
             src.data_ptr(), _DTYPE_CODE[src.dtype], max(_stride(src), V), src.shape[0],
@@ -123,7 +124,8 @@ def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, 
             0 if noise is None else max(_stride(noise), V), _ptr(heat), everywhere, B, K, V,
             _ptr(pool), slot_ptr, _ptr(path), _ptr(bits), 0 if bits is None else bits.shape[1],
             _ptr(tok_next), num_states, tokens.data_ptr(), counts.data_ptr(),
-            logprobs.data_ptr(), _ptr(states), int(write_back), _stream(src)))
+            logprobs.data_ptr(), _ptr(states), int(write_back),
+            work.data_ptr(), _stream(src)))
     return VerifyResult(tokens, counts, logprobs, states)
 
 

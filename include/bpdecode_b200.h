@@ -431,7 +431,9 @@ bpd_status bpd_lora_project(
  *
  * A request with len < 0 or > max_drafts, or rows outside src or probs, is
  * idle: no tokens, count 0, its state as it was. max_drafts <= BPD_MAX_DRAFTS.
- * slots of one call must be distinct. */
+ * slots of one call must be distinct. workspace: bpd_verify_workspace_bytes,
+ * 16-byte aligned, any contents. */
+size_t bpd_verify_workspace_bytes(int32_t batch, int32_t max_drafts);
 bpd_status bpd_verify_drafts(
     const void* src, int32_t src_dtype, int64_t src_stride, int64_t src_total,
     const int64_t* src_rows, const void* drafts, int32_t drafts_int64,
@@ -443,7 +445,8 @@ bpd_status bpd_verify_drafts(
     int32_t* state_pool, const int64_t* slots, const int32_t* path,
     const uint32_t* allow_bits, int32_t words_stride, const int32_t* tok_next,
     int32_t num_states, int64_t* tokens_out, int32_t* counts_out,
-    float* logprobs_out, int32_t* next_out, int32_t write_back, void* stream);
+    float* logprobs_out, int32_t* next_out, int32_t write_back, void* workspace,
+    void* stream);
 
 /* --------------------------------------------------------------------------
  * Continuous-batching turnover on the device (NEW; the reference leaves the
