@@ -45,9 +45,11 @@ constexpr int kMaxChunks = 32;  // of a row
 #ifndef SC
 #define SC 5
 #define LC 4
-#define CW 8
-#define LW 8
+#define CC 0.04
+#define SV 2
 #define RV 2
+#define FEW 16
+#define WARM 1
 #endif
 constexpr int kScanCtas = SC, kLastCtas = LC;  // on an SM
 constexpr int kRaceVecs = RV;
@@ -199,7 +201,7 @@ struct Row {
     return __ldg(reinterpret_cast<const uint4*>(p + head) + j);
   }
   // Brings block b to L2, if a fair share of its vectors keep a token, and its
-  // noise: in 128-byte lines, a lane for each.
+  // noise.
   __device__ __forceinline__ void warm(int32_t b, uint32_t word, const float* noise) const {
     uint32_t marks = word | word >> 1 | word >> 2 | word >> 3;
     if (kEpv == 8) marks |= marks >> 4;
@@ -207,13 +209,10 @@ struct Row {
     const uint32_t kept = __reduce_add_sync(
         kFull, mine < words ? __popc(marks & (kEpv == 8 ? 0x01010101u : 0x11111111u)) : 0);
     if (kept < 32) return;
-    const int32_t j = b * 128;
-    const uint8_t* at = reinterpret_cast<const uint8_t*>(p + token(j)) + mine * 128;
-    if (mine < 16 && static_cast<int32_t>(mine) * 8 < vecs - j)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
-    if (noise) {
-      const int32_t t = token(j) + static_cast<int32_t>(mine) * 32;
-      if (mine < words && t < token(vecs)) asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + t));
+    if (mine == 0) {
+      const int32_t n = min(128, vecs - b * 128);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + token(b * 128)), "r"(n * 16) : "memory");
+      if (noise) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise + token(b * 128)), "r"(n * kEpv * 4) : "memory");
     }
   }
   // the blocks [first, end) of chunk c of n
@@ -499,7 +498,8 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
 struct Scan {
   static constexpr float kReach = 16.0f;
   float m = -INFINITY, ref = 0.0f, limit = -INFINITY, s = 0.0f;
-  int32_t from = -1;         // the block that has m (-1: none)
+  int32_t from = -1;         // the block whose vectors have m (-1: see idx)
+  int32_t idx = INT_MAX;     // the first token that has m
   float score = -INFINITY;   // the race: log2 of this thread's best
   float bar = 0.0f;          // what it has to pass, times -1
   int32_t best = -1;
@@ -523,26 +523,27 @@ struct ScanShared {
 
 // Looks at four vectors of each lane, `word` their allow bits. kRace: with the
 // noise, two at a time for the registers' sake.
-template <typename T, bool RACE>
-__device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_t word, float c,
+template <typename T, bool RACE, int N>
+__device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, const uint32_t (&word)[N], float c,
                                            const float* noise, bool noise_fits, Scan& k,
                                            ScanShared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
-  constexpr int kAtOnce = RACE ? kRaceVecs : 4;
-  const int32_t j0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
+  constexpr int kAtOnce = RACE ? kRaceVecs : 4 * N;
+  const int32_t lane0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
+  auto vec_of = [&](int q) { return lane0 + q / 4 * kScanWarps * 128 + q % 4 * 32; };
 #pragma unroll
-  for (int q0 = 0; q0 < 4; q0 += kAtOnce) {
+  for (int q0 = 0; q0 < 4 * N; q0 += kAtOnce) {
     uint32_t keep[kAtOnce];
     uint4 v[kAtOnce];
     float e[RACE ? kAtOnce : 1][kEpv];
 #pragma unroll
     for (int q = 0; q < kAtOnce; ++q) {
-      keep[q] = Row<T>::keep(word, q0 + q);
+      keep[q] = Row<T>::keep(word[(q0 + q) / 4], (q0 + q) % 4);
       v[q] = uint4{};
-      if (keep[q]) v[q] = row.vec(j0 + (q0 + q) * 32);
+      if (keep[q]) v[q] = row.vec(vec_of(q0 + q));
       if constexpr (RACE) {
         if (keep[q]) {
-          load_floats<kEpv>(noise + row.token(j0 + (q0 + q) * 32), noise_fits, e[q]);
+          load_floats<kEpv>(noise + row.token(vec_of(q0 + q)), noise_fits, e[q]);
         } else {
 #pragma unroll
           for (int i = 0; i < kEpv; ++i) e[q][i] = 0.0f;
@@ -553,11 +554,14 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
     for (int q = 0; q < kAtOnce; ++q) v[q] = masked<T>(v[q], keep[q], sh.lanes);
     uint4 larger = v[0];
     if constexpr (kAtOnce == 2) larger = vec_max2<T>(v[0], v[1]);
-    if constexpr (kAtOnce == 4)
+    if constexpr (kAtOnce >= 4)
       larger = vec_max2<T>(vec_max2<T>(v[0], v[1]), vec_max2<T>(v[2], v[3]));
+    if constexpr (kAtOnce >= 8)
+      larger = vec_max2<T>(larger, vec_max2<T>(vec_max2<T>(v[4], v[5]), vec_max2<T>(v[6], v[7])));
     const float top = vec_top<T>(larger);
     if (top > k.m) {
       k.from = b;
+      k.idx = INT_MAX;
       k.m = top;
     }
     k.raise(top, c);
@@ -598,7 +602,7 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
             const float f = __log2f(w[q][i]) + k.ref - __log2f(e[q][i]);
             if (f > k.score && w[q][i] > 0.0f) {
               k.score = f;
-              k.best = row.token(j0 + (q0 + q) * 32) + i;
+              k.best = row.token(vec_of(q0 + q)) + i;
             }
           }
         const float rise = fminf(k.score, k.ref + __log2f(kMostScore));
@@ -608,23 +612,102 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
   }
 }
 
-// Calls f(block, allow bits) for this warp's blocks of a chunk, with the next
-// one's bits and lines on their way.
-template <typename T, typename F>
+// The same for a block that allows few tokens: each lane goes through the
+// tokens of its word, four at a time.
+template <typename T, bool RACE>
+__device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t word, float c,
+                                         const float* noise, Scan& k, ScanShared& sh) {
+  const int32_t lane = threadIdx.x & 31, t0 = row.token(b * 128) + lane * 32;
+  if (lane >= 4 * Row<T>::kEpv) word = 0;
+  while (__any_sync(kFull, word != 0)) {
+    int32_t t[4];
+    float x[4], e[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      t[u] = t0 + __ffs(word) - 1;
+      x[u] = -INFINITY;
+      e[u] = 0.0f;
+      if (word) {
+        x[u] = row.at(t[u]);
+        if (RACE) e[u] = __ldg(noise + t[u]);
+      }
+      word &= word - 1;
+    }
+    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    if (top > k.m) {
+      k.m = top;
+      k.from = -1;
+#pragma unroll
+      for (int u = 3; u >= 0; --u)
+        if (x[u] == top) k.idx = t[u];
+    }
+    k.raise(top, c);
+    const float bar =
+        RACE ? exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - k.ref) * kSlack : 0;
+    float over = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      x[u] = exp2_fast(fmaf(x[u], c, -k.ref));
+      if (RACE) over = fmaxf(over, fmaf(-bar, e[u], x[u]));
+    }
+    k.s += (x[0] + x[1]) + (x[2] + x[3]);
+    if (RACE && over > 0.0f) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float f = __log2f(x[u]) + k.ref - __log2f(e[u]);
+        if (f > k.score && x[u] > 0.0f) {
+          k.score = f;
+          k.best = t[u];
+        }
+      }
+      const float rise = fminf(k.score, k.ref + __log2f(kMostScore));
+      if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+    }
+  }
+}
+
+// Whether n blocks with `mine` allowed tokens in this lane's words allow few
+// tokens: an eighth.
+template <typename T>
+__device__ __forceinline__ bool few(uint32_t mine, int n) {
+  const uint32_t lane = threadIdx.x & 31;
+  return __reduce_add_sync(kFull, lane < 4 * Row<T>::kEpv ? mine : 0u) <=
+         static_cast<uint32_t>(n * FEW * Row<T>::kEpv);
+}
+
+// Calls f(blocks, their allow bits) for this warp's blocks of a chunk, N at a
+// time, with the next ones' bits on their way (0 behind the last block).
+template <int N, typename T, typename F>
 __device__ __forceinline__ void each_block(const Row<T>& row, const Allow& ok, int32_t chunk,
                                            int32_t chunks, int32_t V, const float* noise, F&& f) {
   int32_t first, end;
   row.chunk(chunk, chunks, first, end);
   int32_t b = first + static_cast<int32_t>(threadIdx.x >> 5);
-  uint32_t word = b < end ? row.bits(ok, b, V) : 0u;
-  uint32_t next = b + kScanWarps < end ? row.bits(ok, b + kScanWarps, V) : 0u;
-  for (; b < end; b += kScanWarps) {
-    const uint32_t behind =
-        b + 2 * kScanWarps < end ? row.bits(ok, b + 2 * kScanWarps, V) : 0u;
-    if (b + kScanWarps < end) row.warm(b + kScanWarps, next, noise);
-    if (__any_sync(kFull, word != 0)) f(b, word);
-    word = next;
-    next = behind;
+  constexpr int kStride = N * kScanWarps;
+  auto bits = [&](int32_t at, uint32_t (&word)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      word[i] = at + i * kScanWarps < end ? row.bits(ok, at + i * kScanWarps, V) : 0u;
+  };
+  uint32_t word[N], next[N], behind[N];
+  bits(b, word);
+  bits(b + kStride, next);
+  for (; b < end; b += kStride) {
+    bits(b + 2 * kStride, behind);
+    if (WARM) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (b + kStride + i * kScanWarps < end) row.warm(b + kStride + i * kScanWarps, next[i], noise);
+    }
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) any |= word[i];
+    if (__any_sync(kFull, any != 0)) f(b, word);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      word[i] = next[i];
+      next[i] = behind[i];
+    }
   }
 }
 
@@ -640,9 +723,19 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
   const bool noise_fits =
       RACE && (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   Scan k;
-  int32_t idx = INT_MAX;
-  each_block(row, ok, chunk, chunks, V, RACE ? noise : nullptr, [&](int32_t b, uint32_t word) {
-    scan_block<T, RACE>(row, b, word, c, noise, noise_fits, k, sh);
+  constexpr int kBlocks = RACE ? 1 : SV;
+  each_block<kBlocks>(row, ok, chunk, chunks, V, RACE && noise_fits ? noise : nullptr,
+                      [&](int32_t b, const uint32_t (&word)[kBlocks]) {
+    uint32_t all = 0;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) all += __popc(word[i]);
+    if (few<T>(all, kBlocks)) {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+        scan_few<T, RACE>(row, b + i * kScanWarps, word[i], c, noise, k, sh);
+    } else {
+      scan_block<T, RACE, kBlocks>(row, b, word, c, noise, noise_fits, k, sh);
+    }
   });
   row.edges(chunk, chunks, V, [&](int32_t t) {
     const float x = ok.has(t) ? fmaxf(row.at(t), -INFINITY) : -INFINITY;
@@ -651,9 +744,9 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
     if (x > k.m) {
       k.m = x;
       k.from = -1;
-      idx = t;
+      k.idx = t;
     } else if (x == k.m) {
-      idx = t;
+      k.idx = k.from < 0 ? min(k.idx, t) : t;
     }
     const float f = exp2_fast(fmaf(x, c, -k.ref));
     k.s += f;
@@ -664,18 +757,22 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
   if (lane == 0) sh.sums[warp] = m;
   __syncthreads();
   m = warp_max(sh.sums[lane & (kScanWarps - 1)]);
+  int32_t idx = k.idx;
   uint64_t won = 0;
   part = Part{m, 0.0f, m > -INFINITY ? 0 : -1, -1, 0.0f, 1.0f};
-  if (greedy && k.m == m && m > -INFINITY) {
-    if (k.from >= 0) {
-      // the first one in this lane's vectors of the block
-      for (int q = 3; q >= 0; --q) {
-        const int32_t j = k.from * 128 + q * 32 + lane;
-        if (j >= row.vecs) continue;
-        for (int n = kEpv - 1; n >= 0; --n) {
-          const int32_t t = row.token(j) + n;
-          if (ok.has(t) && row.at(t) == m) idx = min(idx, t);
-        }
+  if (greedy && m > -INFINITY) {
+    if (k.m != m) idx = INT_MAX;
+    // The vectors of a round in which a lane met m: the warp looks at their
+    // tokens together for the first one.
+    uint32_t lanes = __ballot_sync(kFull, k.m == m && k.from >= 0);
+    for (; lanes; lanes &= lanes - 1) {
+      const int32_t l = __ffs(lanes) - 1, from = __shfl_sync(kFull, k.from, l);
+#pragma unroll
+      for (int q0 = 0; q0 < 4 * kBlocks; q0 += 32 / kEpv) {
+        const int32_t q = q0 + lane / kEpv;
+        const int32_t j = (from + q / 4 * kScanWarps) * 128 + q % 4 * 32 + l;
+        const int32_t t = row.token(j) + lane % kEpv;
+        if (j < row.vecs && ok.has(t) && row.at(t) == m) idx = min(idx, t);
       }
     }
     if (idx != INT_MAX) won = pack_arg(1u, idx);
@@ -813,7 +910,44 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
   const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
   const bool noise_fits = (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   const bool given_fits = given.p && given.template fits<kEpv>(row.head);
-  each_block(row, ok, chunk, chunks, V, noise, [&](int32_t at, uint32_t word) {
+  each_block<1>(row, ok, chunk, chunks, V, noise_fits ? noise : nullptr, [&](int32_t at, const uint32_t (&words)[1]) {
+      uint32_t word = words[0];
+      if (few<T>(__popc(word), 1)) {
+        const int32_t lane = threadIdx.x & 31, t0 = row.token(at * 128) + lane * 32;
+        if (lane >= 4 * kEpv) word = 0;
+        while (__any_sync(kFull, word != 0)) {
+          int32_t t[4];
+          float x[4], e[4], q[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            t[u] = t0 + __ffs(word) - 1;
+            const bool in = word != 0 && t[u] != without;
+            x[u] = in ? row.at(t[u]) : -INFINITY;
+            e[u] = in ? __ldg(noise + t[u]) : 0.0f;
+            q[u] = in && given.p ? load_prob(given.p, given.dtype, t[u]) : 0.0f;
+            word &= word - 1;
+          }
+          const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+          float over = 0.0f;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            x[u] = fmaf(exp2_fast(fmaf(x[u], c, -ref)), fix, -q[u]);
+            over = fmaxf(over, fmaf(-bar, e[u], x[u]));
+          }
+          if (over > 0.0f) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float f = fmaxf(__fdividef(x[u], e[u]), 0.0f);
+              if (x[u] > 0.0f && f > top) {
+                top = f;
+                idx = t[u];
+              }
+            }
+            if (top > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(top, kMostScore)));
+          }
+        }
+        return;
+      }
       const int32_t j0 = at * 128 + static_cast<int32_t>(threadIdx.x & 31);
 #pragma unroll
       for (int q0 = 0; q0 < 4; q0 += 2) {
@@ -968,12 +1102,22 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
 
 // ---------------------------------------------------------------------------
 
-// Chunks of a row: enough CTAs to fill the SMs a few times over, none with
-// less than eight blocks of 128 vectors (one for each warp).
-int32_t chunks_of(int64_t rows, int32_t vocab, int32_t vec, int32_t waves) {
-  const int64_t want = (static_cast<int64_t>(sm_count()) * waves + rows - 1) / std::max<int64_t>(rows, 1);
-  const int64_t most = (static_cast<int64_t>(vocab) / vec + 1023) / 1024;
-  return static_cast<int32_t>(std::max<int64_t>(1, std::min({want, most, int64_t{kMaxChunks}})));
+// Chunks of a row: CTAs that fill the SMs' room (`room` CTAs) in whole waves as
+// nearly as can be, each chunk with a block of 128 vectors for every warp; a
+// cost for each more.
+int32_t chunks_of(int64_t rows, int32_t vocab, int32_t vec, int64_t room) {
+  const int64_t most = std::min<int64_t>(kMaxChunks, (static_cast<int64_t>(vocab) / vec + 1023) / 1024);
+  int32_t best = 1;
+  double least = 0.0;
+  for (int32_t c = 1; c <= most; ++c) {
+    const int64_t waves = (rows * c + room - 1) / room;
+    const double cost = static_cast<double>(waves) * (1.0 / c + CC);
+    if (c == 1 || cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
 }
 
 size_t lay_out(int32_t batch, int32_t max_drafts, void* base, Workspace* w) {
@@ -1048,8 +1192,8 @@ extern "C" bpd_status bpd_verify_drafts(
     const int64_t rows = static_cast<int64_t>(batch) * max_drafts;
     Workspace w{};
     lay_out(batch, max_drafts, workspace, &w);
-    const int32_t chunks = chunks_of(rows, vocab_size, Dt<T>::kPerVec, CW);
-    const int32_t lasts = chunks_of(batch, vocab_size, Dt<T>::kPerVec, LW);
+    const int32_t chunks = chunks_of(rows, vocab_size, Dt<T>::kPerVec, kScanCtas * static_cast<int64_t>(sm_count()));
+    const int32_t lasts = chunks_of(batch, vocab_size, Dt<T>::kPerVec, kLastCtas * static_cast<int64_t>(sm_count()));
     if (std::max(rows * chunks, static_cast<int64_t>(batch) * lasts) > INT_MAX)
       return fail(BPD_ERR_CAPACITY, "%s: batch too large", what);
     cudaError_t e = launch_pdl(walk_kernel<T>, dim3((batch + 3) / 4), dim3(128), 0, st, a, w);
