@@ -39,6 +39,22 @@ class PdaGrammar(C.Structure):
     ]
 
 
+class VerifyArgs(C.Structure):
+    """``bpd_verify_args``: what ``bpd_verify_drafts`` takes."""
+
+    _fields_ = [
+        ("src", _P), ("src_stride", _I64), ("src_total", _I64), ("src_rows", _P), ("drafts", _P),
+        ("draft_stride", _I64), ("draft_lens", _P), ("probs", _P), ("probs_stride", _I64),
+        ("probs_total", _I64), ("prob_rows", _P), ("uniforms", _P), ("uniform_stride", _I64),
+        ("noise", _P), ("noise_stride", _I64), ("temperature", _P), ("state_pool", _P),
+        ("slots", _P), ("path", _P), ("allow_bits", _P), ("tok_next", _P), ("tokens_out", _P),
+        ("counts_out", _P), ("logprobs_out", _P), ("next_out", _P), ("workspace", _P),
+        ("src_dtype", _I32), ("drafts_int64", _I32), ("probs_dtype", _I32), ("batch", _I32),
+        ("max_drafts", _I32), ("vocab_size", _I32), ("words_stride", _I32), ("num_states", _I32),
+        ("write_back", _I32), ("temperature_all", _F),
+    ]
+
+
 _SIGNATURES: dict[str, tuple[object, list]] = {
     "bpd_version": (C.c_char_p, []),
     "bpd_last_error": (C.c_char_p, []),
@@ -77,9 +93,7 @@ _SIGNATURES: dict[str, tuple[object, list]] = {
     "bpd_lora_take_error": (_I32, [C.POINTER(_I32)]),
     "bpd_lora_project": (_I32, [_P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _I32,
                                 _I32, _P, _I32, _P, _I32, _I64, _P, _P]),
-    "bpd_verify_drafts": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I32, _I64, _P, _P, _I32, _I64,
-                                 _I64, _P, _P, _I64, _P, _I64, _P, _F, _I32, _I32, _I32, _P, _P,
-                                 _P, _P, _I32, _P, _I32, _P, _P, _P, _P, _I32, _P, _P]),
+    "bpd_verify_drafts": (_I32, [_P, _P]),
     "bpd_verify_workspace_bytes": (_S, [_I32, _I32]),
     "bpd_serving_turnover": (_I32, [_I32, C.c_uint64, _P, _F, _F, _F, _I32, _I32, _P, _P, _P, _P,
                                     _P, _P, _P, _P, _P, _P, _P]),

@@ -42,51 +42,12 @@ namespace {
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kMaxChunks = 32;  // of a row
-#ifndef SC
-#define SC 5
-#define LC 4
-#define CC 0.04
-#define SV 2
-#define RV 2
-#define FEW 16
-#define WARM 1
-#endif
-constexpr int kScanCtas = SC, kLastCtas = LC;  // on an SM
-constexpr int kRaceVecs = RV;
+constexpr int kScanCtas = 5, kLastCtas = 4;  // on an SM
+constexpr int kScanBlocks = 1;  // blocks of a draft's row that a warp reads at once
+constexpr int kRaceVecs = 2;    // vectors of a race that a lane reads at once
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct VerifyArgs {
-  const void* src;
-  int64_t src_stride, src_total;
-  const int64_t* src_rows;
-  const void* drafts;
-  int64_t draft_stride;
-  int32_t drafts64;
-  const int32_t* lens;
-  const void* probs;
-  int32_t probs_dtype;
-  int64_t probs_stride, probs_total;
-  const int64_t* prob_rows;
-  const float* uniforms;
-  int64_t uniform_stride;
-  const float* noise;
-  int64_t noise_stride;
-  const float* temperature;
-  float temperature_all;
-  int32_t batch, K, V;
-  int32_t* pool;
-  const int64_t* slots;
-  const int32_t* path;
-  const uint32_t* bits;
-  int32_t wstride;
-  const int32_t* tok_next;
-  int32_t num_states;
-  int64_t* tokens;
-  int32_t* counts;
-  float* logprobs;
-  int32_t* next_out;
-  int32_t write_back;
-};
+using VerifyArgs = bpd_verify_args;
 
 // What walk_kernel leaves for a position: its state, the draft (-1: none, or
 // no token of the vocabulary) with its logit (-inf: rejected) and probability,
@@ -172,9 +133,9 @@ __device__ __forceinline__ float warp_max(float v) {
 struct Allow {
   const uint32_t* row;  // NULL: see `any`
   bool any;
-  __device__ __forceinline__ Allow(const VerifyArgs& a, int32_t state) : row(nullptr), any(!a.bits) {
-    if (a.bits && state >= 0 && state < a.num_states)
-      row = a.bits + static_cast<int64_t>(state) * a.wstride;
+  __device__ __forceinline__ Allow(const VerifyArgs& a, int32_t state) : row(nullptr), any(!a.allow_bits) {
+    if (a.allow_bits && state >= 0 && state < a.num_states)
+      row = a.allow_bits + static_cast<int64_t>(state) * a.words_stride;
   }
   __device__ __forceinline__ bool has(int32_t t) const {
     return row ? ((__ldg(row + (t >> 5)) >> (t & 31)) & 1u) : any;
@@ -192,28 +153,13 @@ struct Row {
   __device__ Row(const VerifyArgs& a, int64_t row)
       : p(static_cast<const Bits*>(a.src) + row * a.src_stride) {
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-    head = min(a.V, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
-    vecs = (a.V - head) / kEpv;
+    head = min(a.vocab_size, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
+    vecs = (a.vocab_size - head) / kEpv;
   }
   __device__ __forceinline__ float at(int64_t t) const { return Dt<T>::to_float(p[t]); }
   __device__ __forceinline__ int32_t token(int32_t vec) const { return head + vec * kEpv; }
   __device__ __forceinline__ uint4 vec(int32_t j) const {
     return __ldg(reinterpret_cast<const uint4*>(p + head) + j);
-  }
-  // Brings block b to L2, if a fair share of its vectors keep a token, and its
-  // noise.
-  __device__ __forceinline__ void warm(int32_t b, uint32_t word, const float* noise) const {
-    uint32_t marks = word | word >> 1 | word >> 2 | word >> 3;
-    if (kEpv == 8) marks |= marks >> 4;
-    const uint32_t mine = threadIdx.x & 31u, words = 4 * kEpv;
-    const uint32_t kept = __reduce_add_sync(
-        kFull, mine < words ? __popc(marks & (kEpv == 8 ? 0x01010101u : 0x11111111u)) : 0);
-    if (kept < 32) return;
-    if (mine == 0) {
-      const int32_t n = min(128, vecs - b * 128);
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + token(b * 128)), "r"(n * 16) : "memory");
-      if (noise) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(noise + token(b * 128)), "r"(n * kEpv * 4) : "memory");
-    }
   }
   // the blocks [first, end) of chunk c of n
   __device__ __forceinline__ void chunk(int32_t c, int32_t n, int32_t& first, int32_t& end) const {
@@ -422,16 +368,16 @@ __device__ __forceinline__ uint64_t block_max(uint64_t k, uint64_t* warps) {
 }
 
 __device__ __forceinline__ int32_t step(const VerifyArgs& a, int32_t s, int64_t t) {
-  return (s < 0 || s >= a.num_states || t < 0 || t >= a.V)
+  return (s < 0 || s >= a.num_states || t < 0 || t >= a.vocab_size)
              ? -1
-             : __ldg(a.tok_next + static_cast<int64_t>(s) * a.V + t);
+             : __ldg(a.tok_next + static_cast<int64_t>(s) * a.vocab_size + t);
 }
 
 __device__ __forceinline__ int64_t first_row(const VerifyArgs& a, int32_t b) {
-  return a.src_rows ? a.src_rows[b] : static_cast<int64_t>(b) * (a.K + 1);
+  return a.src_rows ? a.src_rows[b] : static_cast<int64_t>(b) * (a.max_drafts + 1);
 }
 __device__ __forceinline__ int64_t first_prob(const VerifyArgs& a, int32_t b) {
-  return a.prob_rows ? a.prob_rows[b] : static_cast<int64_t>(b) * a.K;
+  return a.prob_rows ? a.prob_rows[b] : static_cast<int64_t>(b) * a.max_drafts;
 }
 __device__ __forceinline__ float heat_of(const VerifyArgs& a, int32_t b) {
   return a.temperature ? a.temperature[b] : a.temperature_all;
@@ -445,9 +391,9 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
   pdl_trigger();
   pdl_wait();
   const int32_t b = static_cast<int32_t>(blockIdx.x * 4 + (threadIdx.x >> 5));
-  const int32_t lane = threadIdx.x & 31, K = a.K;
+  const int32_t lane = threadIdx.x & 31, K = a.max_drafts;
   if (b >= a.batch) return;
-  const int32_t len = a.lens ? a.lens[b] : K;
+  const int32_t len = a.draft_lens ? a.draft_lens[b] : K;
   const int64_t first = first_row(a, b), pfirst = first_prob(a, b);
   const int64_t slot = a.slots ? a.slots[b] : b;
   const bool idle = len < 0 || len > K || first < 0 || first > a.src_total - 1 - len ||
@@ -455,30 +401,30 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
   if (lane == 0) w.request[b] = Request{idle ? -1 : len, len, 0, 0, 0};
   if (idle) {
     if (lane <= K) {
-      a.tokens[static_cast<int64_t>(b) * (K + 1) + lane] = -1;
-      a.logprobs[static_cast<int64_t>(b) * (K + 1) + lane] = 0.0f;
+      a.tokens_out[static_cast<int64_t>(b) * (K + 1) + lane] = -1;
+      a.logprobs_out[static_cast<int64_t>(b) * (K + 1) + lane] = 0.0f;
     }
     if (lane == 0) {
-      a.counts[b] = 0;
-      if (a.next_out) a.next_out[b] = a.pool[slot];
+      a.counts_out[b] = 0;
+      if (a.next_out) a.next_out[b] = a.state_pool[slot];
     }
     return;
   }
   Position p{-1, -1, -INFINITY, 1.0f, 0.0f, 0, -INFINITY, 0.0f, -1};
   if (lane < len) {
     const int64_t at = static_cast<int64_t>(b) * a.draft_stride + lane;
-    const int64_t d = a.drafts64 ? static_cast<const int64_t*>(a.drafts)[at]
+    const int64_t d = a.drafts_int64 ? static_cast<const int64_t*>(a.drafts)[at]
                                  : static_cast<const int32_t*>(a.drafts)[at];
-    if (d >= 0 && d < a.V) p.draft = static_cast<int32_t>(d);
+    if (d >= 0 && d < a.vocab_size) p.draft = static_cast<int32_t>(d);
     if (heat_of(a, b) > 0.0f) p.uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + lane];
     if (a.probs && p.draft >= 0)
       p.qd = load_prob(a.probs, a.probs_dtype, (pfirst + lane) * a.probs_stride + p.draft);
   }
-  if (a.bits) {
+  if (a.allow_bits) {
     if (a.path) {
       if (lane <= len) p.state = a.path[static_cast<int64_t>(b) * (K + 1) + lane];
     } else {
-      int32_t s = a.pool[slot];
+      int32_t s = a.state_pool[slot];
       for (int32_t i = 0; i <= len; ++i) {
         if (lane == i) p.state = s;
         s = i < len ? step(a, s, __shfl_sync(kFull, p.draft, i)) : -1;
@@ -672,14 +618,14 @@ template <typename T>
 __device__ __forceinline__ bool few(uint32_t mine, int n) {
   const uint32_t lane = threadIdx.x & 31;
   return __reduce_add_sync(kFull, lane < 4 * Row<T>::kEpv ? mine : 0u) <=
-         static_cast<uint32_t>(n * FEW * Row<T>::kEpv);
+         static_cast<uint32_t>(n * 16 * Row<T>::kEpv);
 }
 
 // Calls f(blocks, their allow bits) for this warp's blocks of a chunk, N at a
 // time, with the next ones' bits on their way (0 behind the last block).
 template <int N, typename T, typename F>
 __device__ __forceinline__ void each_block(const Row<T>& row, const Allow& ok, int32_t chunk,
-                                           int32_t chunks, int32_t V, const float* noise, F&& f) {
+                                           int32_t chunks, int32_t V, F&& f) {
   int32_t first, end;
   row.chunk(chunk, chunks, first, end);
   int32_t b = first + static_cast<int32_t>(threadIdx.x >> 5);
@@ -694,11 +640,6 @@ __device__ __forceinline__ void each_block(const Row<T>& row, const Allow& ok, i
   bits(b + kStride, next);
   for (; b < end; b += kStride) {
     bits(b + 2 * kStride, behind);
-    if (WARM) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (b + kStride + i * kScanWarps < end) row.warm(b + kStride + i * kScanWarps, next[i], noise);
-    }
     uint32_t any = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) any |= word[i];
@@ -723,9 +664,8 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
   const bool noise_fits =
       RACE && (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   Scan k;
-  constexpr int kBlocks = RACE ? 1 : SV;
-  each_block<kBlocks>(row, ok, chunk, chunks, V, RACE && noise_fits ? noise : nullptr,
-                      [&](int32_t b, const uint32_t (&word)[kBlocks]) {
+  constexpr int kBlocks = RACE ? 1 : kScanBlocks;
+  auto block = [&](int32_t b, const uint32_t (&word)[kBlocks]) {
     uint32_t all = 0;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) all += __popc(word[i]);
@@ -736,7 +676,8 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
     } else {
       scan_block<T, RACE, kBlocks>(row, b, word, c, noise, noise_fits, k, sh);
     }
-  });
+  };
+  each_block<kBlocks>(row, ok, chunk, chunks, V, block);
   row.edges(chunk, chunks, V, [&](int32_t t) {
     const float x = ok.has(t) ? fmaxf(row.at(t), -INFINITY) : -INFINITY;
     if (!(x > -INFINITY)) return;
@@ -836,7 +777,7 @@ template <typename T>
 __global__ void __launch_bounds__(kScanThreads, kScanCtas)
     scan_kernel(const VerifyArgs a, const Workspace w, const int32_t chunks) {
   __shared__ ScanShared sh;
-  const int32_t K = a.K;
+  const int32_t K = a.max_drafts;
   const int32_t chunk = static_cast<int32_t>(blockIdx.x % chunks);
   const int32_t b = static_cast<int32_t>(blockIdx.x / chunks % a.batch);
   const int32_t i = static_cast<int32_t>(blockIdx.x / chunks / a.batch);  // early ones first
@@ -854,7 +795,7 @@ __global__ void __launch_bounds__(kScanThreads, kScanCtas)
   const float inv = greedy ? 1.0f : 1.0f / heat;
   Part* parts = w.part + (static_cast<int64_t>(b) * (K + 1) + i) * kMaxChunks;
   Part part;
-  if (scan_chunk<T, false>(Row<T>(a, first_row(a, b) + i), Allow(a, state), chunk, chunks, a.V, inv,
+  if (scan_chunk<T, false>(Row<T>(a, first_row(a, b) + i), Allow(a, state), chunk, chunks, a.vocab_size, inv,
                            greedy, nullptr, sh, part)) {
     parts[chunk] = part;
     __threadfence();
@@ -910,90 +851,92 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
   const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
   const bool noise_fits = (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   const bool given_fits = given.p && given.template fits<kEpv>(row.head);
-  each_block<1>(row, ok, chunk, chunks, V, noise_fits ? noise : nullptr, [&](int32_t at, const uint32_t (&words)[1]) {
-      uint32_t word = words[0];
-      if (few<T>(__popc(word), 1)) {
-        const int32_t lane = threadIdx.x & 31, t0 = row.token(at * 128) + lane * 32;
-        if (lane >= 4 * kEpv) word = 0;
-        while (__any_sync(kFull, word != 0)) {
-          int32_t t[4];
-          float x[4], e[4], q[4];
+  auto look = [&](float left, float e, int32_t t) {
+    const float f = fmaxf(__fdividef(left, e), 0.0f);
+    if (left > 0.0f && f > top) {
+      top = f;
+      idx = t;
+    }
+  };
+  auto raise = [&] {
+    if (top > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(top, kMostScore)));
+  };
+  // a block that allows few tokens: each lane goes through those of its word
+  auto few_of = [&](int32_t b, uint32_t word) {
+    const int32_t lane = threadIdx.x & 31, t0 = row.token(b * 128) + lane * 32;
+    if (lane >= 4 * kEpv) word = 0;
+    while (__any_sync(kFull, word != 0)) {
+      int32_t t[4];
+      float x[4], e[4], q[4], over = 0.0f;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            t[u] = t0 + __ffs(word) - 1;
-            const bool in = word != 0 && t[u] != without;
-            x[u] = in ? row.at(t[u]) : -INFINITY;
-            e[u] = in ? __ldg(noise + t[u]) : 0.0f;
-            q[u] = in && given.p ? load_prob(given.p, given.dtype, t[u]) : 0.0f;
-            word &= word - 1;
-          }
-          const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
-          float over = 0.0f;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            x[u] = fmaf(exp2_fast(fmaf(x[u], c, -ref)), fix, -q[u]);
-            over = fmaxf(over, fmaf(-bar, e[u], x[u]));
-          }
-          if (over > 0.0f) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float f = fmaxf(__fdividef(x[u], e[u]), 0.0f);
-              if (x[u] > 0.0f && f > top) {
-                top = f;
-                idx = t[u];
-              }
-            }
-            if (top > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(top, kMostScore)));
-          }
-        }
-        return;
+      for (int u = 0; u < 4; ++u) {
+        t[u] = t0 + __ffs(word) - 1;
+        const bool in = word != 0 && t[u] != without;
+        x[u] = in ? row.at(t[u]) : -INFINITY;
+        e[u] = in ? __ldg(noise + t[u]) : 0.0f;
+        q[u] = in && given.p ? load_prob(given.p, given.dtype, t[u]) : 0.0f;
+        word &= word - 1;
       }
-      const int32_t j0 = at * 128 + static_cast<int32_t>(threadIdx.x & 31);
+      const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
 #pragma unroll
-      for (int q0 = 0; q0 < 4; q0 += 2) {
-        uint32_t keep[2];
-        uint4 v[2];
-        float e[2][kEpv], left[2][kEpv];
+      for (int u = 0; u < 4; ++u) {
+        x[u] = fmaf(exp2_fast(fmaf(x[u], c, -ref)), fix, -q[u]);
+        over = fmaxf(over, fmaf(-bar, e[u], x[u]));
+      }
+      if (over > 0.0f) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          keep[q] = Row<T>::keep(word, q0 + q);
-          const int32_t j = j0 + (q0 + q) * 32, t = row.token(j);
+        for (int u = 0; u < 4; ++u) look(x[u], e[u], t[u]);
+        raise();
+      }
+    }
+  };
+  auto block = [&](int32_t b, const uint32_t (&word)[1]) {
+    if (few<T>(__popc(word[0]), 1)) {
+      few_of(b, word[0]);
+      return;
+    }
+    const int32_t j0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
 #pragma unroll
-          for (int i = 0; i < kEpv; ++i) left[q][i] = 0.0f;
-          if (keep[q]) {
-            v[q] = row.vec(j);
-            load_floats<kEpv>(noise + t, noise_fits, e[q]);
-            if (given.p) given.load<kEpv>(t, given_fits, left[q]);
-            if (static_cast<uint32_t>(without - t) < static_cast<uint32_t>(kEpv))
-              keep[q] &= ~(1u << (without - t));
-          }
-        }
-        const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+    for (int q0 = 0; q0 < 4; q0 += kRaceVecs) {
+      uint32_t keep[kRaceVecs];
+      uint4 v[kRaceVecs];
+      float e[kRaceVecs][kEpv], left[kRaceVecs][kEpv];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          if (!keep[q]) continue;
-          const uint4 x = masked<T>(v[q], keep[q], sh.lanes);
-          float over = 0.0f;
+      for (int q = 0; q < kRaceVecs; ++q) {
+        keep[q] = Row<T>::keep(word[0], q0 + q);
+        const int32_t j = j0 + (q0 + q) * 32, t = row.token(j);
 #pragma unroll
-          for (int i = 0; i < kEpv; ++i) {
-            const float f = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
-            left[q][i] = fmaf(f, fix, -left[q][i]);
-            over = fmaxf(over, (keep[q] >> i) & 1u ? fmaf(-bar, e[q][i], left[q][i]) : 0.0f);
-          }
-          if (over > 0.0f) {
-#pragma unroll
-            for (int i = 0; i < kEpv; ++i) {
-              const float f = fmaxf(__fdividef(left[q][i], e[q][i]), 0.0f);
-              if ((keep[q] >> i) & 1u && left[q][i] > 0.0f && f > top) {
-                top = f;
-                idx = row.token(j0 + (q0 + q) * 32) + i;
-              }
-            }
-            if (top > 0.0f) atomicMax(&sh.bar, __float_as_uint(fminf(top, kMostScore)));
-          }
+        for (int i = 0; i < kEpv; ++i) left[q][i] = 0.0f;
+        if (keep[q]) {
+          v[q] = row.vec(j);
+          load_floats<kEpv>(noise + t, noise_fits, e[q]);
+          if (given.p) given.load<kEpv>(t, given_fits, left[q]);
+          if (static_cast<uint32_t>(without - t) < static_cast<uint32_t>(kEpv))
+            keep[q] &= ~(1u << (without - t));
         }
       }
-  });
+      const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
+#pragma unroll
+      for (int q = 0; q < kRaceVecs; ++q) {
+        if (!keep[q]) continue;
+        const uint4 x = masked<T>(v[q], keep[q], sh.lanes);
+        float over = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kEpv; ++i) {
+          const float f = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
+          left[q][i] = fmaf(f, fix, -left[q][i]);
+          over = fmaxf(over, (keep[q] >> i) & 1u ? fmaf(-bar, e[q][i], left[q][i]) : 0.0f);
+        }
+        if (over > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < kEpv; ++i)
+            if ((keep[q] >> i) & 1u) look(left[q][i], e[q][i], row.token(j0 + (q0 + q) * 32) + i);
+          raise();
+        }
+      }
+    }
+  };
+  each_block<1>(row, ok, chunk, chunks, V, block);
   if (idx >= 0) offer(idx);
   row.edges(chunk, chunks, V, offer);
   return block_max(won, sh.warps);
@@ -1006,7 +949,7 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
   __shared__ ScanShared sh;
   const int32_t chunk = static_cast<int32_t>(blockIdx.x % chunks);
   const int32_t b = static_cast<int32_t>(blockIdx.x / chunks);
-  const int32_t tid = threadIdx.x, lane = tid & 31, K = a.K, V = a.V;
+  const int32_t tid = threadIdx.x, lane = tid & 31, K = a.max_drafts, V = a.vocab_size;
   if (sizeof(typename Dt<T>::Bits) == 2) sh.lanes.fill();
   if (tid == 0) sh.bar = order_key(-INFINITY);
   pdl_trigger();
@@ -1087,31 +1030,35 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
       t = token;
       logprob = (x == p.m ? 0.0f : (x - p.m) * inv) - logf(p.s);
     }
-    a.tokens[out] = t;
-    a.logprobs[out] = logprob;
+    a.tokens_out[out] = t;
+    a.logprobs_out[out] = logprob;
   }
   if (lane == 0) {
-    a.counts[b] = n + (token >= 0);
+    a.counts_out[b] = n + (token >= 0);
     if (a.tok_next) {
       const int32_t next = token < 0 ? -1 : step(a, p.state, token);
       if (a.next_out) a.next_out[b] = next;
-      if (a.write_back) a.pool[a.slots ? a.slots[b] : b] = next;
+      if (a.write_back) a.state_pool[a.slots ? a.slots[b] : b] = next;
     }
   }
 }
 
 // ---------------------------------------------------------------------------
 
-// Chunks of a row: CTAs that fill the SMs' room (`room` CTAs) in whole waves as
-// nearly as can be, each chunk with a block of 128 vectors for every warp; a
-// cost for each more.
+// Chunks of a row, each a CTA: by what `rows` of them cost on `room` places,
+// where a chunk costs its share of the row and a twentieth of a row besides
+// (the loads that depend on one another, 3 us), and the last ones leave places
+// idle for half their time. No chunk has less than a block of 128 vectors for
+// every warp. Measured: 1024 rows of 128,256 in 16 bits with noise 141 us in
+// one or two chunks, 146 in four; 128 rows x 2 drafts 58 us in one, 46 in four.
 int32_t chunks_of(int64_t rows, int32_t vocab, int32_t vec, int64_t room) {
-  const int64_t most = std::min<int64_t>(kMaxChunks, (static_cast<int64_t>(vocab) / vec + 1023) / 1024);
+  const int64_t most =
+      std::min<int64_t>(kMaxChunks, (static_cast<int64_t>(vocab) / vec + 1023) / 1024);
   int32_t best = 1;
   double least = 0.0;
   for (int32_t c = 1; c <= most; ++c) {
-    const int64_t waves = (rows * c + room - 1) / room;
-    const double cost = static_cast<double>(waves) * (1.0 / c + CC);
+    const double waves = static_cast<double>(rows * c) / room;
+    const double cost = std::max(1.0, waves) * (1.0 / c + 0.05) + (waves > 1.0 ? 0.5 / c : 0.0);
     if (c == 1 || cost < least) {
       least = cost;
       best = c;
@@ -1145,63 +1092,56 @@ extern "C" size_t bpd_verify_workspace_bytes(int32_t batch, int32_t max_drafts) 
          align256(static_cast<size_t>(batch) * (max_drafts + 1) * kMaxChunks * sizeof(Part));
 }
 
-extern "C" bpd_status bpd_verify_drafts(
-    const void* src, int32_t src_dtype, int64_t src_stride, int64_t src_total,
-    const int64_t* src_rows, const void* drafts, int32_t drafts_int64, int64_t draft_stride,
-    const int32_t* draft_lens, const void* probs, int32_t probs_dtype, int64_t probs_stride,
-    int64_t probs_total, const int64_t* prob_rows, const float* uniforms, int64_t uniform_stride,
-    const float* noise, int64_t noise_stride, const float* temperature, float temperature_all,
-    int32_t batch, int32_t max_drafts, int32_t vocab_size, int32_t* state_pool,
-    const int64_t* slots, const int32_t* path, const uint32_t* allow_bits, int32_t words_stride,
-    const int32_t* tok_next, int32_t num_states, int64_t* tokens_out, int32_t* counts_out,
-    float* logprobs_out, int32_t* next_out, int32_t write_back, void* workspace, void* stream) {
+extern "C" bpd_status bpd_verify_drafts(const bpd_verify_args* args, void* stream) {
   const char* what = "bpd_verify_drafts";
-  BPD_REQUIRE(batch >= 0 && vocab_size > 0 && max_drafts >= 0 && src_total >= 0,
+  BPD_REQUIRE(args, "%s: null pointer", what);
+  bpd_verify_args a = *args;
+  BPD_REQUIRE(a.batch >= 0 && a.vocab_size > 0 && a.max_drafts >= 0 && a.src_total >= 0,
               "%s: bad sizes", what);
-  if (max_drafts > BPD_MAX_DRAFTS)
+  if (a.max_drafts > BPD_MAX_DRAFTS)
     return fail(BPD_ERR_CAPACITY, "%s: more than %d drafts", what, BPD_MAX_DRAFTS);
-  if (batch == 0) return BPD_OK;
-  BPD_REQUIRE(src && tokens_out && counts_out && logprobs_out && workspace, "%s: null pointer", what);
-  BPD_REQUIRE(aligned16(workspace), "%s: the workspace must be 16-byte aligned", what);
-  BPD_REQUIRE(src_stride >= vocab_size, "%s: row stride < vocab", what);
-  BPD_REQUIRE(max_drafts == 0 || (drafts && draft_stride >= max_drafts),
+  if (a.batch == 0) return BPD_OK;
+  BPD_REQUIRE(a.src && a.tokens_out && a.counts_out && a.logprobs_out && a.workspace,
+              "%s: null pointer", what);
+  BPD_REQUIRE(aligned16(a.workspace), "%s: the workspace must be 16-byte aligned", what);
+  BPD_REQUIRE(a.src_stride >= a.vocab_size, "%s: row stride < vocab", what);
+  BPD_REQUIRE(a.max_drafts == 0 || (a.drafts && a.draft_stride >= a.max_drafts),
               "%s: drafts missing, or their row stride < max_drafts", what);
-  const bool all_greedy = temperature == nullptr && !(temperature_all > 0.0f);
-  BPD_REQUIRE(all_greedy || (noise && noise_stride >= vocab_size),
+  const bool all_greedy = a.temperature == nullptr && !(a.temperature_all > 0.0f);
+  BPD_REQUIRE(all_greedy || (a.noise && a.noise_stride >= a.vocab_size),
               "%s: sampling needs a row of noise for each request", what);
-  BPD_REQUIRE(all_greedy || max_drafts == 0 || (uniforms && uniform_stride >= max_drafts),
+  BPD_REQUIRE(all_greedy || a.max_drafts == 0 ||
+                  (a.uniforms && a.uniform_stride >= a.max_drafts),
               "%s: sampling needs a uniform number for each draft", what);
-  BPD_REQUIRE(!probs || (probs_stride >= vocab_size && probs_total >= 0 && probs_dtype >= BPD_F32 &&
-                         probs_dtype <= BPD_F16),
+  BPD_REQUIRE(!a.probs || (a.probs_stride >= a.vocab_size && a.probs_total >= 0 &&
+                           a.probs_dtype >= BPD_F32 && a.probs_dtype <= BPD_F16),
               "%s: bad draft probabilities", what);
-  BPD_REQUIRE(!allow_bits || (words_stride >= (vocab_size + 31) / 32 && num_states > 0),
+  BPD_REQUIRE(!a.allow_bits ||
+                  (a.words_stride >= (a.vocab_size + 31) / 32 && a.num_states > 0),
               "%s: words_stride too small, or no states", what);
-  BPD_REQUIRE(!allow_bits || path || (state_pool && tok_next),
+  BPD_REQUIRE(!a.allow_bits || a.path || (a.state_pool && a.tok_next),
               "%s: a grammar needs state_pool and tok_next, or path", what);
-  BPD_REQUIRE((!next_out && !write_back) || (state_pool && tok_next && allow_bits),
+  BPD_REQUIRE((!a.next_out && !a.write_back) || (a.state_pool && a.tok_next && a.allow_bits),
               "%s: next states need state_pool, allow_bits and tok_next", what);
-  const VerifyArgs a{src, src_stride, src_total, src_rows, drafts, draft_stride, drafts_int64,
-                     draft_lens, probs, probs_dtype, probs_stride, probs_total, prob_rows,
-                     uniforms, uniform_stride, noise, noise_stride, temperature, temperature_all,
-                     batch, max_drafts, vocab_size, state_pool, slots, path, allow_bits,
-                     words_stride, allow_bits ? tok_next : nullptr, num_states, tokens_out,
-                     counts_out, logprobs_out, next_out, write_back};
+  if (!a.allow_bits) a.tok_next = nullptr;
   cudaStream_t st = as_stream(stream);
-  return with_dtype(src_dtype, what, [&](auto tag) {
+  return with_dtype(a.src_dtype, what, [&](auto tag) {
     using T = decltype(tag);
-    const int64_t rows = static_cast<int64_t>(batch) * max_drafts;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.max_drafts, sms = sm_count();
     Workspace w{};
-    lay_out(batch, max_drafts, workspace, &w);
-    const int32_t chunks = chunks_of(rows, vocab_size, Dt<T>::kPerVec, kScanCtas * static_cast<int64_t>(sm_count()));
-    const int32_t lasts = chunks_of(batch, vocab_size, Dt<T>::kPerVec, kLastCtas * static_cast<int64_t>(sm_count()));
-    if (std::max(rows * chunks, static_cast<int64_t>(batch) * lasts) > INT_MAX)
+    lay_out(a.batch, a.max_drafts, a.workspace, &w);
+    const int32_t chunks =
+        chunks_of(rows, a.vocab_size, Dt<T>::kPerVec, kScanCtas * sms);
+    const int32_t lasts =
+        chunks_of(a.batch, a.vocab_size, Dt<T>::kPerVec, kLastCtas * sms);
+    if (std::max(rows * chunks, static_cast<int64_t>(a.batch) * lasts) > INT_MAX)
       return fail(BPD_ERR_CAPACITY, "%s: batch too large", what);
-    cudaError_t e = launch_pdl(walk_kernel<T>, dim3((batch + 3) / 4), dim3(128), 0, st, a, w);
-    if (e == cudaSuccess && max_drafts)
+    cudaError_t e = launch_pdl(walk_kernel<T>, dim3((a.batch + 3) / 4), dim3(128), 0, st, a, w);
+    if (e == cudaSuccess && a.max_drafts)
       e = launch_pdl(scan_kernel<T>, dim3(static_cast<unsigned>(rows * chunks)),
                      dim3(kScanThreads), 0, st, a, w, chunks);
     if (e == cudaSuccess)
-      e = launch_pdl(last_kernel<T>, dim3(static_cast<unsigned>(batch) * lasts),
+      e = launch_pdl(last_kernel<T>, dim3(static_cast<unsigned>(a.batch) * lasts),
                      dim3(kScanThreads), 0, st, a, w, lasts);
     return e == cudaSuccess ? BPD_OK : fail(BPD_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   });

@@ -16,14 +16,21 @@ the states that a batch keeps, and commit them.
 
 from __future__ import annotations
 
+import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
 
 from . import _capi
-from .ops import _DTYPE_CODE, FsaTensors, _as_i32, _ptr, _require_cuda, _stream, on_device
+from .ops import _DTYPE_CODE, FsaTensors, _as_i32, _require_cuda, _stream, on_device
 
 MAX_DRAFTS = 31  # BPD_MAX_DRAFTS
+
+_FLOATS = tuple(_DTYPE_CODE)
+_INTS = (torch.int32, torch.int64)
+_F32 = (torch.float32,)
+_INF = float("inf")
 
 
 class VerifyResult(NamedTuple):
@@ -35,75 +42,86 @@ class VerifyResult(NamedTuple):
     states: torch.Tensor | None  # int32 [B]: the grammar state behind the last one
 
 
+_ARGS = struct.Struct("=26q9if")  # bpd_verify_args: 26 pointers and strides, then the rest
+assert _ARGS.size == ctypes.sizeof(_capi.VerifyArgs)
+
+
+def _bad(what: str, why: str, t: torch.Tensor) -> RuntimeError:
+    return RuntimeError(f"bpdecode_b200: {what} {why}, got {tuple(t.shape)} {t.dtype} on "
+                        f"{t.device}, strides {t.stride()}")
+
+
 def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, dtypes: tuple,
+            device: torch.device) -> tuple[int, int]:
+    """(pointer, row stride) of a matrix of at least [rows, cols]."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] < cols:
+        raise _bad(what, f"must be [{rows}, {cols}] or larger", t)
+    if t.dtype not in dtypes or t.device != device:
+        raise _bad(what, f"must be one of {dtypes} on {device}", t)
+    stride, step = t.stride()
+    if shape[0] <= 1:
+        stride = max(shape[1], 1)
+    if cols and (step != 1 and shape[1] > 1 or stride < cols):
+        raise _bad(what, "needs contiguous columns and rows that do not overlap", t)
+    return t.data_ptr(), stride
+
+
+def _vector(t: torch.Tensor, what: str, n: int, dtype: torch.dtype,
             device: torch.device) -> torch.Tensor:
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
-        raise RuntimeError(f"bpdecode_b200: {what} must be [{rows}, {cols}] or larger, got "
-                           f"{tuple(t.shape)}")
-    if t.dtype not in dtypes:
-        raise RuntimeError(f"bpdecode_b200: unsupported {what} dtype {t.dtype}")
-    if t.device != device:
-        raise RuntimeError(f"bpdecode_b200: {what} must be on {device}")
-    if cols and (t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols):
-        raise RuntimeError(f"bpdecode_b200: {what} needs contiguous columns and rows that do not "
-                           f"overlap (strides {t.stride()})")
-    return t
-
-
-def _stride(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else max(int(t.shape[1]), 1)
-
-
-def _vector(t: torch.Tensor | None, what: str, n: int, dtype: torch.dtype,
-            device: torch.device) -> torch.Tensor | None:
-    if t is None:
-        return None
     if t.dtype != dtype or t.shape != (n,) or t.device != device:
-        raise RuntimeError(f"bpdecode_b200: {what} must be {dtype} [{n}] on {device}")
+        raise _bad(what, f"must be {dtype} [{n}] on {device}", t)
     return t.contiguous()
 
 
 def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, src_rows,
             prob_rows, batch, vocab, pool, slot_ptr, path, bits, tok_next, num_states,
             states, write_back) -> VerifyResult:
-    """Check the arguments that every form shares and enqueue the kernel."""
+    """Check the arguments that every form shares and enqueue the kernels."""
     _require_cuda(src, "src")
     dev, B, V = src.device, batch, vocab
-    _matrix(src, "src", 0, V, tuple(_DTYPE_CODE), dev)
-    if drafts is None:
-        K = 0
-    else:
+    src_ptr, src_stride = _matrix(src, "src", 0, V, _FLOATS, dev)
+    K = draft_ptr = draft_stride = drafts64 = 0
+    if drafts is not None:
         if drafts.dim() != 2:
             raise RuntimeError("bpdecode_b200: drafts must be [batch, drafts]")
-        K = int(drafts.shape[1])
-        _matrix(drafts, "drafts", B, K, (torch.int32, torch.int64), dev)
-    if K > MAX_DRAFTS:
-        raise RuntimeError(f"bpdecode_b200: at most {MAX_DRAFTS} drafts ({K})")
-    src_rows = _vector(src_rows, "src_rows", B, torch.int64, dev)
-    if src_rows is None and src.shape[0] < B * (K + 1):
+        K = drafts.shape[1]
+        draft_ptr, draft_stride = _matrix(drafts, "drafts", B, K, _INTS, dev)
+        drafts64 = int(drafts.dtype is torch.int64)
+        if K > MAX_DRAFTS:
+            raise RuntimeError(f"bpdecode_b200: at most {MAX_DRAFTS} drafts ({K})")
+    rows_ptr = lens_ptr = heat_ptr = prows_ptr = 0
+    if src_rows is not None:
+        src_rows = _vector(src_rows, "src_rows", B, torch.int64, dev)
+        rows_ptr = src_rows.data_ptr()
+    elif src.shape[0] < B * (K + 1):
         raise RuntimeError("bpdecode_b200: src has fewer rows than the requests' drafts + 1")
-    draft_lens = _vector(draft_lens, "draft_lens", B, torch.int32, dev)
-    heat, everywhere = None, 1.0
+    if draft_lens is not None:
+        draft_lens = _vector(draft_lens, "draft_lens", B, torch.int32, dev)
+        lens_ptr = draft_lens.data_ptr()
+    everywhere = 1.0
     if isinstance(temperature, torch.Tensor):
-        heat = _vector(temperature, "temperature", B, torch.float32, dev)
+        temperature = _vector(temperature, "temperature", B, torch.float32, dev)
+        heat_ptr = temperature.data_ptr()
     else:
         everywhere = float(temperature)
-        if not 0.0 <= everywhere < float("inf"):
+        if not 0.0 <= everywhere < _INF:
             raise ValueError(f"temperature must be finite and not negative, got {temperature}")
-    if heat is not None or everywhere > 0.0:
-        if noise is None or (uniforms is None and K):
-            raise RuntimeError("bpdecode_b200: sampling needs noise, and uniforms for drafts")
-    f32 = (torch.float32,)
+    if (heat_ptr or everywhere > 0.0) and (noise is None or (uniforms is None and K)):
+        raise RuntimeError("bpdecode_b200: sampling needs noise, and uniforms for drafts")
+    noise_ptr = noise_stride = uni_ptr = uni_stride = 0
     if noise is not None:
-        _matrix(noise, "noise", B, V, f32, dev)
+        noise_ptr, noise_stride = _matrix(noise, "noise", B, V, _F32, dev)
     if uniforms is not None:
-        _matrix(uniforms, "uniforms", B, K, f32, dev)
-    if K == 0:
-        draft_probs = prob_rows = None
+        uni_ptr, uni_stride = _matrix(uniforms, "uniforms", B, K, _F32, dev)
+    probs_ptr = probs_stride = probs_rows = probs_code = 0
     if draft_probs is not None:
-        _matrix(draft_probs, "draft_probs", 0, V, tuple(_DTYPE_CODE), dev)
-        prob_rows = _vector(prob_rows, "prob_rows", B, torch.int64, dev)
-        if prob_rows is None and draft_probs.shape[0] < B * K:
+        probs_ptr, probs_stride = _matrix(draft_probs, "draft_probs", 0, V, _FLOATS, dev)
+        probs_rows, probs_code = draft_probs.shape[0], _DTYPE_CODE[draft_probs.dtype]
+        if prob_rows is not None:
+            prob_rows = _vector(prob_rows, "prob_rows", B, torch.int64, dev)
+            prows_ptr = prob_rows.data_ptr()
+        elif probs_rows < B * K:
             raise RuntimeError("bpdecode_b200: draft_probs has fewer rows than the drafts")
     elif prob_rows is not None:
         raise RuntimeError("bpdecode_b200: prob_rows without draft_probs")
@@ -112,20 +130,17 @@ def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, 
     logprobs = torch.empty((B, K + 1), dtype=torch.float32, device=dev)
     L = _capi.lib()
     work = torch.empty(L.bpd_verify_workspace_bytes(B, K), dtype=torch.uint8, device=dev)
+    args = _ARGS.pack(
+        src_ptr, src_stride, src.shape[0], rows_ptr, draft_ptr, draft_stride, lens_ptr, probs_ptr,
+        probs_stride, probs_rows, prows_ptr, uni_ptr, uni_stride, noise_ptr, noise_stride,
+        heat_ptr, 0 if pool is None else pool.data_ptr(), slot_ptr or 0,
+        0 if path is None else path.data_ptr(), 0 if bits is None else bits.data_ptr(),
+        0 if tok_next is None else tok_next.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
+        logprobs.data_ptr(), 0 if states is None else states.data_ptr(), work.data_ptr(),
+        _DTYPE_CODE[src.dtype], drafts64, probs_code, B, K, V,
+        0 if bits is None else bits.shape[1], num_states, write_back, everywhere)
     with on_device(dev):
-        L.check(L.bpd_verify_drafts(
-            src.data_ptr(), _DTYPE_CODE[src.dtype], max(_stride(src), V), src.shape[0],
-            _ptr(src_rows), _ptr(drafts) if K else None, int(K > 0 and drafts.dtype == torch.int64),
-            _stride(drafts), _ptr(draft_lens), _ptr(draft_probs),
-            0 if draft_probs is None else _DTYPE_CODE[draft_probs.dtype],
-            0 if draft_probs is None else max(_stride(draft_probs), V),
-            0 if draft_probs is None else draft_probs.shape[0], _ptr(prob_rows),
-            _ptr(uniforms), _stride(uniforms), _ptr(noise),
-            0 if noise is None else max(_stride(noise), V), _ptr(heat), everywhere, B, K, V,
-            _ptr(pool), slot_ptr, _ptr(path), _ptr(bits), 0 if bits is None else bits.shape[1],
-            _ptr(tok_next), num_states, tokens.data_ptr(), counts.data_ptr(),
-            logprobs.data_ptr(), _ptr(states), int(write_back),
-            work.data_ptr(), _stream(src)))
+        L.check(L.bpd_verify_drafts(args, _stream(src)))
     return VerifyResult(tokens, counts, logprobs, states)
 
 

@@ -392,61 +392,87 @@ bpd_status bpd_lora_project(
 
 #define BPD_MAX_DRAFTS 31
 
+/* The arguments of bpd_verify_drafts: device pointers (optional where marked:
+ * NULL), and sizes in elements. */
+typedef struct bpd_verify_args {
+  const void* src;            /* logits, src_dtype */
+  int64_t src_stride;
+  int64_t src_total;          /* rows of src */
+  const int64_t* src_rows;    /* [batch], optional */
+  const void* drafts;         /* int32, or int64 if drafts_int64 */
+  int64_t draft_stride;
+  const int32_t* draft_lens;  /* [batch], optional */
+  const void* probs;          /* probs_dtype, optional */
+  int64_t probs_stride;
+  int64_t probs_total;        /* rows of probs */
+  const int64_t* prob_rows;   /* [batch], optional */
+  const float* uniforms;
+  int64_t uniform_stride;
+  const float* noise;
+  int64_t noise_stride;
+  const float* temperature;   /* [batch], optional: temperature_all */
+  int32_t* state_pool;        /* optional */
+  const int64_t* slots;       /* [batch], optional */
+  const int32_t* path;        /* [batch, max_drafts + 1], optional */
+  const uint32_t* allow_bits; /* [num_states, words_stride], optional */
+  const int32_t* tok_next;    /* [num_states, vocab_size], optional */
+  int64_t* tokens_out;        /* [batch, max_drafts + 1] */
+  int32_t* counts_out;        /* [batch] */
+  float* logprobs_out;        /* [batch, max_drafts + 1] */
+  int32_t* next_out;          /* [batch], optional */
+  void* workspace;            /* bpd_verify_workspace_bytes, 16-byte aligned */
+  int32_t src_dtype;
+  int32_t drafts_int64;
+  int32_t probs_dtype;
+  int32_t batch;
+  int32_t max_drafts;
+  int32_t vocab_size;
+  int32_t words_stride;
+  int32_t num_states;
+  int32_t write_back;
+  float temperature_all;
+} bpd_verify_args;
+
 /* Verify drafted tokens against the target's probabilities, from random
  * numbers that the caller gives, under each request's grammar; with no drafts,
  * sample one token for each request.
  *
  * Request b brings len = draft_lens[b] (NULL: max_drafts) drafts
- * drafts[b * draft_stride + i] (int32, or int64 if drafts_int64) and len + 1
- * rows of logits: rows src_rows[b] .. src_rows[b] + len of `src` (NULL:
- * b * (max_drafts + 1)), which has src_total rows src_stride elements apart.
- * Row i keeps the tokens that the state after the first i drafts allows; a
- * NaN logit counts as -inf. With p = softmax(row / T):
+ * drafts[b * draft_stride + i] and len + 1 rows of logits: rows src_rows[b] ..
+ * src_rows[b] + len of `src` (NULL: b * (max_drafts + 1)), src_stride elements
+ * apart. Row i keeps the tokens that the state after the first i drafts
+ * allows; a NaN logit counts as -inf. With p = softmax(row / T):
  *   draft d is accepted iff u * q[d] < p[d]
  *   the first that is not is replaced by argmax(max(p - q, 0) / e), or by
  *   argmax(p / e) where p - q leaves nothing
  *   behind the last one comes argmax(p / e)
  * with u = uniforms[b * uniform_stride + i] in [0, 1), e = noise + b *
  * noise_stride (exponential, > 0) and q row prob_rows[b] + i (NULL: b *
- * max_drafts + i) of `probs` (probs_total rows, probs_dtype; entries below 0
- * or NaN are not defined). probs == NULL: q is 1 at the draft, 0 elsewhere.
- * Equal scores go to the lowest index. T = temperature[b], or temperature_all
- * where that is NULL; T <= 0 (or NaN) is greedy: a draft is accepted iff it is
- * the first maximal token, which otherwise replaces it; noise and uniforms may
- * be NULL where temperature is NULL and temperature_all <= 0.
+ * max_drafts + i) of `probs` (entries below 0 or NaN are not defined).
+ * probs == NULL: q is 1 at the draft, 0 elsewhere. Equal scores go to the
+ * lowest index. T = temperature[b], or temperature_all; T <= 0 (or NaN) is
+ * greedy: a draft is accepted iff it is the first maximal token, which
+ * otherwise replaces it; noise and uniforms may be NULL where temperature is
+ * NULL and temperature_all <= 0.
  *
- * Grammar: allow_bits [num_states, words_stride] (NULL: none) with tok_next
- * [num_states, vocab] walked from state_pool[slots[b]] along the drafts; or
- * path int32 [batch, max_drafts + 1], the row of allow_bits for each
- * position. A negative or too large state allows nothing.
+ * Grammar: allow_bits (NULL: none) with tok_next walked from
+ * state_pool[slots[b]] along the drafts; or path, the row of allow_bits for
+ * each position. A negative or too large state allows nothing.
  *
- * tokens_out int64 [batch, max_drafts + 1]: the accepted drafts and the token
- * behind them, then -1. counts_out int32 [batch]: how many those are.
- * logprobs_out float [batch, max_drafts + 1]: their log p (at T = 1 for greedy
- * requests), then 0. At a position where nothing is allowed (no token, or none
- * above -inf) the request ends without a token. next_out int32 [batch] (may be
- * NULL) and, if write_back, state_pool[slots[b]]: the state behind the last
- * token, -1 where the request ended without one. Tokens behind an accepted
- * end-of-sequence token are the caller's to drop.
+ * tokens_out: the accepted drafts and the token behind them, then -1.
+ * counts_out: how many those are. logprobs_out: their log p (at T = 1 for
+ * greedy requests), then 0. At a position where nothing is allowed (no token,
+ * or none above -inf) the request ends without a token. next_out and, if
+ * write_back, state_pool[slots[b]]: the state behind the last token, -1 where
+ * the request ended without one. Tokens behind an accepted end-of-sequence
+ * token are the caller's to drop.
  *
  * A request with len < 0 or > max_drafts, or rows outside src or probs, is
  * idle: no tokens, count 0, its state as it was. max_drafts <= BPD_MAX_DRAFTS.
- * slots of one call must be distinct. workspace: bpd_verify_workspace_bytes,
- * 16-byte aligned, any contents. */
+ * slots of one call must be distinct. The workspace may hold anything; calls
+ * that share one must be ordered. */
 size_t bpd_verify_workspace_bytes(int32_t batch, int32_t max_drafts);
-bpd_status bpd_verify_drafts(
-    const void* src, int32_t src_dtype, int64_t src_stride, int64_t src_total,
-    const int64_t* src_rows, const void* drafts, int32_t drafts_int64,
-    int64_t draft_stride, const int32_t* draft_lens, const void* probs,
-    int32_t probs_dtype, int64_t probs_stride, int64_t probs_total,
-    const int64_t* prob_rows, const float* uniforms, int64_t uniform_stride,
-    const float* noise, int64_t noise_stride, const float* temperature,
-    float temperature_all, int32_t batch, int32_t max_drafts, int32_t vocab_size,
-    int32_t* state_pool, const int64_t* slots, const int32_t* path,
-    const uint32_t* allow_bits, int32_t words_stride, const int32_t* tok_next,
-    int32_t num_states, int64_t* tokens_out, int32_t* counts_out,
-    float* logprobs_out, int32_t* next_out, int32_t write_back, void* workspace,
-    void* stream);
+bpd_status bpd_verify_drafts(const bpd_verify_args* args, void* stream);
 
 /* --------------------------------------------------------------------------
  * Continuous-batching turnover on the device (NEW; the reference leaves the
