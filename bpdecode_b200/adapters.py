@@ -21,6 +21,7 @@ from . import _capi
 from .ops import _DTYPE_CODE, _require_cuda, _stream, on_device
 
 MAX_RANK = 128  # BPD_LORA_MAX_RANK
+_TYPES = (torch.bfloat16, torch.float16)
 _TILE = 128  # outputs of one tile of the packed B
 
 
@@ -99,11 +100,13 @@ class AdapterBank:
 
 def _check_rows(t: torch.Tensor, what: str, cols: int, dtype: torch.dtype) -> int:
     """The row stride of a matrix whose rows start on 16-byte boundaries."""
-    if t.dim() != 2 or t.shape[1] != cols or t.dtype != dtype:
+    stride, step = t.stride()
+    if t.shape[0] <= 1:
+        stride = (cols + 7) // 8 * 8
+    if t.shape[1] != cols or t.dtype != dtype:
         raise RuntimeError(f"bpdecode_b200: {what} must be [rows, {cols}] {dtype}, got "
                            f"{tuple(t.shape)} {t.dtype}")
-    stride = t.stride(0) if t.shape[0] > 1 else (cols + 7) // 8 * 8
-    if t.stride(1) != 1 or stride < cols or stride % 8 or t.data_ptr() % 16:
+    if step != 1 or stride < cols or stride % 8 or t.data_ptr() % 16:
         raise RuntimeError(f"bpdecode_b200: {what} needs contiguous columns and rows that start "
                            f"on 16-byte boundaries (strides {t.stride()})")
     return stride
@@ -127,53 +130,54 @@ def project(
     (contiguous columns, any row stride). Launches on torch's current stream
     without synchronising."""
     _require_cuda(x, "x")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError(f"bpdecode_b200: unsupported dtype {x.dtype}")
-    if weight.device != x.device:
+    dtype, dev = x.dtype, x.device
+    if dtype not in _TYPES:
+        raise RuntimeError(f"bpdecode_b200: unsupported dtype {dtype}")
+    if weight.device != dev:
         raise RuntimeError("bpdecode_b200: x and weight live on different devices")
     if x.dim() != 2 or weight.dim() != 2:
         raise RuntimeError("bpdecode_b200: x and weight are matrices")
-    T, K = int(x.shape[0]), int(x.shape[1])
-    N = int(weight.shape[0])
+    T, K = x.shape
+    N = weight.shape[0]
     if K % 8:
         raise RuntimeError("bpdecode_b200: in_features must be a multiple of 8")
-    xs = _check_rows(x, "x", K, x.dtype)
-    ws = _check_rows(weight, "weight", K, x.dtype)
+    xs = _check_rows(x, "x", K, dtype)
+    ws = _check_rows(weight, "weight", K, dtype)
     if (bank is None) != (adapter_ids is None):
         raise RuntimeError("bpdecode_b200: bank and adapter_ids come together")
     if out is None:
-        out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=x.device)
-    elif (out.shape != (T, N) or out.device != x.device
+        out = torch.empty((T, N), dtype=out_dtype or dtype, device=dev)
+    elif (out.shape != (T, N) or out.device != dev
           or (out_dtype is not None and out.dtype != out_dtype) or (N > 1 and out.stride(1) != 1)
           or (T > 1 and out.stride(0) < N)):
         raise RuntimeError(f"bpdecode_b200: out must be [{T}, {N}] with contiguous columns")
-    if out.dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"bpdecode_b200: the result is {x.dtype} or fp32, not {out.dtype}")
+    if out.dtype is not dtype and out.dtype is not torch.float32:
+        raise RuntimeError(f"bpdecode_b200: the result is {dtype} or fp32, not {out.dtype}")
     L = _capi.lib()
-    a = b = scale = ids = ws_ptr = work = None
+    a = b = scale = ids_ptr = work_ptr = None
     n = rank = ids64 = 0
     if bank is not None:
-        if bank.device != x.device or bank.dtype != x.dtype:
+        if bank.device != dev or bank.dtype != dtype:
             raise RuntimeError(f"bpdecode_b200: the bank is {bank.dtype} on {bank.device}")
         if (bank.in_features, bank.out_features) != (K, N):
             raise RuntimeError(f"bpdecode_b200: the bank is for [{bank.out_features}, "
                                f"{bank.in_features}], the weight is [{N}, {K}]")
-        if (adapter_ids.dtype not in (torch.int32, torch.int64) or adapter_ids.shape != (T,)
-                or adapter_ids.device != x.device):
+        ids64 = int(adapter_ids.dtype is torch.int64)
+        if ((not ids64 and adapter_ids.dtype is not torch.int32) or adapter_ids.shape != (T,)
+                or adapter_ids.device != dev):
             raise RuntimeError("bpdecode_b200: adapter_ids must be int32 or int64 [rows] on the "
                                "device")
-        ids = adapter_ids.contiguous()
-        ids64 = int(ids.dtype == torch.int64)
+        adapter_ids = adapter_ids.contiguous()
+        ids_ptr = adapter_ids.data_ptr()
         a, b, scale = bank._a.data_ptr(), bank._b.data_ptr(), bank._scale.data_ptr()
         n, rank = bank.max_adapters, bank.rank_pad
-        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank, n), dtype=torch.uint8,
-                           device=x.device)
-        ws_ptr = work.data_ptr()
-    with on_device(x.device):
+        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank, n), dtype=torch.uint8, device=dev)
+        work_ptr = work.data_ptr()
+    with on_device(dev):
         L.check(L.bpd_lora_project(
-            x.data_ptr(), xs, weight.data_ptr(), ws, _DTYPE_CODE[x.dtype], T, K, N, a, b, scale,
-            n, rank, None if ids is None else ids.data_ptr(), ids64, out.data_ptr(),
-            _DTYPE_CODE[out.dtype], out.stride(0) if T > 1 else max(N, 1), ws_ptr, _stream(x)))
+            x.data_ptr(), xs, weight.data_ptr(), ws, _DTYPE_CODE[dtype], T, K, N, a, b, scale,
+            n, rank, ids_ptr, ids64, out.data_ptr(), _DTYPE_CODE[out.dtype],
+            out.stride(0) if T > 1 else max(N, 1), work_ptr, _stream(x)))
     return out
 
 

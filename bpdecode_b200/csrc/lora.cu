@@ -335,11 +335,11 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
   // each part is a contiguous share of the inner elements, a multiple of 32
   const int32_t share = ((g.K + 31) / 32 + kParts * split - 1) / (kParts * split) * 32;
   const int32_t k0 = min(g.K, part * share), k1 = min(g.K, k0 + share);
-  int32_t unit = 0;
+  // units are counted through the items; this CTA takes every turns-th
+  int32_t before = 0, next = turn;
   for (int32_t i = 0; i < total; ++i) {
-    const int32_t units = (members[i] + kRows - 1) / kRows;
-    const int32_t u0 = (turn - unit % turns + turns) % turns;  // the first one of this turn
-    unit += units;
+    const int32_t units = (members[i] + kRows - 1) / kRows, u0 = next - before;
+    before += units;
     if (u0 >= units) continue;  // alike in all threads of the cluster
     const int32_t a = static_cast<int32_t>(items[i].x);
     const int32_t n = items[i].y & 31u, b0 = (items[i].y >> 5) & 15u;
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
         }
       }
     }
-    for (int32_t u = u0; u < units; u += turns) {
+    for (int32_t u = u0; u < units; u += turns, next += turns) {
       const int32_t m0 = u * kRows, have = min(kRows, members[i] - m0);
       const int32_t r0 = group * 16 + (lane >> 2), r1 = r0 + 8;  // this lane's two rows
       const bool in0 = r0 < have, in1 = r1 < have;
@@ -937,6 +937,19 @@ cudaError_t launch_shrink_rank(const LoraArgs& g, int32_t turns, int32_t split, 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
+  // The largest share of an SM's memory as shared memory, as the product needs
+  // it: an SM that is set up otherwise takes none of its CTAs until this
+  // kernel's are gone (64 rows, 4096 x 4096: 22 us instead of 17).
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev].load(std::memory_order_relaxed))) {
+    e = cudaFuncSetAttribute(shrink_kernel<T, GROUPS, RS>,
+                             cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return e;
   return cudaLaunchKernelEx(&cfg, shrink_kernel<T, GROUPS, RS>, g, turns, split);
 }
 
@@ -950,15 +963,16 @@ cudaError_t launch_shrink_groups(const LoraArgs& g, int32_t turns, int32_t split
 template <typename T>
 cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
   // A tile's items go round its CTAs in turn: as many CTAs as it can have
-  // items where there is one tile, a few for each tile of a prompt. What is
-  // left of the SMs splits the inner elements.
+  // items where there is one tile, up to nine for each tile of a prompt, 32
+  // rows at a time. What is left of the SMs splits the inner elements.
   const bool prompt = g.row_tiles > 1;
-  const int32_t turns = prompt ? 4 : std::min(g.T, g.adapters);
+  const int32_t turns = prompt ? std::max(1, std::min(9, sm_count() / g.row_tiles))
+                               : std::min(g.T, g.adapters);
   int32_t split = 1;
   while (split < kMaxSplit && static_cast<int64_t>(g.row_tiles) * turns * split * 2 <= sm_count() &&
          split * 512 <= g.K)
     split *= 2;
-  return prompt ? launch_shrink_groups<T, 4>(g, turns, split, st)
+  return prompt ? launch_shrink_groups<T, 2>(g, turns, split, st)
                 : launch_shrink_groups<T, 1>(g, turns, split, st);
 }
 

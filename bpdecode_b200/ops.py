@@ -62,12 +62,13 @@ def on_device(device: torch.device):
     """A context in which ``device`` is torch's current CUDA device, which is
     the one that a launch through the C ABI goes to (nothing to do, and nothing
     paid, where it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _CURRENT():
         return _HERE
     return torch.cuda.device(device)
 
 
 _HERE = contextlib.nullcontext()
+_CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _require_cuda(t: torch.Tensor, what: str) -> None:
