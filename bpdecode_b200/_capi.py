@@ -89,7 +89,7 @@ _SIGNATURES: dict[str, tuple[object, list]] = {
     "bpd_pda_step_greedy_from_n": (_I32, [C.POINTER(PdaGrammar), _P, _I32, _I64, _P, _P, _I64,
                                           _P, _P, _P, _I32, _P, _P, _I32, _P, _F, _P, _P, _I32,
                                           _P]),
-    "bpd_lora_workspace_bytes": (_S, [_I32, _I32, _I32]),
+    "bpd_lora_workspace_bytes": (_S, [_I32, _I32, _I32, _I32]),
     "bpd_lora_take_error": (_I32, [C.POINTER(_I32)]),
     "bpd_lora_project": (_I32, [_P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _I32,
                                 _I32, _P, _I32, _P, _I32, _I64, _P, _P]),

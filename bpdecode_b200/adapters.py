@@ -171,7 +171,8 @@ def project(
         ids_ptr = adapter_ids.data_ptr()
         a, b, scale = bank._a.data_ptr(), bank._b.data_ptr(), bank._scale.data_ptr()
         n, rank = bank.max_adapters, bank.rank_pad
-        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank, n), dtype=torch.uint8, device=dev)
+        work = torch.empty(L.bpd_lora_workspace_bytes(T, rank, n, _DTYPE_CODE[out.dtype]),
+                           dtype=torch.uint8, device=dev)
         work_ptr = work.data_ptr()
     with on_device(dev):
         L.check(L.bpd_lora_project(

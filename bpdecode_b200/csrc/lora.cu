@@ -21,9 +21,15 @@
 // items are wide rather than exact: with 16-row items alone, 256 rows with 24
 // adapters took 226 us at 65,536 outputs, against 134 us without adapters.
 //
-// S is held as the sum of two 16-bit values (its rounding, and what that left
-// off): together 2^-17 of it in bf16, 2^-22 in fp16, so an fp32 result keeps
-// what fp32 sums have. One 16-bit value would cost 2^-9 of the adapter's part.
+// S is held as the sum of 16-bit values, each the rounding of what those before
+// it left off: two of them keep 2^-17 of it in bf16 and 2^-22 in fp16 (one would
+// cost 2^-9 of the adapter's part), and an fp32 result has a third in bf16.
+//
+// The matrix unit cuts its sums off to fp32 at every step, always towards zero:
+// 4.4e-6 of the result at 4096 inner elements, and growing with them. A 16-bit
+// result does not see that. An fp32 result is therefore accumulated 512 inner
+// elements at a time, and these sums are added up in registers (5e-7, as fp32
+// arithmetic has it).
 #include <cuda.h>
 
 #include <algorithm>
@@ -41,6 +47,7 @@ constexpr int kStepK = 64;         // inner elements of a step: one 128-byte swi
 constexpr int kBlock = 16;         // rows of x of a block
 constexpr int kRankStep = 32;      // inner elements of an adapter's step, at most
 constexpr int kMaxItems = 8;       // items of an adapters' step, at most
+constexpr int kGroup = 8;           // steps that an fp32 result is accumulated over at once
 constexpr int kReach = 4;          // blocks that an item spans for each row that it has, at most
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share one tile's inner elements
 constexpr int kThreads = 192;      // loads, products, four warps that write
@@ -65,10 +72,11 @@ struct LoraArgs {
   // workspace: the items of each tile of rows
   int32_t* count;       // [row tiles]
   uint2* items;         // [row tiles, tile]: adapter; first block of S << 9 | first block << 5 | blocks
-  uint8_t* low;         // [row tiles, most_blocks, rank * 64 bytes]: S of the items' blocks
+  uint8_t* low;         // [row tiles, most_blocks, rank * parts * 32 bytes]: S of the items' blocks
   int32_t tile;         // rows of a tile
   int32_t most_blocks;  // of S, of a tile's items
   int32_t row_tiles, out_tiles;
+  int32_t parts;        // 16-bit values that make up one of S
 };
 
 __device__ __forceinline__ int32_t adapter_of(const LoraArgs& g, int32_t t) {
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     const int32_t a = static_cast<int32_t>(items[i].x);
     const int32_t n = items[i].y & 31u, b0 = (items[i].y >> 5) & 15u;
     uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (items[i].y >> 9)) *
-                               (g.rank * 64);
+                               (g.rank * g.parts * 32);
     const float scale = g.scale[a];
     // the item's rows, in order
     const bool mine = own == a && tid >= b0 * kBlock && tid < (b0 + n) * kBlock;
@@ -355,10 +363,10 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     for (int32_t w = 0; w < warp; ++w) at += warp_rows[w];
     if (mine) list[at] = static_cast<uint8_t>(tid);
     __syncthreads();
-    // An operand's place: [rank step][rounded values, rests][rank / 8][rows][8].
-    auto place = [&](int32_t row, int32_t col, int32_t half) {
+    // An operand's place: [rank step][part][rank / 8][rows][8].
+    auto place = [&](int32_t row, int32_t col, int32_t which) {
       const int32_t c = col / kRankStep * kRankStep, wide = min(kRankStep, g.rank - c);
-      return low + (c * 2 + half * wide) * n * (kBlock * 2) +
+      return low + (c * g.parts + which * wide) * n * (kBlock * 2) +
              ((col - c) >> 3) * n * (kBlock * 16) + row * 16;
     };
     if (u0 == 0) {  // the rows between
@@ -366,8 +374,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
            v += kShrinkThreads * split) {
         const int32_t row = v % (n * kBlock), col = v / (n * kBlock) * 8;
         if (ids[b0 * kBlock + row] != a) {
-          *reinterpret_cast<uint4*>(place(row, col, 0)) = uint4{};
-          *reinterpret_cast<uint4*>(place(row, col, 1)) = uint4{};
+          for (int32_t which = 0; which < g.parts; ++which)
+            *reinterpret_cast<uint4*>(place(row, col, which)) = uint4{};
         }
       }
     }
@@ -454,16 +462,19 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] = sums[0][r][col + e];
           }
-          alignas(16) Bits hi[8], rest[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            s[e] *= scale;
-            hi[e] = Dt<T>::from_float_dev(s[e]);
-            rest[e] = Dt<T>::from_float_dev(s[e] - Dt<T>::to_float(hi[e]));
-          }
+          for (int e = 0; e < 8; ++e) s[e] *= scale;
           const int32_t row = list[m0 + r] - b0 * kBlock;
-          *reinterpret_cast<uint4*>(place(row, c + col, 0)) = *reinterpret_cast<uint4*>(hi);
-          *reinterpret_cast<uint4*>(place(row, c + col, 1)) = *reinterpret_cast<uint4*>(rest);
+          for (int32_t which = 0; which < g.parts; ++which) {
+            alignas(16) Bits part_of[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              part_of[e] = Dt<T>::from_float_dev(s[e]);
+              s[e] -= Dt<T>::to_float(part_of[e]);
+            }
+            *reinterpret_cast<uint4*>(place(row, c + col, which)) =
+                *reinterpret_cast<uint4*>(part_of);
+          }
         }
         if (split > 1)
           cluster_sync();
@@ -482,7 +493,7 @@ struct Shape {
   static constexpr int kWeightBytes = kTileN * kStepK * 2;
   // a stage holds a step's tiles of W and x, or at least one item of any size
   static constexpr int kStageBytes =
-      std::max(kWeightBytes + NT * kStepK * 2, kRankStep * (kTileN * 2 + NT * 4));
+      std::max(kWeightBytes + NT * kStepK * 2, kRankStep * (kTileN * 2 + NT * (NT > 128 ? 4 : 6)));
   // leaves room for a CTA of shrink_kernel on the same SM
   static constexpr int kStages = (200 * 1024) / kStageBytes;
   static constexpr int kColumns = std::max(32, 2 * NT);  // tensor memory: two accumulators
@@ -492,10 +503,17 @@ struct Shape {
 constexpr int kMaxStages = 11;
 constexpr uint32_t kEnd = 0;  // an empty step behind the last adapter of a tile
 
+// An item of a step as the matrix instructions take it: operands, first column,
+// instruction; how far S goes on for the next 16 inner elements.
+struct __align__(16) Op {
+  uint64_t b, low;
+  uint32_t to, idesc, next, pad;
+};
+
 struct ProjectShared {
   uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
   uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | items; kEnd
-  uint32_t item[kMaxStages][kMaxItems];  // its items, as in `plan`
+  Op op[kMaxStages][kMaxItems];  // its items
   uint32_t tmem;
   uint32_t failed;
   // the items of the tile of rows, and the steps that they go in
@@ -516,6 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ ProjectShared sh;
   const uint32_t ring = (shared_addr(dynamic) + 1023u) & ~1023u;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr bool kGroups = std::is_same_v<O, float>;
   const int32_t part = split > 1 ? static_cast<int32_t>(blockIdx.x % split) : 0;
   const int32_t tiles = g.row_tiles * g.out_tiles;
   const int32_t first = split > 1 ? blockIdx.x / split : blockIdx.x;
@@ -587,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // A step takes as many items as fit: the ring is as long as the queue
         // of loads in front of HBM, so a step costs its share of that queue
         // however little it carries (one adapter a step: 0.7 us each). The
-        // plan is made once for a tile of rows; places are in units of 64
+        // plan is made once for a tile of rows; places are in units of 32
         // bytes for each inner element of a step.
         listed = rows;
         const int32_t items = min(g.count[rows], NT);
@@ -600,15 +619,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           sh.plan[i - p0] = item.y & 511u;
         }
         __syncwarp();
-        const int32_t room = S::kStageBytes / (64 * min(kRankStep, g.rank));
+        const int32_t room = S::kStageBytes / (32 * min(kRankStep, g.rank));
         int32_t n = 0, used = 0, b_at = 0;
         uint32_t last = ~0u;
         nsteps = 0;
         if (lane == 0) {
           for (int32_t i = 0; i < p1 - p0; ++i) {
             const uint32_t a = sh.adapter[i], item = sh.plan[i];
-            const int32_t wide = item & 31u;
-            if (i == 0 || n == kMaxItems || used + (a == last ? 0 : kTileN / 32) + wide > room) {
+            const int32_t wide = (item & 31u) * g.parts;
+            if (i == 0 || n == kMaxItems || used + (a == last ? 0 : kTileN / 16) + wide > room) {
               sh.step[nsteps++] = static_cast<uint16_t>(i);
               n = used = 0;
               last = ~0u;
@@ -616,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool load = a != last;
             if (load) {
               b_at = used;
-              used += kTileN / 32;
+              used += kTileN / 16;
             }
             sh.plan[i] = item | static_cast<uint32_t>(load) << 31 |
                          static_cast<uint32_t>(b_at) << 20 | static_cast<uint32_t>(used) << 9;
@@ -635,30 +654,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int32_t s = 0; s < nsteps; ++s) {
           const int32_t i0 = sh.step[s], n = sh.step[s + 1] - i0;
           const uint32_t at = ring + stage * S::kStageBytes;
-          const uint32_t item = lane < n ? sh.plan[i0 + lane] : 0, wide = item & 31u;
+          const uint32_t item = lane < n ? sh.plan[i0 + lane] : 0, wide = (item & 31u) * g.parts;
           const bool load = item >> 31;
-          int32_t units = lane < n ? wide + (load ? kTileN / 32 : 0) : 0;
+          int32_t units = lane < n ? wide + (load ? kTileN / 16 : 0) : 0;
 #pragma unroll
           for (int o = kMaxItems / 2; o > 0; o >>= 1) units += __shfl_xor_sync(kFull, units, o);
           ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
           if (!ok) break;
-          if (lane < n) sh.item[stage][lane] = item;
+          if (lane < n) {
+            const uint32_t blocks = item & 31u;
+            Op& op = sh.op[stage][lane];
+            op.b = desc_plain(at + ((item >> 20) & 2047u) * rc * 32, kTileN * 16);
+            op.low = desc_plain(at + ((item >> 9) & 2047u) * rc * 32, blocks * kBlock * 16);
+            op.to = ((item >> 5) & 15u) * kBlock;
+            op.idesc = instruction<T>(0) | (blocks * (kBlock >> 3)) << 17;
+            op.next = blocks * kBlock * 2;
+          }
           if (lane == 0) sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
           __syncwarp();
           const uint32_t bar = shared_addr(&sh.full[stage]);
-          if (lane == 0) bar_expect(bar, units * rc * 64);
+          if (lane == 0) bar_expect(bar, units * rc * 32);
           __syncwarp();
           if (lane < n) {
             if (load)
-              load_bulk(at + ((item >> 20) & 2047u) * rc * 64,
+              load_bulk(at + ((item >> 20) & 2047u) * rc * 32,
                         static_cast<const uint8_t*>(g.b) +
                             ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles + outs) *
                                  g.rank + c) * (kTileN * 2),
                         rc * kTileN * 2, bar);
-            load_bulk(at + ((item >> 9) & 2047u) * rc * 64,
+            load_bulk(at + ((item >> 9) & 2047u) * rc * 32,
                       g.low + (static_cast<int64_t>(rows) * g.most_blocks + sh.blocks[i0 + lane]) *
-                                  (g.rank * 64) + wide * c * 64,
-                      wide * rc * 64, bar);
+                                  (g.rank * g.parts * 32) + wide * c * 32,
+                      wide * rc * 32, bar);
           }
           next();
         }
@@ -690,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int32_t tile = first; tile < tiles && ok; tile += stride) {
         if (!(ok = bar_wait(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
         fence_after();
-        const uint32_t d = tmem + buffer * NT;
+        uint32_t d = tmem + buffer * NT;
         auto finish = [&] {
           mma_commit(shared_addr(&sh.empty[stage]));
           if (++stage == S::kStages) {
@@ -699,13 +726,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         };
         for (int32_t s = s0; s < s1; ++s) {
+          if (kGroups && s > s0 && (s - s0) % kGroup == 0) {  // the other accumulator
+            mma_commit(shared_addr(&sh.done[buffer]));
+            buffer ^= 1;
+            turn ^= buffer == 0;
+            if (!(ok = bar_wait(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
+            fence_after();
+            d = tmem + buffer * NT;
+          }
           if (!(ok = bar_wait(shared_addr(&sh.full[stage]), phase))) break;
           fence_after();
           const uint32_t at = ring + stage * S::kStageBytes;
           const uint64_t wd = desc_swizzled(at), xd = desc_swizzled(at + S::kWeightBytes);
 #pragma unroll
           for (int k = 0; k < kStepK / 16; ++k)
-            mma(d, wd + 2 * k, xd + 2 * k, instruction<T>(NT), s > s0 || k > 0);
+            mma(d, wd + 2 * k, xd + 2 * k, instruction<T>(NT),
+                k > 0 || (kGroups ? (s - s0) % kGroup != 0 : s > s0));
           finish();
         }
         if (!ok) break;
@@ -721,15 +757,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int32_t rc = shape >> 8, n = shape & 255;
             for (int32_t i = 0; i < n; ++i) {
-              const uint32_t item = sh.item[stage][i], wide = item & 31u;
-              const uint32_t to = d + ((item >> 5) & 15u) * kBlock;
-              const uint64_t b = desc_plain(at + ((item >> 20) & 2047u) * rc * 64, kTileN * 16);
-              const uint64_t low =
-                  desc_plain(at + ((item >> 9) & 2047u) * rc * 64, wide * kBlock * 16);
-              const uint32_t idesc = instruction<T>(0) | (wide * (kBlock >> 3)) << 17;
-              for (int32_t k = 0; k < 2 * rc; k += 16)  // the rounded values, then the rests
-                mma(to, b + (k < rc ? k : k - rc) * (kTileN * 2 / 16),
-                    low + k * (wide * kBlock * 2 / 16), idesc, true);
+              const Op op = sh.op[stage][i];
+              uint64_t low = op.low;
+              for (int32_t p = 0; p < g.parts; ++p, low += op.next) {
+                mma(d + op.to, op.b, low, op.idesc, true);
+                if (rc > 16) {
+                  low += op.next;
+                  mma(d + op.to, op.b + kTileN * 2, low, op.idesc, true);
+                }
+              }
             }
             finish();
           }
@@ -753,40 +789,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     using OBits = typename Dt<O>::Bits;
     int32_t buffer = 0;
     uint32_t turn = 0;
-    for (int32_t tile = first; tile < tiles; tile += stride) {
+    const int32_t groups = kGroups ? (s1 - s0 + kGroup - 1) / kGroup : 1;
+    for (int32_t tile = first; tile < tiles && ok; tile += stride) {
       const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles;
-      ok = bar_wait(shared_addr(&sh.done[buffer]), turn);
-      if (!__all_sync(kFull, ok)) {
-        ok = false;
-        sh.failed = 1;
-        break;
-      }
-      fence_after();
       const int32_t n = outs * kTileN + quarter * 32 + lane;
       OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
       const int32_t have = min(NT, g.T - rows * NT);
-      for (int32_t c = 0; c < NT; c += 16) {
-        uint32_t v[16];
-        tmem_load16(mine + buffer * NT + c, v);
+      // 16 rows of the tile: for the cluster's sum, [row][output] in shared memory
+      auto put = [&](int32_t c, const float (&v)[16]) {
         if (split > 1) {
-          // [row][output] in shared memory, for the cluster's sum
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(
                              ring + ((c + i) * kTileN + quarter * 32 + lane) * 4),
-                         "r"(v[i])
+                         "f"(v[i])
                          : "memory");
         } else if (n < g.N) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (c + i < have)
-              out[(c + i) * g.out_stride] = Dt<O>::from_float_dev(__uint_as_float(v[i]));
+            if (c + i < have) out[(c + i) * g.out_stride] = Dt<O>::from_float_dev(v[i]);
+        }
+      };
+      float sum[kGroups ? NT / 16 : 1][16];
+      for (int32_t group = 0; group < groups; ++group) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.done[buffer]), turn));
+        if (!ok) {
+          sh.failed = 1;
+          break;
+        }
+        fence_after();
+        if constexpr (kGroups) {
+#pragma unroll
+          for (int c = 0; c < NT; c += 16) {
+            uint32_t v[16];
+            tmem_load16(mine + buffer * NT + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              sum[c / 16][i] =
+                  group == 0 ? __uint_as_float(v[i]) : sum[c / 16][i] + __uint_as_float(v[i]);
+          }
+        } else {
+          for (int c = 0; c < NT; c += 16) {
+            uint32_t v[16];
+            tmem_load16(mine + buffer * NT + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[0][i] = __uint_as_float(v[i]);
+            put(c, sum[0]);
+          }
+        }
+        fence_before();
+        if (lane == 0) bar_arrive(shared_addr(&sh.free[buffer]));
+        buffer ^= 1;
+        turn ^= buffer == 0;
+      }
+      if constexpr (kGroups) {
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < NT; c += 16) put(c, sum[c / 16]);
         }
       }
-      fence_before();
-      if (lane == 0) bar_arrive(shared_addr(&sh.free[buffer]));
-      buffer ^= 1;
-      turn ^= buffer == 0;
     }
   }
   __syncwarp();
@@ -863,16 +924,17 @@ bool matrix_map(CUtensorMap* map, EncodeFn encode, const void* base, bool bf16, 
 }
 
 // Rows of x of a tile: all of them where that is one tile, W is then read once.
-int32_t row_tile(int32_t rows) {
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+// (An fp32 result keeps its sums in registers, which hold 128.)
+int32_t row_tile(int32_t rows, bool fp32) {
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || fp32 ? 128 : 256;
 }
 
 struct Workspace {
   int32_t most_blocks;
   size_t count, items, low, bytes;
 };
-Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters) {
-  const int32_t nt = row_tile(rows);
+Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters, bool fp32) {
+  const int32_t nt = row_tile(rows, fp32);
   const size_t tiles = (static_cast<size_t>(rows) + nt - 1) / nt;
   Workspace w;
   w.most_blocks = std::min<int64_t>(kReach * nt, static_cast<int64_t>(nt / kBlock) *
@@ -880,7 +942,7 @@ Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters) {
   w.count = 0;
   w.items = align256(tiles * sizeof(int32_t));
   w.low = w.items + align256(tiles * nt * sizeof(uint2));
-  w.bytes = w.low + align256(tiles * w.most_blocks * rank * 64);
+  w.bytes = w.low + align256(tiles * w.most_blocks * rank * 32 * (fp32 ? 3 : 2));
   return w;
 }
 
@@ -986,7 +1048,8 @@ cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, con
       case 32: e = launch_tile<T, O, 32>(wmap, xmap, g, st); break;
       case 64: e = launch_tile<T, O, 64>(wmap, xmap, g, st); break;
       case 128: e = launch_tile<T, O, 128>(wmap, xmap, g, st); break;
-      default: e = launch_tile<T, O, 256>(wmap, xmap, g, st);
+      default:
+        if constexpr (!std::is_same_v<O, float>) e = launch_tile<T, O, 256>(wmap, xmap, g, st);
     }
   }
   if (e != cudaSuccess) (void)cudaGetLastError();
@@ -998,8 +1061,10 @@ cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, con
 
 using namespace bpd;
 
-extern "C" size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t num_adapters) {
-  return workspace_of(std::max(rows, 1), std::max(rank, 0), num_adapters).bytes;
+extern "C" size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t num_adapters,
+                                           int32_t out_dtype) {
+  return workspace_of(std::max(rows, 1), std::max(rank, 0), num_adapters, out_dtype == BPD_F32)
+      .bytes;
 }
 
 extern "C" bpd_status bpd_lora_take_error(int32_t* error_out) {
@@ -1048,7 +1113,8 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
     if (num_adapters > (1 << 28))
       return fail(BPD_ERR_CAPACITY, "%s: too many adapters", what);
   }
-  const int32_t nt = row_tile(rows);
+  const bool fp32 = out_dtype == BPD_F32;
+  const int32_t nt = row_tile(rows, fp32);
   const int32_t row_tiles = (rows - 1) / nt + 1, out_tiles = (out_features - 1) / kTileN + 1;
   if (static_cast<int64_t>(row_tiles) * out_tiles > INT_MAX / 2)
     return fail(BPD_ERR_CAPACITY, "%s: too many tiles", what);
@@ -1059,13 +1125,13 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   if (!matrix_map(&wmap, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
       !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, nt))
     return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
-  const Workspace w = workspace_of(rows, rank, num_adapters);
+  const Workspace w = workspace_of(rows, rank, num_adapters, fp32);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
                    reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, w.most_blocks, row_tiles,
-                   out_tiles};
+                   out_tiles, fp32 && bf16 ? 3 : 2};
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (bf16)

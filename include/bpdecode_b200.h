@@ -377,7 +377,8 @@ bpd_status bpd_pda_step_greedy_from_n(
  * bpd_lora_take_error waits for the device and tells whether a projection on
  * the current device gave up waiting for its own loads since the last call
  * (its result is then not complete); 0 unless the device misbehaves. */
-size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t num_adapters);
+size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t num_adapters,
+                                int32_t out_dtype);
 bpd_status bpd_lora_take_error(int32_t* error_out);
 bpd_status bpd_lora_project(
     const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
