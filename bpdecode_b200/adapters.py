@@ -15,6 +15,8 @@ backward pass: adapters are served here, not trained.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _capi
@@ -182,4 +184,16 @@ def project(
     return out
 
 
-__all__ = ["MAX_RANK", "AdapterBank", "project"]
+def check_device() -> None:
+    """Wait for the current device and raise if a projection on it gave up
+    waiting for its own loads since the last call (its result is then not
+    complete). The kernels end with that mark, instead of hanging, should the
+    device ever misbehave; a step need not ask."""
+    error = ctypes.c_int32(0)
+    L = _capi.lib()
+    L.check(L.bpd_lora_take_error(ctypes.byref(error)))
+    if error.value:
+        raise RuntimeError("bpdecode_b200: a projection gave up waiting for its loads")
+
+
+__all__ = ["MAX_RANK", "AdapterBank", "check_device", "project"]

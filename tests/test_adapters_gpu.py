@@ -190,3 +190,16 @@ def test_refusals() -> None:
     for size in ((60, 96, 2, 16), (64, 0, 2, 16), (64, 96, 0, 16), (64, 96, 2, 0), (64, 96, 2, 129)):
         with pytest.raises(ValueError):
             AdapterBank(*size)
+
+
+def test_no_projection_gave_up_waiting() -> None:
+    from bpdecode_b200.adapters import AdapterBank, check_device, project
+
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(33, 256, generator=g).bfloat16().cuda()
+    w = torch.randn(300, 256, generator=g).bfloat16().cuda()
+    bank = AdapterBank(256, 300, 2, 16)
+    bank.load(1, torch.randn(16, 256, generator=g), torch.randn(300, 16, generator=g))
+    project(x, w, bank, torch.arange(33, device="cuda") % 3)
+    check_device()
+    check_device()
