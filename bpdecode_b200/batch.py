@@ -12,6 +12,8 @@ changes is underneath:
   until the batch membership changes (the reference rebuilds and uploads it
   from a Python list on every call, batch.py:171-174);
 * :meth:`ConstraintBatch.step_greedy` fuses mask + argmax + commit;
+  :meth:`ConstraintBatch.verify_drafts` and :meth:`ConstraintBatch.step_sample`
+  do the same for drafted and sampled tokens;
 * a batch may mix grammars (NEW): pass a list of :class:`FsaTensors` and
   ``add(seq_id, grammar=i)``; their states are concatenated into one global
   state space so a mixed batch is still one launch per step (the reference is
@@ -37,6 +39,8 @@ from .ops import (
     _tokens,
     apply_mask_,
 )
+from .speculative import VerifyResult
+from .speculative import _launch as _verify
 
 FREE = -2  # slot holds no sequence
 BROKEN = -1  # a committed token left the grammar-valid path
@@ -540,6 +544,52 @@ class ConstraintBatch:
             tokens.data_ptr(), None, int(chunks_per_row), self._scratch.data_ptr(),
             _stream(src)))
         return tokens
+
+    def verify_drafts(
+        self,
+        seq_ids: Sequence[Hashable],
+        src: torch.Tensor,
+        drafts: torch.Tensor | None = None,
+        uniforms: torch.Tensor | None = None,
+        noise: torch.Tensor | None = None,
+        *,
+        draft_lens: torch.Tensor | None = None,
+        draft_probs: torch.Tensor | None = None,
+        temperature: float | torch.Tensor = 1.0,
+        src_rows: torch.Tensor | None = None,
+        prob_rows: torch.Tensor | None = None,
+    ) -> VerifyResult:
+        """NEW: :func:`~bpdecode_b200.speculative.verify_drafts` of drafted
+        tokens for ``seq_ids`` under their grammars, and the commit of what was
+        accepted: each sequence moves to the state behind its last token (BROKEN
+        where nothing was allowed)."""
+        slots, slot_ptr = self._slots_arg(seq_ids)
+        B = int(slots.numel())
+        if drafts is not None and int(drafts.shape[0]) != B:
+            raise RuntimeError("bpdecode_b200: one row of drafts per seq_id")
+        t = self._t
+        nxt = torch.empty(B, dtype=torch.int32, device=self.device)
+        if src.device != self.device:
+            raise RuntimeError(f"bpdecode_b200: src must be on {self.device}")
+        return _verify(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature,
+                       src_rows, prob_rows, B, t.vocab_size, self._state, slot_ptr, None,
+                       t.allow_bits, t.tok_next, t.num_states, nxt, True)
+
+    def step_sample(
+        self,
+        seq_ids: Sequence[Hashable],
+        src: torch.Tensor,
+        noise: torch.Tensor,
+        temperature: float | torch.Tensor = 1.0,
+        src_rows: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """NEW: one token sampled for each sequence from ``softmax(row /
+        temperature)`` over the tokens that its grammar allows, and committed:
+        :meth:`verify_drafts` without drafts. ``noise`` float32 [batch, >= vocab]
+        is exponential; ``src`` is not modified. Returns the tokens (int64, -1
+        where nothing is allowed)."""
+        return self.verify_drafts(seq_ids, src, noise=noise, temperature=temperature,
+                                  src_rows=src_rows).tokens[:, 0]
 
     # --- queries ------------------------------------------------------
     def state_of(self, seq_id: Hashable) -> int:

@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
     }
     if (lane == 0) {
       a.counts_out[b] = 0;
-      if (a.next_out) a.next_out[b] = a.state_pool[slot];
+      if (a.next_out) a.next_out[b] = a.tok_next ? a.state_pool[slot] : -2;
     }
     return;
   }
@@ -1039,6 +1039,8 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
       const int32_t next = token < 0 ? -1 : step(a, p.state, token);
       if (a.next_out) a.next_out[b] = next;
       if (a.write_back) a.state_pool[a.slots ? a.slots[b] : b] = next;
+    } else if (a.next_out) {
+      a.next_out[b] = token < 0 ? -1 : p.state;
     }
   }
 }
@@ -1121,8 +1123,12 @@ extern "C" bpd_status bpd_verify_drafts(const bpd_verify_args* args, void* strea
               "%s: words_stride too small, or no states", what);
   BPD_REQUIRE(!a.allow_bits || a.path || (a.state_pool && a.tok_next),
               "%s: a grammar needs state_pool and tok_next, or path", what);
-  BPD_REQUIRE((!a.next_out && !a.write_back) || (a.state_pool && a.tok_next && a.allow_bits),
-              "%s: next states need state_pool, allow_bits and tok_next", what);
+  const bool walks = a.state_pool && a.tok_next && a.allow_bits;
+  BPD_REQUIRE(!a.write_back || walks, "%s: write_back needs state_pool, allow_bits and tok_next",
+              what);
+  BPD_REQUIRE(!a.next_out || walks || (a.path && a.allow_bits && !a.tok_next),
+              "%s: next_out needs state_pool, allow_bits and tok_next, or path without tok_next",
+              what);
   if (!a.allow_bits) a.tok_next = nullptr;
   cudaStream_t st = as_stream(stream);
   return with_dtype(a.src_dtype, what, [&](auto tag) {

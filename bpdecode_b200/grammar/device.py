@@ -30,6 +30,8 @@ import torch
 
 from .. import _capi
 from ..ops import _check_logits, _require_cuda, _stream, _tokens, _upload
+from ..speculative import VerifyResult
+from ..speculative import _launch as _verify
 from ..tokenizer import as_vocabulary
 
 # Must match the C ABI (BPD_PDA_MAX_CONFIGS / BPD_PDA_MAX_DEPTH / ..._INTS) and
@@ -520,6 +522,76 @@ class CFGConstraintBatch:
             _stream(src)))
         self.last_status = status
         return tokens
+
+    def verify_drafts(
+        self,
+        seq_ids: Sequence[Hashable],
+        src: torch.Tensor,
+        drafts: torch.Tensor | None = None,
+        uniforms: torch.Tensor | None = None,
+        noise: torch.Tensor | None = None,
+        *,
+        draft_lens: torch.Tensor | None = None,
+        draft_probs: torch.Tensor | None = None,
+        temperature: float | torch.Tensor = 1.0,
+        src_rows: torch.Tensor | None = None,
+        prob_rows: torch.Tensor | None = None,
+    ) -> VerifyResult:
+        """NEW: :func:`~bpdecode_b200.speculative.verify_drafts` of drafted
+        tokens for ``seq_ids`` under the grammar, and the commit of what was
+        accepted. Copies of the config-sets walk along the drafts, a mask and an
+        advance for each position. ``states`` of the result is the status of
+        :meth:`commit`: 1, or -1 for a sequence that is broken, now (nothing was
+        allowed) or earlier."""
+        slots = self._slots(seq_ids)
+        B, V = int(slots.numel()), self.g.vocab_size
+        K = 0 if drafts is None else int(drafts.shape[1])
+        if drafts is not None and int(drafts.shape[0]) != B:
+            raise RuntimeError("bpdecode_b200: one row of drafts per seq_id")
+        if src.device != self.device:
+            raise RuntimeError(f"bpdecode_b200: src must be on {self.device}")
+        config, broken = self._configs[slots], self._broken[slots]
+        # config-sets and allow bits of every position; a broken sequence allows nothing
+        configs = torch.empty((K + 1, B, PDA_CONFIG_FLAT), dtype=torch.int32, device=self.device)
+        bits = torch.empty((K + 1, B, (V + 31) // 32), dtype=torch.int32, device=self.device)
+        for i in range(K + 1):
+            configs[i] = config
+            bits[i] = pda_compute_mask(self.g, config)
+            if i < K:
+                # behind a sequence's drafts: no token, which leaves the config-set as it is
+                d = drafts[:, i].to(torch.int64)
+                if draft_lens is not None:
+                    d = torch.where(draft_lens > i, d, -1)
+                pda_advance_state(config, self.g, d)
+        path = torch.arange((K + 1) * B, dtype=torch.int32, device=self.device).view(K + 1, B)
+        path = torch.where(broken, -1, path).t().contiguous()
+        last = torch.empty(B, dtype=torch.int32, device=self.device)
+        got = _verify(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, src_rows,
+                      prob_rows, B, V, None, None, path, bits.view((K + 1) * B, -1), None,
+                      (K + 1) * B, last, False)
+        # the config-set at each sequence's last token, and that token
+        idle, ended = last == -2, last == -1
+        config = configs.view(-1, PDA_CONFIG_FLAT)[last.clamp(min=0).long()]
+        token = got.tokens.gather(1, (got.counts - 1).clamp(min=0).long()[:, None])[:, 0]
+        pda_advance_state(config, self.g, torch.where(last >= 0, token, -1))
+        broken = broken | ended
+        self._configs[slots] = torch.where((idle | broken)[:, None], self._configs[slots], config)
+        self._broken[slots] = broken
+        return got._replace(states=torch.where(broken, _BROKEN, 1).to(torch.int32))
+
+    def step_sample(
+        self,
+        seq_ids: Sequence[Hashable],
+        src: torch.Tensor,
+        noise: torch.Tensor,
+        temperature: float | torch.Tensor = 1.0,
+        src_rows: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """NEW: one token sampled for each sequence, under the grammar, and
+        committed (as :meth:`ConstraintBatch.step_sample
+        <bpdecode_b200.batch.ConstraintBatch.step_sample>`)."""
+        return self.verify_drafts(seq_ids, src, noise=noise, temperature=temperature,
+                                  src_rows=src_rows).tokens[:, 0]
 
     # --- queries ------------------------------------------------------
     def is_complete(self, seq_id: Hashable) -> bool:

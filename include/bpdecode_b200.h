@@ -465,8 +465,11 @@ typedef struct bpd_verify_args {
  * greedy requests), then 0. At a position where nothing is allowed (no token,
  * or none above -inf) the request ends without a token. next_out and, if
  * write_back, state_pool[slots[b]]: the state behind the last token, -1 where
- * the request ended without one. Tokens behind an accepted end-of-sequence
- * token are the caller's to drop.
+ * the request ended without one. With path and no tok_next, next_out is the
+ * entry of path at the position of the last token (-1 where the request ended
+ * without one, -2 where it is idle), for callers that keep other states than
+ * tok_next's. Tokens behind an accepted end-of-sequence token are the caller's
+ * to drop.
  *
  * A request with len < 0 or > max_drafts, or rows outside src or probs, is
  * idle: no tokens, count 0, its state as it was. max_drafts <= BPD_MAX_DRAFTS.
