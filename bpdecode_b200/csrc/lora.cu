@@ -1024,12 +1024,12 @@ cudaError_t launch_shrink_groups(const LoraArgs& g, int32_t turns, int32_t split
 
 template <typename T>
 cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
-  // A tile's items go round its CTAs in turn: as many CTAs as it can have
-  // items where there is one tile, up to nine for each tile of a prompt, 32
+  // A tile's items go round its CTAs in turn, 16 rows at a time: as many CTAs as
+  // that can come to where there is one tile, up to nine for each tile of a prompt, 32
   // rows at a time. What is left of the SMs splits the inner elements.
   const bool prompt = g.row_tiles > 1;
   const int32_t turns = prompt ? std::max(1, std::min(9, sm_count() / g.row_tiles))
-                               : std::min(g.T, g.adapters);
+                               : std::min(g.T, g.adapters + g.T / 16);
   int32_t split = 1;
   while (split < kMaxSplit && static_cast<int64_t>(g.row_tiles) * turns * split * 2 <= sm_count() &&
          split * 512 <= g.K)
