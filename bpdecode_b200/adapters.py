@@ -148,7 +148,7 @@ def project(
     if (bank is None) != (adapter_ids is None):
         raise RuntimeError("bpdecode_b200: bank and adapter_ids come together")
     if out is None:
-        out = torch.empty((T, N), dtype=out_dtype or dtype, device=dev)
+        out = torch.empty(T, N, dtype=out_dtype or dtype, device=dev)
     elif (out.shape != (T, N) or out.device != dev
           or (out_dtype is not None and out.dtype != out_dtype) or (N > 1 and out.stride(1) != 1)
           or (T > 1 and out.stride(0) < N)):

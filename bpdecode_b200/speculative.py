@@ -54,15 +54,16 @@ def _bad(what: str, why: str, t: torch.Tensor) -> RuntimeError:
 def _matrix(t: torch.Tensor, what: str, rows: int, cols: int, dtypes: tuple,
             device: torch.device) -> tuple[int, int]:
     """(pointer, row stride) of a matrix of at least [rows, cols]."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] < rows or shape[1] < cols:
+    if t.dim() != 2:
+        raise _bad(what, f"must be [{rows}, {cols}] or larger", t)
+    (have, width), (stride, step) = t.shape, t.stride()
+    if have < rows or width < cols:
         raise _bad(what, f"must be [{rows}, {cols}] or larger", t)
     if t.dtype not in dtypes or t.device != device:
         raise _bad(what, f"must be one of {dtypes} on {device}", t)
-    stride, step = t.stride()
-    if shape[0] <= 1:
-        stride = max(shape[1], 1)
-    if cols and (step != 1 and shape[1] > 1 or stride < cols):
+    if have <= 1:
+        stride = max(width, 1)
+    if cols and (step != 1 and width > 1 or stride < cols):
         raise _bad(what, "needs contiguous columns and rows that do not overlap", t)
     return t.data_ptr(), stride
 
@@ -78,7 +79,6 @@ def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, 
             prob_rows, batch, vocab, pool, slot_ptr, path, bits, tok_next, num_states,
             states, write_back) -> VerifyResult:
     """Check the arguments that every form shares and enqueue the kernels."""
-    _require_cuda(src, "src")
     dev, B, V = src.device, batch, vocab
     src_ptr, src_stride = _matrix(src, "src", 0, V, _FLOATS, dev)
     K = draft_ptr = draft_stride = drafts64 = 0
@@ -125,9 +125,10 @@ def _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, 
             raise RuntimeError("bpdecode_b200: draft_probs has fewer rows than the drafts")
     elif prob_rows is not None:
         raise RuntimeError("bpdecode_b200: prob_rows without draft_probs")
-    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=dev)
+    # sizes one by one: a tuple of them costs a microsecond more
+    tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
     counts = torch.empty(B, dtype=torch.int32, device=dev)
-    logprobs = torch.empty((B, K + 1), dtype=torch.float32, device=dev)
+    logprobs = torch.empty(B, K + 1, dtype=torch.float32, device=dev)
     L = _capi.lib()
     work = torch.empty(L.bpd_verify_workspace_bytes(B, K), dtype=torch.uint8, device=dev)
     args = _ARGS.pack(
@@ -186,23 +187,26 @@ def verify_drafts(
     if src.dim() != 2:
         raise RuntimeError("bpdecode_b200: src must be [rows, vocab]")
     if states is not None:
-        B = int(states.numel())
+        B = states.numel()
     elif drafts is not None:
-        B = int(drafts.shape[0])
+        B = drafts.shape[0]
     elif src_rows is not None:
-        B = int(src_rows.shape[0])
+        B = src_rows.shape[0]
     else:
-        B = int(src.shape[0])
-    if drafts is not None and int(drafts.shape[0]) != B:
+        B = src.shape[0]
+    if drafts is not None and drafts.shape[0] != B:
         raise RuntimeError(f"bpdecode_b200: one row of drafts per request ({drafts.shape[0]} != {B})")
     if fsa is None:
         return _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature,
-                       src_rows, prob_rows, B, int(src.shape[1]), None, None, None, None, None,
+                       src_rows, prob_rows, B, src.shape[1], None, None, None, None, None,
                        0, None, False)
     tok_next, bits = fsa.dense_tables()
     if fsa.device != src.device:
         raise RuntimeError("bpdecode_b200: src and tables live on different devices")
-    st = _as_i32(states, B, fsa.device)
+    st = states
+    if (st.dtype is not torch.int32 or st.dim() != 1 or not st.is_contiguous()
+            or st.device != src.device):
+        st = _as_i32(states, B, fsa.device)
     nxt = torch.empty(B, dtype=torch.int32, device=src.device)
     return _launch(src, drafts, uniforms, noise, draft_lens, draft_probs, temperature, src_rows,
                    prob_rows, B, fsa.vocab_size, st, None, None, bits, tok_next, fsa.num_states,
