@@ -21,6 +21,13 @@
 // items are wide rather than exact: with 16-row items alone, 256 rows with 24
 // adapters took 226 us at 65,536 outputs, against 134 us without adapters.
 //
+// Tiles of 256 rows are bound by what an SM loads, 48 KB for every 64 inner
+// elements. Two CTAs then work as a pair (cta_group::2): an instruction of the
+// first multiplies 256 outputs by 256 rows, each CTA has its own 128 outputs of
+// W and half of the rows of x, and both accumulate their outputs for all rows.
+// The first CTA's barriers count the loads of both; copies that only a CTA's own
+// barrier can count (the adapters') are told on by a thread of the second.
+//
 // S is held as the sum of 16-bit values, each the rounding of what those before
 // it left off: two of them keep 2^-17 of it in bf16 and 2^-22 in fp16 (one would
 // cost 2^-9 of the adapter's part), and an fp32 result has a third in bf16.
@@ -77,6 +84,7 @@ struct LoraArgs {
   int32_t most_blocks;  // of S, of a tile's items
   int32_t row_tiles, out_tiles;
   int32_t parts;        // 16-bit values that make up one of S
+  int32_t pair;         // CTAs that share the product's instructions: 1 or 2
 };
 
 __device__ __forceinline__ int32_t adapter_of(const LoraArgs& g, int32_t t) {
@@ -118,13 +126,63 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// As bar_try, for what the cluster's other CTAs arrived for.
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // False where the wait gave up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  if (bar_try(bar, parity)) return true;
+template <typename There>
+__device__ __forceinline__ bool wait_for(There&& there) {
+  if (there()) return true;
   const uint64_t start = now_ns();
-  while (!bar_try(bar, parity))
+  while (!there())
     if (now_ns() - start > kGiveUpNs) return false;
   return true;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  return wait_for([&] { return bar_try(bar, parity); });
+}
+template <int PAIR>
+__device__ __forceinline__ bool bar_wait_free(uint32_t bar, uint32_t parity) {
+  return wait_for(
+      [&] { return PAIR == 2 ? bar_try_cluster(bar, parity) : bar_try(bar, parity); });
+}
+// Says to the first CTA that copies have landed here. Nothing but the copies is
+// passed on, and a barrier has said that they are in place, so this needs no
+// ordering of its own (as a release it took a microsecond for each step).
+__device__ __forceinline__ void bar_tell(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool bar_told(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The barrier at the same place in the cluster's CTA `rank`.
+__device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar), "r"(rank)
+      : "memory");
 }
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y,
                                          uint32_t bar) {
@@ -133,6 +191,20 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// A CTA's part of a pair's operands, counted by the first CTA's barrier.
+__device__ __forceinline__ void load_box_for(uint32_t dst, const CUtensorMap* map, int32_t x,
+                                             int32_t y, uint32_t first_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+      "r"(first_bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
 __device__ __forceinline__ void load_bulk(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
   asm volatile(
@@ -140,17 +212,45 @@ __device__ __forceinline__ void load_bulk(uint32_t dst, const void* src, uint32_
           "r"(dst), "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+// One instruction of this CTA (PAIR 1) or of both CTAs of a pair, each with its
+// own operands at these places: 128 outputs each, half of the rows of x each.
+template <int PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-      "r"(idesc), "r"(static_cast<uint32_t>(add))
-      : "memory");
+  if constexpr (PAIR == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
 }
+// Arrives where all instructions so far are through: in every CTA of the pair,
+// or in this one.
+template <int PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
+  if constexpr (PAIR == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+template <int PAIR>
+__device__ __forceinline__ void mma_commit_here(uint32_t bar) {
+  if constexpr (PAIR == 1)
+    mma_commit<1>(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -197,11 +297,11 @@ __device__ __forceinline__ uint64_t desc_plain(uint32_t addr, uint32_t lead) {
 }
 
 // Instruction descriptor: fp32 accumulator, both operands of type T and
-// K-major, M = 128.
-template <typename T>
+// K-major, M = 128 outputs for each CTA.
+template <typename T, int PAIR>
 constexpr uint32_t instruction(uint32_t n) {
   const uint32_t f = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
-  return (1u << 4) | (f << 7) | (f << 10) | ((n >> 3) << 17) | ((kTileN >> 4) << 24);
+  return (1u << 4) | (f << 7) | (f << 10) | ((n >> 3) << 17) | ((PAIR * kTileN >> 4) << 24);
 }
 
 // ---------------------------------------------------------------------------
@@ -265,9 +365,11 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     int32_t start = -1, end = 0, rows = 0;
 #pragma unroll
     for (int32_t b = 0; b < 16; ++b) {
-      const int32_t here = __popc((rows_in[b >> 1] >> ((b & 1) * 16)) & 0xFFFFu);
+      if (b % g.pair) continue;  // a pair has whole blocks of 32 rows, half of each in a CTA
+      const int32_t here = __popc(g.pair == 2 ? rows_in[b >> 1]
+                                              : (rows_in[b >> 1] >> ((b & 1) * 16)) & 0xFFFFu);
       if (here == 0) continue;
-      if (start >= 0 && b + 1 - start > kReach * (rows + here)) {
+      if (start >= 0 && b + g.pair - start > kReach * (rows + here)) {
         f(start, end - start, rows);
         start = -1;
       }
@@ -275,7 +377,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
         start = b;
         rows = 0;
       }
-      end = b + 1;
+      end = b + g.pair;
       rows += here;
     }
     if (start >= 0) f(start, end - start, rows);
@@ -363,11 +465,13 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     for (int32_t w = 0; w < warp; ++w) at += warp_rows[w];
     if (mine) list[at] = static_cast<uint8_t>(tid);
     __syncthreads();
-    // An operand's place: [rank step][part][rank / 8][rows][8].
+    // An operand's place: [CTA of the pair][rank step][part][rank / 8][rows][8].
+    const int32_t rows = n * kBlock / g.pair;
     auto place = [&](int32_t row, int32_t col, int32_t which) {
       const int32_t c = col / kRankStep * kRankStep, wide = min(kRankStep, g.rank - c);
-      return low + (c * g.parts + which * wide) * n * (kBlock * 2) +
-             ((col - c) >> 3) * n * (kBlock * 16) + row * 16;
+      const int32_t cta = row >= rows;
+      return low + (cta * g.rank * g.parts + c * g.parts + which * wide) * rows * 2 +
+             ((col - c) >> 3) * rows * 16 + (row - cta * rows) * 16;
     };
     if (u0 == 0) {  // the rows between
       for (int32_t v = tid + kpart * kShrinkThreads; v < n * kBlock * (g.rank / 8);
@@ -488,12 +592,13 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
 // ---------------------------------------------------------------------------
 // The product.
 
-template <int NT>
+template <int NT, int PAIR>
 struct Shape {
   static constexpr int kWeightBytes = kTileN * kStepK * 2;
   // a stage holds a step's tiles of W and x, or at least one item of any size
   static constexpr int kStageBytes =
-      std::max(kWeightBytes + NT * kStepK * 2, kRankStep * (kTileN * 2 + NT * (NT > 128 ? 4 : 6)));
+      std::max(kWeightBytes + NT / PAIR * kStepK * 2,
+               kRankStep * (kTileN * 2 + NT / PAIR * (NT > 128 ? 4 : 6)));
   // leaves room for a CTA of shrink_kernel on the same SM
   static constexpr int kStages = (200 * 1024) / kStageBytes;
   static constexpr int kColumns = std::max(32, 2 * NT);  // tensor memory: two accumulators
@@ -511,7 +616,7 @@ struct __align__(16) Op {
 };
 
 struct ProjectShared {
-  uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
+  uint64_t full[kMaxStages], empty[kMaxStages], peer[kMaxStages], done[2], free[2], last;
   uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | items; kEnd
   Op op[kMaxStages][kMaxItems];  // its items
   uint32_t tmem;
@@ -523,12 +628,13 @@ struct ProjectShared {
   uint16_t step[257];       // first item of each step
 };
 
-template <typename T, typename O, int NT>
+template <typename T, typename O, int NT, int PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const LoraArgs g, const int32_t split) {
-  using S = Shape<NT>;
-  static_assert(S::kStages <= kMaxStages && S::kStages * S::kStageBytes >= NT * kTileN * 4,
+  using S = Shape<NT, PAIR>;
+  static_assert(S::kStages <= kMaxStages &&
+                    (PAIR == 2 || S::kStages * S::kStageBytes >= NT * kTileN * 4),
                 "barriers for each stage, room for a tile of sums");
   extern __shared__ uint8_t dynamic[];
   __shared__ ProjectShared sh;
@@ -536,9 +642,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr bool kGroups = std::is_same_v<O, float>;
   const int32_t part = split > 1 ? static_cast<int32_t>(blockIdx.x % split) : 0;
-  const int32_t tiles = g.row_tiles * g.out_tiles;
-  const int32_t first = split > 1 ? blockIdx.x / split : blockIdx.x;
-  const int32_t stride = split > 1 ? tiles : gridDim.x;  // a cluster has one tile
+  // A pair has two tiles of outputs side by side, this CTA the cta-th; the first
+  // CTA gives the instructions of both.
+  const int32_t cta = PAIR == 2 ? static_cast<int32_t>(blockIdx.x & 1u) : 0;
+  const int32_t tiles = g.row_tiles * ((g.out_tiles + PAIR - 1) / PAIR);
+  const int32_t first = split > 1 ? blockIdx.x / split : blockIdx.x / PAIR;
+  const int32_t stride = split > 1 ? tiles : gridDim.x / PAIR;  // a cluster of parts has one tile
   const int32_t steps = (g.K + kStepK - 1) / kStepK;
   const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(steps) * part / split);
   const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(steps) * (part + 1) / split);
@@ -547,24 +656,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < S::kStages; ++i) {
       bar_init(shared_addr(&sh.full[i]), 1);
       bar_init(shared_addr(&sh.empty[i]), 1);
+      bar_init(shared_addr(&sh.peer[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(shared_addr(&sh.done[i]), 1);
-      bar_init(shared_addr(&sh.free[i]), 4);
+      bar_init(shared_addr(&sh.free[i]), 4 * PAIR);
     }
     bar_init(shared_addr(&sh.last), 1);
     sh.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     shared_addr(&sh.tmem)),
-                 "n"(S::kColumns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIR == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       shared_addr(&sh.tmem)),
+                   "n"(S::kColumns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       shared_addr(&sh.tmem)),
+                   "n"(S::kColumns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   fence_before();
   __syncthreads();
+  if (PAIR == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = sh.tmem;
   bool ok = true;
@@ -577,6 +696,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     int32_t stage = 0;
     uint32_t phase = 0;
     int32_t issued = 0;
+    // copies that this CTA's own barriers count, where the first CTA's count the
+    // others: stages that had any, and how often (its last bit)
+    uint32_t own = 0, uses = 0;
     auto next = [&] {
       ++issued;
       if (++stage == S::kStages) {
@@ -585,15 +707,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     for (int32_t tile = first; tile < tiles && ok; tile += stride) {
-      const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles;
+      const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles * PAIR + cta;
       for (int32_t s = s0; s < s1; ++s) {
         ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
         if (!ok) break;
         if (lane == 0) {
           const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
-          bar_expect(bar, S::kWeightBytes + NT * kStepK * 2);
-          load_box(at, &wmap, s * kStepK, outs * kTileN, bar);
-          load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT, bar);
+          if constexpr (PAIR == 1) {
+            bar_expect(bar, S::kWeightBytes + NT * kStepK * 2);
+            load_box(at, &wmap, s * kStepK, outs * kTileN, bar);
+            load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT, bar);
+          } else {
+            const uint32_t of_both = in_cta(bar, 0);
+            if (cta == 0) bar_expect(bar, 2 * S::kWeightBytes + NT * kStepK * 2);
+            load_box_for(at, &wmap, s * kStepK, outs * kTileN, of_both);
+            load_box_for(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT + cta * (NT / 2),
+                         of_both);
+          }
         }
         next();
       }
@@ -626,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           for (int32_t i = 0; i < p1 - p0; ++i) {
             const uint32_t a = sh.adapter[i], item = sh.plan[i];
-            const int32_t wide = (item & 31u) * g.parts;
+            const int32_t wide = (item & 31u) * g.parts / PAIR;
             if (i == 0 || n == kMaxItems || used + (a == last ? 0 : kTileN / 16) + wide > room) {
               sh.step[nsteps++] = static_cast<uint16_t>(i);
               n = used = 0;
@@ -654,7 +784,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int32_t s = 0; s < nsteps; ++s) {
           const int32_t i0 = sh.step[s], n = sh.step[s + 1] - i0;
           const uint32_t at = ring + stage * S::kStageBytes;
-          const uint32_t item = lane < n ? sh.plan[i0 + lane] : 0, wide = (item & 31u) * g.parts;
+          const uint32_t item = lane < n ? sh.plan[i0 + lane] : 0;
+          const uint32_t wide = (item & 31u) * g.parts / PAIR;
           const bool load = item >> 31;
           int32_t units = lane < n ? wide + (load ? kTileN / 16 : 0) : 0;
 #pragma unroll
@@ -665,10 +796,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t blocks = item & 31u;
             Op& op = sh.op[stage][lane];
             op.b = desc_plain(at + ((item >> 20) & 2047u) * rc * 32, kTileN * 16);
-            op.low = desc_plain(at + ((item >> 9) & 2047u) * rc * 32, blocks * kBlock * 16);
+            op.low = desc_plain(at + ((item >> 9) & 2047u) * rc * 32, blocks * kBlock * 16 / PAIR);
             op.to = ((item >> 5) & 15u) * kBlock;
-            op.idesc = instruction<T>(0) | (blocks * (kBlock >> 3)) << 17;
-            op.next = blocks * kBlock * 2;
+            op.idesc = instruction<T, PAIR>(0) | (blocks * (kBlock >> 3)) << 17;
+            op.next = blocks * kBlock * 2 / PAIR;
           }
           if (lane == 0) sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
           __syncwarp();
@@ -679,14 +810,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (load)
               load_bulk(at + ((item >> 20) & 2047u) * rc * 32,
                         static_cast<const uint8_t*>(g.b) +
-                            ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles + outs) *
-                                 g.rank + c) * (kTileN * 2),
+                            ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles +
+                              min(outs, g.out_tiles - 1)) * g.rank + c) * (kTileN * 2),
                         rc * kTileN * 2, bar);
             load_bulk(at + ((item >> 9) & 2047u) * rc * 32,
                       g.low + (static_cast<int64_t>(rows) * g.most_blocks + sh.blocks[i0 + lane]) *
-                                  (g.rank * g.parts * 32) + wide * c * 32,
+                                  (g.rank * g.parts * 32) + wide * (cta * g.rank + c) * 32,
                       wide * rc * 32, bar);
           }
+          own |= 1u << stage;
+          uses ^= 1u << stage;
           next();
         }
       }
@@ -697,29 +830,63 @@ __global__ void __launch_bounds__(kThreads, 1)
             sh.shape[stage] = kEnd;
             bar_arrive(shared_addr(&sh.full[stage]));
           }
+          own |= 1u << stage;
+          uses ^= 1u << stage;
           next();
         }
       }
     }
     if (g.ids && !waited) pdl_wait();
+    if (PAIR == 2) {  // the pair's instructions are through, and their arrivals here
+      for (int i = 0; i < S::kStages && ok; ++i) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
     if (!ok && lane == 0) {
       // give up: wait for the copies that are still on their way
       sh.failed = 1;
-      const int32_t open = min(issued, S::kStages);
-      for (int32_t i = issued - open; i < issued; ++i)
-        bar_wait(shared_addr(&sh.full[i % S::kStages]), (i / S::kStages) & 1);
+      if (cta == 0) {
+        const int32_t open = min(issued, S::kStages);
+        for (int32_t i = issued - open; i < issued; ++i)
+          bar_wait(shared_addr(&sh.full[i % S::kStages]), (i / S::kStages) & 1);
+      } else {
+        for (int i = 0; i < S::kStages; ++i)
+          if (own >> i & 1u) bar_wait(shared_addr(&sh.full[i]), (uses >> i & 1u) ^ 1u);
+      }
     }
+  } else if (warp == 1 && cta == 1) {
+    // --- a pair's second CTA says which of its adapters' steps are loaded -----
+    if (lane == 0 && g.ids) {
+      int32_t stage = 0;
+      uint32_t uses = 0;
+      for (int32_t tile = first; tile < tiles && ok; tile += stride) {
+        stage = (stage + s1 - s0) % S::kStages;
+        for (bool end = false; !end;) {
+          if (!(ok = bar_wait(shared_addr(&sh.full[stage]), uses >> stage & 1u))) break;
+          uses ^= 1u << stage;
+          end = sh.shape[stage] == kEnd;
+          bar_tell(shared_addr(&sh.peer[stage]));
+          if (++stage == S::kStages) stage = 0;
+        }
+      }
+      if (!ok) sh.failed = 1;
+    }
+    __syncwarp();
   } else if (warp == 1) {
     // --- products ------------------------------------------------------------
     if (lane == 0) {
       int32_t stage = 0, buffer = 0;
-      uint32_t phase = 0, turn = 0;
+      uint32_t phase = 0, turn = 0, told = 0;
       for (int32_t tile = first; tile < tiles && ok; tile += stride) {
-        if (!(ok = bar_wait(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
+        if (!(ok = bar_wait_free<PAIR>(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
         fence_after();
         uint32_t d = tmem + buffer * NT;
         auto finish = [&] {
-          mma_commit(shared_addr(&sh.empty[stage]));
+          mma_commit<PAIR>(shared_addr(&sh.empty[stage]));
           if (++stage == S::kStages) {
             stage = 0;
             phase ^= 1;
@@ -727,10 +894,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         for (int32_t s = s0; s < s1; ++s) {
           if (kGroups && s > s0 && (s - s0) % kGroup == 0) {  // the other accumulator
-            mma_commit(shared_addr(&sh.done[buffer]));
+            mma_commit<PAIR>(shared_addr(&sh.done[buffer]));
             buffer ^= 1;
             turn ^= buffer == 0;
-            if (!(ok = bar_wait(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
+            if (!(ok = bar_wait_free<PAIR>(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
             fence_after();
             d = tmem + buffer * NT;
           }
@@ -740,16 +907,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t wd = desc_swizzled(at), xd = desc_swizzled(at + S::kWeightBytes);
 #pragma unroll
           for (int k = 0; k < kStepK / 16; ++k)
-            mma(d, wd + 2 * k, xd + 2 * k, instruction<T>(NT),
-                k > 0 || (kGroups ? (s - s0) % kGroup != 0 : s > s0));
+            mma<PAIR>(d, wd + 2 * k, xd + 2 * k, instruction<T, PAIR>(NT),
+                      k > 0 || (kGroups ? (s - s0) % kGroup != 0 : s > s0));
           finish();
         }
         if (!ok) break;
         if (g.ids) {
           for (;;) {
             if (!(ok = bar_wait(shared_addr(&sh.full[stage]), phase))) break;
+            if (PAIR == 2) {
+              ok = wait_for([&] { return bar_told(shared_addr(&sh.peer[stage]), told >> stage & 1u); });
+              if (!ok) break;
+              told ^= 1u << stage;
+            }
             fence_after();
-            const uint32_t at = ring + stage * S::kStageBytes;
             const uint32_t shape = sh.shape[stage];
             if (shape == kEnd) {
               finish();
@@ -760,10 +931,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               const Op op = sh.op[stage][i];
               uint64_t low = op.low;
               for (int32_t p = 0; p < g.parts; ++p, low += op.next) {
-                mma(d + op.to, op.b, low, op.idesc, true);
+                mma<PAIR>(d + op.to, op.b, low, op.idesc, true);
                 if (rc > 16) {
                   low += op.next;
-                  mma(d + op.to, op.b + kTileN * 2, low, op.idesc, true);
+                  mma<PAIR>(d + op.to, op.b + kTileN * 2, low, op.idesc, true);
                 }
               }
             }
@@ -771,13 +942,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!ok) break;
         }
-        mma_commit(shared_addr(&sh.done[buffer]));
+        mma_commit<PAIR>(shared_addr(&sh.done[buffer]));
         buffer ^= 1;
         turn ^= buffer == 0;
       }
       if (!ok) {
         sh.failed = 1;
-        mma_commit(shared_addr(&sh.last));
+        mma_commit_here<PAIR>(shared_addr(&sh.last));
         bar_wait(shared_addr(&sh.last), 0);
       }
     }
@@ -791,7 +962,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t turn = 0;
     const int32_t groups = kGroups ? (s1 - s0 + kGroup - 1) / kGroup : 1;
     for (int32_t tile = first; tile < tiles && ok; tile += stride) {
-      const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles;
+      const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles * PAIR + cta;
       const int32_t n = outs * kTileN + quarter * 32 + lane;
       OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
       const int32_t have = min(NT, g.T - rows * NT);
@@ -838,7 +1009,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         fence_before();
-        if (lane == 0) bar_arrive(shared_addr(&sh.free[buffer]));
+        if (lane == 0) {
+          if (cta == 0)
+            bar_arrive(shared_addr(&sh.free[buffer]));
+          else
+            bar_arrive_at(shared_addr(&sh.free[buffer]), 0);
+        }
         buffer ^= 1;
         turn ^= buffer == 0;
       }
@@ -851,6 +1027,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncwarp();
+  if (PAIR == 2) cluster_sync();  // nothing reads or arrives in the other CTA any more
   if (split > 1) {
     cluster_sync();
     // this CTA's share of the tile's rows, summed over the cluster in its order
@@ -881,8 +1058,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "n"(S::kColumns));
+    if constexpr (PAIR == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "n"(S::kColumns));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "n"(S::kColumns));
   }
   if (tid == 0 && sh.failed) atomicExch(&g_error, 1u);
 }
@@ -929,6 +1110,17 @@ int32_t row_tile(int32_t rows, bool fp32) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || fp32 ? 128 : 256;
 }
 
+// Whether two CTAs share the instructions of tiles of 256 rows: each then loads
+// half of x, which is most of what an SM loads of them (at 4096 x 65536, 256
+// rows: 118 us in pairs, 135 alone; 4096 rows by 8192 outputs: 177, 188). With
+// smaller tiles W is most of it, and pairs gain nothing (64 rows, 128,256
+// outputs: 172, 169; 128 rows, 65,536 outputs: 102, 103). With adapters, whose
+// first steps wait longer in a pair, only where SMs have more than one tile (86
+// tiles of outputs, 24 adapters: 54 us in pairs, 48 alone; 512 tiles: 150, 161).
+int32_t pair_of(int32_t nt, int64_t tiles, bool adapters) {
+  return nt == 256 && tiles * (adapters ? 1 : 2) > sm_count() ? 2 : 1;
+}
+
 struct Workspace {
   int32_t most_blocks;
   size_t count, items, low, bytes;
@@ -946,41 +1138,43 @@ Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters, bool fp32) 
   return w;
 }
 
-template <typename T, typename O, int NT>
+template <typename T, typename O, int NT, int PAIR>
 cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
                         cudaStream_t st) {
   static std::atomic<bool> ready[64];
-  auto kernel = project_kernel<T, O, NT>;
+  using S = Shape<NT, PAIR>;
+  auto kernel = project_kernel<T, O, NT, PAIR>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Shape<NT>::kBytes);
+                             S::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
-  const int64_t tiles = static_cast<int64_t>(g.row_tiles) * g.out_tiles;
+  const int64_t tiles = static_cast<int64_t>(g.row_tiles) * ((g.out_tiles + PAIR - 1) / PAIR);
   const int32_t sms = sm_count(), steps = (g.K + kStepK - 1) / kStepK;
   // Few tiles leave SMs idle: a cluster then shares a tile, each CTA with a
   // part of the inner elements.
   int32_t split = 1;
-  while (split < kMaxSplit && tiles * split * 2 <= sms && split * 2 <= steps) split *= 2;
+  while (PAIR == 1 && split < kMaxSplit && tiles * split * 2 <= sms && split * 2 <= steps)
+    split *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? tiles * split
-                                                     : std::min<int64_t>(tiles, sms)));
+                                                     : std::min<int64_t>(tiles, sms / PAIR) * PAIR));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<NT>::kBytes;
+  cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = BPD_PDL ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.x = split * PAIR;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = split > 1 ? 2 : 1;
+  cfg.numAttrs = split * PAIR > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g, split);
 }
 
@@ -1044,12 +1238,14 @@ cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, con
   cudaError_t e = g.ids ? launch_shrink<T>(g, st) : cudaSuccess;
   if (e == cudaSuccess) {
     switch (g.tile) {
-      case 16: e = launch_tile<T, O, 16>(wmap, xmap, g, st); break;
-      case 32: e = launch_tile<T, O, 32>(wmap, xmap, g, st); break;
-      case 64: e = launch_tile<T, O, 64>(wmap, xmap, g, st); break;
-      case 128: e = launch_tile<T, O, 128>(wmap, xmap, g, st); break;
-      default:
-        if constexpr (!std::is_same_v<O, float>) e = launch_tile<T, O, 256>(wmap, xmap, g, st);
+      case 16: e = launch_tile<T, O, 16, 1>(wmap, xmap, g, st); break;
+      case 32: e = launch_tile<T, O, 32, 1>(wmap, xmap, g, st); break;
+      case 64: e = launch_tile<T, O, 64, 1>(wmap, xmap, g, st); break;
+      case 128: e = launch_tile<T, O, 128, 1>(wmap, xmap, g, st); break;
+      default:  // an fp32 result has tiles of up to 128 rows
+        if constexpr (!std::is_same_v<O, float>)
+          e = g.pair == 2 ? launch_tile<T, O, 256, 2>(wmap, xmap, g, st)
+                          : launch_tile<T, O, 256, 1>(wmap, xmap, g, st);
     }
   }
   if (e != cudaSuccess) (void)cudaGetLastError();
@@ -1118,12 +1314,13 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   const int32_t row_tiles = (rows - 1) / nt + 1, out_tiles = (out_features - 1) / kTileN + 1;
   if (static_cast<int64_t>(row_tiles) * out_tiles > INT_MAX / 2)
     return fail(BPD_ERR_CAPACITY, "%s: too many tiles", what);
+  const int32_t pair = pair_of(nt, static_cast<int64_t>(row_tiles) * out_tiles, ids != nullptr);
   const EncodeFn encode = encoder();
   if (!encode) return fail(BPD_ERR_CUDA, "%s: the driver has no tensor maps", what);
   CUtensorMap wmap, xmap;
   const bool bf16 = dtype == BPD_BF16;
   if (!matrix_map(&wmap, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
-      !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, nt))
+      !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, nt / pair))
     return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
   const Workspace w = workspace_of(rows, rank, num_adapters, fp32);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1131,7 +1328,7 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
                    reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, w.most_blocks, row_tiles,
-                   out_tiles, fp32 && bf16 ? 3 : 2};
+                   out_tiles, fp32 && bf16 ? 3 : 2, pair};
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (bf16)

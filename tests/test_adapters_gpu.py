@@ -92,6 +92,27 @@ def test_mixes_of_adapters(kind, T) -> None:
     check(got, *c)
 
 
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("T,K,N,n,r,order", [
+    (33, 136, 9601, 5, 16, "mixed"), (50, 1608, 9733, 43, 12, "runs"),
+    (64, 64, 9728, 1, 16, "all"), (65, 320, 10240, 70, 33, "mixed"),
+    (100, 520, 19000, 9, 48, "runs"), (128, 8, 9610, 128, 8, "mixed"),
+    (200, 200, 9733, 43, 12, "runs"), (256, 768, 9857, 24, 16, "mixed"),
+    (290, 136, 6500, 300, 16, "mixed"), (600, 264, 4999, 8, 128, "runs"),
+    (1030, 512, 2049, 11, 64, "runs")])
+def test_tiles_for_every_sm(dtype, out, T, K, N, n, r, order) -> None:
+    """More tiles than half of the SMs: two CTAs then share a tile's products."""
+    from bpdecode_b200.adapters import project
+
+    t = torch.arange(T)
+    ids = {"mixed": None, "all": torch.zeros(T).long(), "runs": t * (n + 1) // T - 1}[order]
+    c = make(T, K, N, n, r, dtype, seed=T + N, ids=ids if ids is None else ids.cuda())
+    bank = bank_of(*c[2:5])
+    got = project(c[0], c[1], bank, c[5], out_dtype=out)
+    check(got, *c)
+    assert torch.equal(got, project(c[0], c[1], bank, c[5], out_dtype=out))
+
+
 def test_no_bank_is_the_projection_alone() -> None:
     from bpdecode_b200.adapters import project
 
