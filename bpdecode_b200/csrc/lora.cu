@@ -56,6 +56,11 @@ constexpr int kRankStep = 32;      // inner elements of an adapter's step, at mo
 constexpr int kMaxItems = 8;       // items of an adapters' step, at most
 constexpr int kGroup = 8;           // steps that an fp32 result is accumulated over at once
 constexpr int kReach = 4;          // blocks that an item spans for each row that it has, at most
+// Tiles of rows up to which S is gathered row by row beside the product: with
+// more, products of all of a block's adapters in front of it take less (750 rows
+// by 4096 x 8192, 8 adapters of rank 64: 61 us, gathered 79; 24 of rank 16: 76,
+// 85; 4096 rows: 201, 217), with fewer, more (500 rows, 24 of rank 16: 66, 52).
+constexpr int kGatherTiles = 2;
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share one tile's inner elements
 constexpr int kThreads = 192;      // loads, products, four warps that write
 constexpr int kShrinkThreads = 256;
@@ -305,14 +310,15 @@ constexpr uint32_t instruction(uint32_t n) {
 }
 
 // ---------------------------------------------------------------------------
-// S. An item's rows are gathered, up to 16 * GROUPS of them, and multiplied by
-// its adapter's A over all inner elements; the warps split over 16-row groups
-// and over the inner elements, which a cluster splits further where there are
-// few items. Bound by the latency of reading A and x, and hidden behind the
-// product's reading of W: a CTA is small enough (20 KB of shared memory) to
-// stand beside one of the product's. The products go through mma.sync, whose
-// rate is no limit here. The order of the inner elements within a step is
-// permuted, alike in both operands, so that every load is 16 bytes.
+// S. An item's rows are gathered, up to 16 of them, and multiplied by its
+// adapter's A over all inner elements; the warps split over the inner elements,
+// which a cluster splits further where there are few items. Bound by the latency
+// of reading A and x (12 to 18 us alone: 64 to 256 rows, 24 adapters of 4096
+// inner elements), and hidden behind the product's reading of W: a CTA is small
+// enough (20 KB of shared memory) to stand beside one of the product's. The
+// products go through mma.sync, whose rate is no limit here. The order of the
+// inner elements within a step is permuted, alike in both operands, so that every
+// load is 16 bytes.
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -332,33 +338,50 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
   }
 }
 
-template <typename T, int GROUPS, int RS>
-__global__ void __launch_bounds__(kShrinkThreads, 2)
-    shrink_kernel(const LoraArgs g, const int32_t turns, const int32_t split) {
-  using Bits = typename Dt<T>::Bits;
+// Where an item of `blocks` keeps eight values of S of its row `row`, from the
+// inner element `col`: [CTA of the pair][rank step][part][rank / 8][rows][8].
+__device__ __forceinline__ uint8_t* place_of(const LoraArgs& g, uint8_t* low, int32_t blocks,
+                                             int32_t row, int32_t col, int32_t which) {
+  const int32_t rows = blocks * kBlock / g.pair, cta = row >= rows;
+  const int32_t c = col / kRankStep * kRankStep, wide = min(kRankStep, g.rank - c);
+  return low + (cta * g.rank * g.parts + c * g.parts + which * wide) * rows * 2 +
+         ((col - c) >> 3) * rows * 16 + (row - cta * rows) * 16;
+}
+// Writes them: each 16-bit part is the rounding of what those before it left.
+template <typename T>
+__device__ __forceinline__ void put_low(const LoraArgs& g, uint8_t* low, int32_t blocks,
+                                        int32_t row, int32_t col, float (&s)[8]) {
+  for (int32_t which = 0; which < g.parts; ++which) {
+    alignas(16) typename Dt<T>::Bits part_of[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      part_of[e] = Dt<T>::from_float_dev(s[e]);
+      s[e] -= Dt<T>::to_float(part_of[e]);
+    }
+    *reinterpret_cast<uint4*>(place_of(g, low, blocks, row, col, which)) =
+        *reinterpret_cast<uint4*>(part_of);
+  }
+}
+
+// The items of a tile of rows, made by kShrinkThreads threads, one for each row.
+struct Plan {
+  alignas(16) int32_t ids[256];
+  uint2 items[256];       // as in LoraArgs
+  uint16_t members[256];  // rows of an item that are its adapter's
+  int32_t warp_items[kShrinkThreads / 32], warp_blocks[kShrinkThreads / 32];
+};
+
+// How many there are; `own` is the adapter of this thread's row, `rows_in` the
+// rows that have it, a bit each.
+__device__ __forceinline__ int32_t plan_items(const LoraArgs& g, int32_t t0, Plan& sh,
+                                              int32_t& own, uint32_t (&rows_in)[8]) {
   constexpr int kWarps = kShrinkThreads / 32;
-  constexpr int kRows = GROUPS * 16;           // rows of a unit
-  constexpr int kParts = kWarps / GROUPS;      // parts of the inner elements
-  constexpr int kSlots = std::min(kParts, 4096 / (kRows * RS));  // parts that are added at once
-  constexpr int kUnroll = RS == 16 ? 4 : RS == 32 ? 3 : 2;
-  __shared__ int32_t ids[256];
-  __shared__ uint2 items[256];
-  __shared__ uint16_t members[256];  // of an item
-  __shared__ uint8_t list[256];      // the rows of this item in the tile
-  __shared__ int32_t warp_items[kWarps], warp_blocks[kWarps], warp_rows[kWarps];
-  __shared__ float sums[kSlots][kRows][RS];
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t kpart = blockIdx.x % split;
-  const int32_t turn = blockIdx.x / split % turns, tile = blockIdx.x / split / turns;
-  const int32_t t0 = tile * g.tile;
-  pdl_wait();
-  pdl_trigger();  // what ran before has completed: x is there for the next kernel, too
-  const int32_t own = tid < g.tile ? adapter_of(g, t0 + tid) : -1;
-  ids[tid] = own;
+  own = tid < g.tile ? adapter_of(g, t0 + tid) : -1;
+  sh.ids[tid] = own;
   __syncthreads();
   // The first row of each adapter finds the adapter's items: runs of blocks
   // that hold at least one of its rows for every kReach blocks.
-  uint32_t rows_in[8];  // the rows with this thread's adapter, a bit each
   bool lead = own >= 0;
   int32_t found = 0, blocks = 0;
   auto each_item = [&](auto&& f) {
@@ -388,7 +411,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
       uint32_t m = 0;
 #pragma unroll
       for (int32_t j = 0; j < 32; j += 4) {
-        const int4 v = *reinterpret_cast<const int4*>(&ids[w * 32 + j]);
+        const int4 v = *reinterpret_cast<const int4*>(&sh.ids[w * 32 + j]);
         m |= (v.x == own ? 1u : 0u) << j | (v.y == own ? 2u : 0u) << j |
              (v.z == own ? 4u : 0u) << j | (v.w == own ? 8u : 0u) << j;
       }
@@ -413,8 +436,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     }
   }
   if (lane == 31) {
-    warp_items[warp] = at_item;
-    warp_blocks[warp] = at_block;
+    sh.warp_items[warp] = at_item;
+    sh.warp_blocks[warp] = at_block;
   }
   __syncthreads();
   int32_t total = 0;
@@ -423,37 +446,61 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) {
-      at_item += warp_items[w];
-      at_block += warp_blocks[w];
+      at_item += sh.warp_items[w];
+      at_block += sh.warp_blocks[w];
     }
-    total += warp_items[w];
+    total += sh.warp_items[w];
   }
   if (lead)
     each_item([&](int32_t start, int32_t n, int32_t rows) {
-      items[at_item] = make_uint2(static_cast<uint32_t>(own),
+      sh.items[at_item] = make_uint2(static_cast<uint32_t>(own),
                                   static_cast<uint32_t>(at_block << 9 | start << 5 | n));
-      members[at_item++] = static_cast<uint16_t>(rows);
+      sh.members[at_item++] = static_cast<uint16_t>(rows);
       at_block += n;
     });
   __syncthreads();
+  return total;
+}
+
+template <typename T, int RS>
+__global__ void __launch_bounds__(kShrinkThreads, 2)
+    shrink_kernel(const LoraArgs g, const int32_t turns, const int32_t split) {
+  using Bits = typename Dt<T>::Bits;
+  constexpr int kWarps = kShrinkThreads / 32;
+  constexpr int kRows = 16;  // of a unit
+  constexpr int kSlots = std::min(kWarps, 4096 / (kRows * RS));  // parts that are added at once
+  constexpr int kUnroll = RS == 16 ? 4 : RS == 32 ? 3 : 2;
+  __shared__ Plan plan;
+  __shared__ uint8_t list[256];      // the rows of this item in the tile
+  __shared__ int32_t warp_rows[kWarps];
+  __shared__ float sums[kSlots][kRows][RS];
+  const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t kpart = blockIdx.x % split;
+  const int32_t turn = blockIdx.x / split % turns, tile = blockIdx.x / split / turns;
+  const int32_t t0 = tile * g.tile;
+  pdl_wait();
+  pdl_trigger();  // what ran before has completed: x is there for the next kernel, too
+  int32_t own;
+  uint32_t rows_in[8];
+  const int32_t total = plan_items(g, t0, plan, own, rows_in);
   if (turn == 0 && kpart == 0) {
-    if (tid < total) g.items[static_cast<int64_t>(tile) * g.tile + tid] = items[tid];
+    if (tid < total) g.items[static_cast<int64_t>(tile) * g.tile + tid] = plan.items[tid];
     if (tid == 0) g.count[tile] = total;
   }
 
-  const int32_t group = warp % GROUPS, part = warp / GROUPS + kpart * kParts;
+  const int32_t part = warp + kpart * kWarps;
   // each part is a contiguous share of the inner elements, a multiple of 32
-  const int32_t share = ((g.K + 31) / 32 + kParts * split - 1) / (kParts * split) * 32;
+  const int32_t share = ((g.K + 31) / 32 + kWarps * split - 1) / (kWarps * split) * 32;
   const int32_t k0 = min(g.K, part * share), k1 = min(g.K, k0 + share);
   // units are counted through the items; this CTA takes every turns-th
   int32_t before = 0, next = turn;
   for (int32_t i = 0; i < total; ++i) {
-    const int32_t units = (members[i] + kRows - 1) / kRows, u0 = next - before;
+    const int32_t units = (plan.members[i] + kRows - 1) / kRows, u0 = next - before;
     before += units;
     if (u0 >= units) continue;  // alike in all threads of the cluster
-    const int32_t a = static_cast<int32_t>(items[i].x);
-    const int32_t n = items[i].y & 31u, b0 = (items[i].y >> 5) & 15u;
-    uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (items[i].y >> 9)) *
+    const int32_t a = static_cast<int32_t>(plan.items[i].x);
+    const int32_t n = plan.items[i].y & 31u, b0 = (plan.items[i].y >> 5) & 15u;
+    uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (plan.items[i].y >> 9)) *
                                (g.rank * g.parts * 32);
     const float scale = g.scale[a];
     // the item's rows, in order
@@ -465,39 +512,33 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     for (int32_t w = 0; w < warp; ++w) at += warp_rows[w];
     if (mine) list[at] = static_cast<uint8_t>(tid);
     __syncthreads();
-    // An operand's place: [CTA of the pair][rank step][part][rank / 8][rows][8].
-    const int32_t rows = n * kBlock / g.pair;
     auto place = [&](int32_t row, int32_t col, int32_t which) {
-      const int32_t c = col / kRankStep * kRankStep, wide = min(kRankStep, g.rank - c);
-      const int32_t cta = row >= rows;
-      return low + (cta * g.rank * g.parts + c * g.parts + which * wide) * rows * 2 +
-             ((col - c) >> 3) * rows * 16 + (row - cta * rows) * 16;
+      return place_of(g, low, n, row, col, which);
     };
     if (u0 == 0) {  // the rows between
       for (int32_t v = tid + kpart * kShrinkThreads; v < n * kBlock * (g.rank / 8);
            v += kShrinkThreads * split) {
         const int32_t row = v % (n * kBlock), col = v / (n * kBlock) * 8;
-        if (ids[b0 * kBlock + row] != a) {
+        if (plan.ids[b0 * kBlock + row] != a) {
           for (int32_t which = 0; which < g.parts; ++which)
             *reinterpret_cast<uint4*>(place(row, col, which)) = uint4{};
         }
       }
     }
     for (int32_t u = u0; u < units; u += turns, next += turns) {
-      const int32_t m0 = u * kRows, have = min(kRows, members[i] - m0);
-      const int32_t r0 = group * 16 + (lane >> 2), r1 = r0 + 8;  // this lane's two rows
+      const int32_t m0 = u * kRows, have = min(kRows, plan.members[i] - m0);
+      const int32_t r0 = lane >> 2, r1 = r0 + 8;  // this lane's two rows
       const bool in0 = r0 < have, in1 = r1 < have;
       const Bits* x0 = static_cast<const Bits*>(g.x) +
                        static_cast<int64_t>(t0 + (in0 ? list[m0 + r0] : 0)) * g.x_stride;
       const Bits* x1 = static_cast<const Bits*>(g.x) +
                        static_cast<int64_t>(t0 + (in1 ? list[m0 + r1] : 0)) * g.x_stride;
-      const bool idle = group * 16 >= have;
       for (int32_t c = 0; c < g.rank; c += RS) {
         const int32_t rc = min(RS, g.rank - c);
         const Bits* w = static_cast<const Bits*>(g.a) +
                         (static_cast<int64_t>(a) * g.rank + c + (lane >> 2)) * g.K;
         float acc[RS / 8][4] = {};
-        for (int32_t k = idle ? k1 : k0; k < k1; k += 32 * kUnroll) {
+        for (int32_t k = k0; k < k1; k += 32 * kUnroll) {
           uint4 p[kUnroll], q[kUnroll], v[kUnroll][RS / 8];
 #pragma unroll
           for (int s = 0; s < kUnroll; ++s) {
@@ -520,8 +561,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
             }
         }
         // the parts meet in a fixed order, kSlots at a time
-        for (int32_t round = 0; round < kParts; round += kSlots) {
-          const int32_t slot = warp / GROUPS - round;
+        for (int32_t round = 0; round < kWarps; round += kSlots) {
+          const int32_t slot = warp - round;
           if (slot >= 0 && slot < kSlots) {
 #pragma unroll
             for (int j = 0; j < RS / 8; ++j)
@@ -568,17 +609,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[e] *= scale;
-          const int32_t row = list[m0 + r] - b0 * kBlock;
-          for (int32_t which = 0; which < g.parts; ++which) {
-            alignas(16) Bits part_of[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              part_of[e] = Dt<T>::from_float_dev(s[e]);
-              s[e] -= Dt<T>::to_float(part_of[e]);
-            }
-            *reinterpret_cast<uint4*>(place(row, c + col, which)) =
-                *reinterpret_cast<uint4*>(part_of);
-          }
+          put_low<T>(g, low, n, list[m0 + r] - b0 * kBlock, c + col, s);
         }
         if (split > 1)
           cluster_sync();
@@ -587,6 +618,290 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
       }
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// S of prompts: 128 rows of x by the adapters that they have, up to 128 of their
+// ranks at a time, as tcgen05 products whose D holds a row in each lane; a row
+// keeps the columns of its own adapter. A cluster splits the inner elements.
+// Bound by the loads of x and A and by what they wait for at first: 22 us alone
+// for 4096 rows of 8 adapters of rank 64 (45 gathered), 25 at rank 128. Its CTAs
+// leave no room for the product's, which begins as they end.
+
+constexpr int kWideRows = 128;
+constexpr int kWideRanks = 128;  // columns of D at a time
+constexpr int kWideStageBytes = (kWideRows + kWideRanks) * kStepK * 2;
+constexpr int kWideStages = 4;
+constexpr int kWideBytes =
+    kWideStages * kWideStageBytes + kWideRows * (kWideRanks + 4) * 4 + 1024;
+
+struct WideShared {
+  Plan plan;
+  uint64_t full[kWideStages], empty[kWideStages], done[2], free[2], last;
+  uint32_t tmem, failed;
+  int32_t who[kWideRows];   // the adapters of these rows
+  int32_t count[kWideRows / 32];
+  int32_t item[kWideRows];  // of a row
+  float scale[kWideRows];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kShrinkThreads, 1)
+    shrink_wide_kernel(const __grid_constant__ CUtensorMap amap,
+                       const __grid_constant__ CUtensorMap xmap, const LoraArgs g,
+                       const int32_t split) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ WideShared sh;
+  const uint32_t ring = (shared_addr(dynamic) + 1023u) & ~1023u;
+  const int32_t pitch = g.rank + 4;  // of a row's sums, 16-byte aligned
+  const uint32_t sums = ring + kWideStages * kWideStageBytes;
+  const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t kpart = blockIdx.x % split, block = blockIdx.x / split;
+  const int32_t halves = g.tile / kWideRows, tile = block / halves;
+  const int32_t base = block % halves * kWideRows;  // of these rows in their tile
+  const int32_t t0 = tile * g.tile;
+  const int32_t steps = (g.K + kStepK - 1) / kStepK;
+  const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(steps) * kpart / split);
+  const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(steps) * (kpart + 1) / split);
+  if (tid == 0) {
+    for (int i = 0; i < kWideStages; ++i) {
+      bar_init(shared_addr(&sh.full[i]), 1);
+      bar_init(shared_addr(&sh.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(shared_addr(&sh.done[i]), 1);
+      bar_init(shared_addr(&sh.free[i]), 4);
+    }
+    bar_init(shared_addr(&sh.last), 1);
+    sh.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     shared_addr(&sh.tmem)),
+                 "n"(2 * kWideRanks)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pdl_trigger();
+  int32_t own;
+  uint32_t rows_in[8];
+  const int32_t total = plan_items(g, t0, sh.plan, own, rows_in);
+  if (base == 0 && kpart == 0) {
+    if (tid < total) g.items[static_cast<int64_t>(tile) * g.tile + tid] = sh.plan.items[tid];
+    if (tid == 0) g.count[tile] = total;
+  }
+  // the adapters of these rows, in the order of their first rows
+  const bool here = tid >= base && tid < base + kWideRows;
+  bool lead = here && own >= 0;
+  if (lead) {
+#pragma unroll
+    for (int32_t w = 0; w < 8; ++w) {
+      if (w < base / 32) continue;
+      if (w < warp) lead = lead && rows_in[w] == 0;
+      if (w == warp) lead = lead && (rows_in[w] & ((1u << lane) - 1u)) == 0;
+    }
+  }
+  const uint32_t vote = __ballot_sync(kFull, lead);
+  if (here && lane == 0) sh.count[warp - base / 32] = __popc(vote);
+  __syncthreads();
+  int32_t adapters = 0;
+#pragma unroll
+  for (int w = 0; w < kWideRows / 32; ++w) adapters += sh.count[w];
+  if (lead) {
+    int32_t at = __popc(vote & ((1u << lane) - 1u));
+    for (int32_t w = 0; w < warp - base / 32; ++w) at += sh.count[w];
+    sh.who[at] = own;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int32_t most = kWideRanks / g.rank;  // adapters at a time
+  const int32_t chunks = (adapters + most - 1) / most;
+  // as the product, an fp32 result's sums of 512 inner elements at a time
+  const int32_t group = g.parts == 3 ? kGroup : steps;
+  bool ok = true;
+  if (warp == 0) {
+    int32_t stage = 0, issued = 0;
+    uint32_t phase = 0;
+    for (int32_t c = 0; c < chunks && ok; ++c) {
+      const int32_t n = min(most, adapters - c * most);
+      for (int32_t s = s0; s < s1; ++s) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
+        if (!ok) break;
+        const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * kWideStageBytes;
+        if (lane == 0) {
+          bar_expect(bar, kWideRows * kStepK * 2 + n * g.rank * kStepK * 2);
+          load_box(at, &xmap, s * kStepK, t0 + base, bar);
+        }
+        __syncwarp();
+        if (lane < n)
+          load_box(at + (kWideRows + lane * g.rank) * kStepK * 2, &amap, s * kStepK,
+                   sh.who[c * most + lane] * g.rank, bar);
+        ++issued;
+        if (++stage == kWideStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      sh.failed = 1;
+      for (int32_t i = issued - min(issued, kWideStages); i < issued; ++i)
+        bar_wait(shared_addr(&sh.full[i % kWideStages]), (i / kWideStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int32_t stage = 0, buffer = 0;
+      uint32_t phase = 0, turn = 0;
+      for (int32_t c = 0; c < chunks && ok; ++c) {
+        const int32_t n = min(most, adapters - c * most);
+        for (int32_t s = s0; s < s1; ++s) {
+          const bool fresh = (s - s0) % group == 0;
+          if (fresh) {
+            if (!(ok = bar_wait(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
+          }
+          if (!(ok = bar_wait(shared_addr(&sh.full[stage]), phase))) break;
+          fence_after();
+          const uint32_t at = ring + stage * kWideStageBytes;
+          const uint64_t xd = desc_swizzled(at), ad = desc_swizzled(at + kWideRows * kStepK * 2);
+#pragma unroll
+          for (int k = 0; k < kStepK / 16; ++k)
+            mma<1>(tmem + buffer * kWideRanks, xd + 2 * k, ad + 2 * k,
+                   instruction<T, 1>(0) | (n * g.rank >> 3) << 17, k > 0 || !fresh);
+          mma_commit<1>(shared_addr(&sh.empty[stage]));
+          if (++stage == kWideStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (s + 1 == s1 || (s + 1 - s0) % group == 0) {
+            mma_commit<1>(shared_addr(&sh.done[buffer]));
+            buffer ^= 1;
+            turn ^= buffer == 0;
+          }
+        }
+      }
+      if (!ok) {
+        sh.failed = 1;
+        mma_commit<1>(shared_addr(&sh.last));
+        bar_wait(shared_addr(&sh.last), 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    const int32_t quarter = warp & 3, r = quarter * 32 + lane;
+    const int32_t a = sh.plan.ids[base + r];
+    int32_t slot = -1;
+    if (a >= 0) {
+      sh.scale[r] = g.scale[a];
+      for (int32_t i = 0; i < adapters; ++i)
+        if (sh.who[i] == a) slot = i;
+      const int32_t at = (base + r) / kBlock;
+      for (int32_t i = 0; i < total; ++i) {
+        const uint2 item = sh.plan.items[i];
+        if (item.x == static_cast<uint32_t>(a) &&
+            static_cast<uint32_t>(at) - ((item.y >> 5) & 15u) < (item.y & 31u))
+          sh.item[r] = i;
+      }
+    }
+    int32_t buffer = 0;
+    uint32_t turn = 0;
+    for (int32_t c = 0; c < chunks && ok; ++c) {
+      const int32_t n = min(most, adapters - c * most);
+      for (int32_t s = s0; s < s1; s += group) {
+        ok = __all_sync(kFull, bar_wait(shared_addr(&sh.done[buffer]), turn));
+        if (!ok) {
+          sh.failed = 1;
+          break;
+        }
+        fence_after();
+        for (int32_t i = 0; i < n; ++i) {
+          const bool mine = slot == c * most + i;
+          if (!__any_sync(kFull, mine)) continue;
+          for (int32_t col = 0; col < g.rank; col += 16) {
+            uint32_t v[16];
+            tmem_load16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buffer * kWideRanks +
+                            i * g.rank + col, v);
+            if (!mine) continue;
+            const uint32_t to = sums + (r * pitch + col) * 4;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              float f[4] = {};
+              if (s > s0)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
+                             : "r"(to + e * 4)
+                             : "memory");
+              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + e * 4),
+                           "f"(f[0] + __uint_as_float(v[e])), "f"(f[1] + __uint_as_float(v[e + 1])),
+                           "f"(f[2] + __uint_as_float(v[e + 2])),
+                           "f"(f[3] + __uint_as_float(v[e + 3]))
+                           : "memory");
+            }
+          }
+        }
+        fence_before();
+        if (lane == 0) bar_arrive(shared_addr(&sh.free[buffer]));
+        buffer ^= 1;
+        turn ^= buffer == 0;
+      }
+    }
+  } else {
+    // the rows between an item's, of these 128: a warp takes whole items
+    for (int32_t i = kpart * 2 + warp - 6; i < total; i += 2 * split) {
+      const uint2 item = sh.plan.items[i];
+      const int32_t n = item.y & 31u, b0 = (item.y >> 5) & 15u;
+      if (sh.plan.members[i] == n * kBlock) continue;
+      uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (item.y >> 9)) *
+                                 (g.rank * g.parts * 32);
+      const int32_t from = max(b0 * kBlock, base), to = min((b0 + n) * kBlock, base + kWideRows);
+      for (int32_t row = from + lane; row < to; row += 32) {
+        if (sh.plan.ids[row] == static_cast<int32_t>(item.x)) continue;
+        for (int32_t which = 0; which < g.parts; ++which)
+          for (int32_t col = 0; col < g.rank; col += 8)
+            *reinterpret_cast<uint4*>(place_of(g, low, n, row - b0 * kBlock, col, which)) = uint4{};
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  // this CTA's share of the rows, summed over the cluster in its order
+  for (int32_t v = tid; v < kWideRows / split * (g.rank / 8); v += kShrinkThreads) {
+    const int32_t r = v / (g.rank / 8) * split + kpart, col = v % (g.rank / 8) * 8;
+    const int32_t a = sh.plan.ids[base + r];
+    if (a < 0) continue;
+    const uint32_t from = sums + (r * pitch + col) * 4;
+    float4 f[kMaxSplit], h[kMaxSplit];
+#pragma unroll
+    for (int p = 0; p < kMaxSplit; ++p) {
+      f[p] = p < split ? peer_float4(from, p) : float4{};
+      h[p] = p < split ? peer_float4(from + 16, p) : float4{};
+    }
+    float sum[8] = {};
+#pragma unroll
+    for (int p = 0; p < kMaxSplit; ++p) {
+      sum[0] += f[p].x; sum[1] += f[p].y; sum[2] += f[p].z; sum[3] += f[p].w;
+      sum[4] += h[p].x; sum[5] += h[p].y; sum[6] += h[p].z; sum[7] += h[p].w;
+    }
+    const float scale = sh.scale[r];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] *= scale;
+    const uint2 item = sh.plan.items[sh.item[r]];
+    uint8_t* low = g.low + (static_cast<int64_t>(tile) * g.most_blocks + (item.y >> 9)) *
+                               (g.rank * g.parts * 32);
+    put_low<T>(g, low, item.y & 31u, base + r - static_cast<int32_t>((item.y >> 5) & 15u) * kBlock,
+               col, sum);
+  }
+  fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "n"(2 * kWideRanks));
+  }
+  if (tid == 0 && sh.failed) atomicExch(&g_error, 1u);
 }
 
 // ---------------------------------------------------------------------------
@@ -1178,7 +1493,7 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g, split);
 }
 
-template <typename T, int GROUPS, int RS>
+template <typename T, int RS>
 cudaError_t launch_shrink_rank(const LoraArgs& g, int32_t turns, int32_t split, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(g.row_tiles * turns * split));
@@ -1200,42 +1515,70 @@ cudaError_t launch_shrink_rank(const LoraArgs& g, int32_t turns, int32_t split, 
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !ready[dev].load(std::memory_order_relaxed))) {
-    e = cudaFuncSetAttribute(shrink_kernel<T, GROUPS, RS>,
+    e = cudaFuncSetAttribute(shrink_kernel<T, RS>,
                              cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, shrink_kernel<T, GROUPS, RS>, g, turns, split);
+  return cudaLaunchKernelEx(&cfg, shrink_kernel<T, RS>, g, turns, split);
 }
 
-template <typename T, int GROUPS>
-cudaError_t launch_shrink_groups(const LoraArgs& g, int32_t turns, int32_t split, cudaStream_t st) {
-  return g.rank <= 16   ? launch_shrink_rank<T, GROUPS, 16>(g, turns, split, st)
-         : g.rank <= 32 ? launch_shrink_rank<T, GROUPS, 32>(g, turns, split, st)
-                        : launch_shrink_rank<T, GROUPS, 64>(g, turns, split, st);
+template <typename T>
+cudaError_t launch_shrink_wide(const LoraArgs& g, const CUtensorMap& amap, const CUtensorMap& xmap,
+                               cudaStream_t st) {
+  static std::atomic<bool> ready[64];
+  auto kernel = shrink_wide_kernel<T>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideBytes);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  const int32_t blocks = g.row_tiles * (g.tile / kWideRows), steps = (g.K + kStepK - 1) / kStepK;
+  int32_t split = 1;
+  while (split < kMaxSplit && blocks * split * 2 <= sm_count() && split * 8 <= steps) split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * split));
+  cfg.blockDim = dim3(kShrinkThreads);
+  cfg.dynamicSmemBytes = kWideBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = BPD_PDL ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, amap, xmap, g, split);
 }
 
 template <typename T>
 cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
   // A tile's items go round its CTAs in turn, 16 rows at a time: as many CTAs as
-  // that can come to where there is one tile, up to nine for each tile of a prompt, 32
-  // rows at a time. What is left of the SMs splits the inner elements.
-  const bool prompt = g.row_tiles > 1;
-  const int32_t turns = prompt ? std::max(1, std::min(9, sm_count() / g.row_tiles))
-                               : std::min(g.T, g.adapters + g.T / 16);
+  // that can come to. What is left of the SMs splits the inner elements.
+  const int32_t turns = std::min(sm_count() / g.row_tiles,
+                                 std::min(g.T, g.adapters + std::min(g.T, g.tile) / 16));
   int32_t split = 1;
   while (split < kMaxSplit && static_cast<int64_t>(g.row_tiles) * turns * split * 2 <= sm_count() &&
          split * 512 <= g.K)
     split *= 2;
-  return prompt ? launch_shrink_groups<T, 2>(g, turns, split, st)
-                : launch_shrink_groups<T, 1>(g, turns, split, st);
+  return g.rank <= 16   ? launch_shrink_rank<T, 16>(g, turns, split, st)
+         : g.rank <= 32 ? launch_shrink_rank<T, 32>(g, turns, split, st)
+                        : launch_shrink_rank<T, 64>(g, turns, split, st);
 }
 
 template <typename T, typename O>
-cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
+cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap,
+                           const CUtensorMap& amap, const CUtensorMap& xrows, const LoraArgs& g,
                            cudaStream_t st) {
-  cudaError_t e = g.ids ? launch_shrink<T>(g, st) : cudaSuccess;
+  cudaError_t e = !g.ids                       ? cudaSuccess
+                  : g.row_tiles > kGatherTiles ? launch_shrink_wide<T>(g, amap, xrows, st)
+                                               : launch_shrink<T>(g, st);
   if (e == cudaSuccess) {
     switch (g.tile) {
       case 16: e = launch_tile<T, O, 16, 1>(wmap, xmap, g, st); break;
@@ -1317,11 +1660,18 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   const int32_t pair = pair_of(nt, static_cast<int64_t>(row_tiles) * out_tiles, ids != nullptr);
   const EncodeFn encode = encoder();
   if (!encode) return fail(BPD_ERR_CUDA, "%s: the driver has no tensor maps", what);
-  CUtensorMap wmap, xmap;
+  CUtensorMap wmap, xmap, amap{}, xrows{};
   const bool bf16 = dtype == BPD_BF16;
   if (!matrix_map(&wmap, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
       !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, nt / pair))
     return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
+  if (ids && row_tiles > kGatherTiles) {
+    if (static_cast<int64_t>(num_adapters) * rank > INT_MAX)
+      return fail(BPD_ERR_CAPACITY, "%s: too many adapters", what);
+    if (!matrix_map(&amap, encode, a, bf16, num_adapters * rank, in_features, in_features, rank) ||
+        !matrix_map(&xrows, encode, x, bf16, rows, in_features, x_stride, kWideRows))
+      return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
+  }
   const Workspace w = workspace_of(rows, rank, num_adapters, fp32);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
@@ -1332,10 +1682,10 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (bf16)
-    e = out_dtype == BPD_F32 ? launch_project<__nv_bfloat16, float>(wmap, xmap, g, st)
-                             : launch_project<__nv_bfloat16, __nv_bfloat16>(wmap, xmap, g, st);
+    e = out_dtype == BPD_F32 ? launch_project<__nv_bfloat16, float>(wmap, xmap, amap, xrows, g, st)
+                             : launch_project<__nv_bfloat16, __nv_bfloat16>(wmap, xmap, amap, xrows, g, st);
   else
-    e = out_dtype == BPD_F32 ? launch_project<__half, float>(wmap, xmap, g, st)
-                             : launch_project<__half, __half>(wmap, xmap, g, st);
+    e = out_dtype == BPD_F32 ? launch_project<__half, float>(wmap, xmap, amap, xrows, g, st)
+                             : launch_project<__half, __half>(wmap, xmap, amap, xrows, g, st);
   return e == cudaSuccess ? BPD_OK : fail(BPD_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
