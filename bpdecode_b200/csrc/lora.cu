@@ -85,7 +85,8 @@ struct LoraArgs {
   int32_t* count;       // [row tiles]
   uint2* items;         // [row tiles, tile]: adapter; first block of S << 9 | first block << 5 | blocks
   uint8_t* low;         // [row tiles, most_blocks, rank * parts * 32 bytes]: S of the items' blocks
-  int32_t tile;         // rows of a tile
+  int32_t tile;         // rows that a tile has room for
+  int32_t step;         // rows of a tile: as many in each, in whole blocks
   int32_t most_blocks;  // of S, of a tile's items
   int32_t row_tiles, out_tiles;
   int32_t parts;        // 16-bit values that make up one of S
@@ -377,7 +378,7 @@ __device__ __forceinline__ int32_t plan_items(const LoraArgs& g, int32_t t0, Pla
                                               int32_t& own, uint32_t (&rows_in)[8]) {
   constexpr int kWarps = kShrinkThreads / 32;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  own = tid < g.tile ? adapter_of(g, t0 + tid) : -1;
+  own = tid < g.step ? adapter_of(g, t0 + tid) : -1;
   sh.ids[tid] = own;
   __syncthreads();
   // The first row of each adapter finds the adapter's items: runs of blocks
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t kpart = blockIdx.x % split;
   const int32_t turn = blockIdx.x / split % turns, tile = blockIdx.x / split / turns;
-  const int32_t t0 = tile * g.tile;
+  const int32_t t0 = tile * g.step;
   pdl_wait();
   pdl_trigger();  // what ran before has completed: x is there for the next kernel, too
   int32_t own;
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 1)
   const int32_t kpart = blockIdx.x % split, block = blockIdx.x / split;
   const int32_t halves = g.tile / kWideRows, tile = block / halves;
   const int32_t base = block % halves * kWideRows;  // of these rows in their tile
-  const int32_t t0 = tile * g.tile;
+  const int32_t t0 = tile * g.step;
   const int32_t steps = (g.K + kStepK - 1) / kStepK;
   const int32_t s0 = static_cast<int32_t>(static_cast<int64_t>(steps) * kpart / split);
   const int32_t s1 = static_cast<int32_t>(static_cast<int64_t>(steps) * (kpart + 1) / split);
@@ -1002,6 +1003,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = sh.tmem;
   bool ok = true;
+  // the rows that a tile has, in whole blocks
+  auto columns = [&](int32_t rows) {
+    return (min(g.step, g.T - rows * g.step) + PAIR * kBlock - 1) / (PAIR * kBlock) *
+           (PAIR * kBlock);
+  };
 
   if (warp == 0) {
     // --- loads ---------------------------------------------------------------
@@ -1031,13 +1037,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (PAIR == 1) {
             bar_expect(bar, S::kWeightBytes + NT * kStepK * 2);
             load_box(at, &wmap, s * kStepK, outs * kTileN, bar);
-            load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT, bar);
+            load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * g.step, bar);
           } else {
             const uint32_t of_both = in_cta(bar, 0);
             if (cta == 0) bar_expect(bar, 2 * S::kWeightBytes + NT * kStepK * 2);
             load_box_for(at, &wmap, s * kStepK, outs * kTileN, of_both);
-            load_box_for(at + S::kWeightBytes, &xmap, s * kStepK, rows * NT + cta * (NT / 2),
-                         of_both);
+            load_box_for(at + S::kWeightBytes, &xmap, s * kStepK,
+                         rows * g.step + cta * (columns(rows) / 2), of_both);
           }
         }
         next();
@@ -1200,6 +1206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = bar_wait_free<PAIR>(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
         fence_after();
         uint32_t d = tmem + buffer * NT;
+        const uint32_t wide = instruction<T, PAIR>(columns(tile % g.row_tiles));
         auto finish = [&] {
           mma_commit<PAIR>(shared_addr(&sh.empty[stage]));
           if (++stage == S::kStages) {
@@ -1222,7 +1229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t wd = desc_swizzled(at), xd = desc_swizzled(at + S::kWeightBytes);
 #pragma unroll
           for (int k = 0; k < kStepK / 16; ++k)
-            mma<PAIR>(d, wd + 2 * k, xd + 2 * k, instruction<T, PAIR>(NT),
+            mma<PAIR>(d, wd + 2 * k, xd + 2 * k, wide,
                       k > 0 || (kGroups ? (s - s0) % kGroup != 0 : s > s0));
           finish();
         }
@@ -1279,8 +1286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int32_t tile = first; tile < tiles && ok; tile += stride) {
       const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles * PAIR + cta;
       const int32_t n = outs * kTileN + quarter * 32 + lane;
-      OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
-      const int32_t have = min(NT, g.T - rows * NT);
+      OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
+      const int32_t have = min(g.step, g.T - rows * g.step);
       // 16 rows of the tile: for the cluster's sum, [row][output] in shared memory
       auto put = [&](int32_t c, const float (&v)[16]) {
         if (split > 1) {
@@ -1307,6 +1314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kGroups) {
 #pragma unroll
           for (int c = 0; c < NT; c += 16) {
+            if (c >= have) break;
             uint32_t v[16];
             tmem_load16(mine + buffer * NT + c, v);
 #pragma unroll
@@ -1315,7 +1323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   group == 0 ? __uint_as_float(v[i]) : sum[c / 16][i] + __uint_as_float(v[i]);
           }
         } else {
-          for (int c = 0; c < NT; c += 16) {
+          for (int c = 0; c < have; c += 16) {
             uint32_t v[16];
             tmem_load16(mine + buffer * NT + c, v);
 #pragma unroll
@@ -1336,7 +1344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (kGroups) {
         if (ok) {
 #pragma unroll
-          for (int c = 0; c < NT; c += 16) put(c, sum[c / 16]);
+          for (int c = 0; c < NT; c += 16)
+            if (c < have) put(c, sum[c / 16]);
         }
       }
     }
@@ -1347,9 +1356,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();
     // this CTA's share of the tile's rows, summed over the cluster in its order
     const int32_t rows = first % g.row_tiles, n = first / g.row_tiles * kTileN + lane * 4;
-    const int32_t have = min(NT, g.T - rows * NT);
+    const int32_t have = min(g.step, g.T - rows * g.step);
     using OBits = typename Dt<O>::Bits;
-    OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * NT * g.out_stride + n;
+    OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
     for (int32_t r = part + split * warp; r < have; r += split * (kThreads / 32)) {
       float4 v[kMaxSplit];
 #pragma unroll
@@ -1657,6 +1666,9 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   const int32_t row_tiles = (rows - 1) / nt + 1, out_tiles = (out_features - 1) / kTileN + 1;
   if (static_cast<int64_t>(row_tiles) * out_tiles > INT_MAX / 2)
     return fail(BPD_ERR_CAPACITY, "%s: too many tiles", what);
+  // (300 rows by 4096 x 65,536, 24 adapters, as 160 and 140: 208 us, as 256 and 44: 229)
+  const int32_t step =
+      row_tiles == 1 ? nt : (rows + row_tiles * 32 - 1) / (row_tiles * 32) * 32;
   const int32_t pair = pair_of(nt, static_cast<int64_t>(row_tiles) * out_tiles, ids != nullptr);
   const EncodeFn encode = encoder();
   if (!encode) return fail(BPD_ERR_CUDA, "%s: the driver has no tensor maps", what);
@@ -1677,7 +1689,8 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
-                   reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, w.most_blocks, row_tiles,
+                   reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, step, w.most_blocks,
+                   row_tiles,
                    out_tiles, fp32 && bf16 ? 3 : 2, pair};
   cudaStream_t st = as_stream(stream);
   cudaError_t e;

@@ -94,6 +94,11 @@ def test_mixes_of_adapters(kind, T) -> None:
 
 @pytest.mark.parametrize("dtype,out", [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
 @pytest.mark.parametrize("T,K,N,n,r,order", [
+    (129, 72, 19201, 3, 16, "mixed"), (140, 264, 19100, 20, 16, "runs"),
+    (165, 64, 19072, 9, 40, "mixed"), (215, 200, 19500, 43, 12, "runs"),
+    (256, 136, 20000, 24, 16, "mixed"), (257, 328, 9999, 30, 16, "runs"),
+    (300, 64, 9730, 6, 128, "mixed"), (321, 128, 9600, 40, 16, "runs"),
+    (700, 136, 6500, 50, 16, "mixed"), (1025, 200, 4000, 8, 64, "runs"),
     (33, 136, 9601, 5, 16, "mixed"), (50, 1608, 9733, 43, 12, "runs"),
     (64, 64, 9728, 1, 16, "all"), (65, 320, 10240, 70, 33, "mixed"),
     (100, 520, 19000, 9, 48, "runs"), (128, 8, 9610, 128, 8, "mixed"),
@@ -101,7 +106,7 @@ def test_mixes_of_adapters(kind, T) -> None:
     (290, 136, 6500, 300, 16, "mixed"), (600, 264, 4999, 8, 128, "runs"),
     (1030, 512, 2049, 11, 64, "runs")])
 def test_tiles_for_every_sm(dtype, out, T, K, N, n, r, order) -> None:
-    """More tiles than half of the SMs: two CTAs then share a tile's products."""
+    """More tiles than SMs, or nearly: large tiles' products are then shared by two CTAs."""
     from bpdecode_b200.adapters import project
 
     t = torch.arange(T)
@@ -111,6 +116,8 @@ def test_tiles_for_every_sm(dtype, out, T, K, N, n, r, order) -> None:
     got = project(c[0], c[1], bank, c[5], out_dtype=out)
     check(got, *c)
     assert torch.equal(got, project(c[0], c[1], bank, c[5], out_dtype=out))
+    alone = torch.full_like(c[5], -1)
+    check(project(c[0], c[1], out_dtype=out), *c[:5], alone)
 
 
 def test_no_bank_is_the_projection_alone() -> None:
