@@ -19,7 +19,7 @@
 // each; they need not be sorted. A matrix instruction over few rows costs
 // nearly what one over 128 costs (about 87 cycles at 16 rows), which is why
 // items are wide rather than exact: with 16-row items alone, 256 rows with 24
-// adapters took 226 us at 65,536 outputs, against 134 us without adapters.
+// adapters took 226 us at 65,536 outputs, against 161 so.
 //
 // Tiles of 256 rows are bound by what an SM loads, 48 KB for every 64 inner
 // elements. Two CTAs then work as a pair (cta_group::2): an instruction of the
@@ -83,7 +83,8 @@ struct LoraArgs {
   int64_t out_stride;
   // workspace: the items of each tile of rows
   int32_t* count;       // [row tiles]
-  uint2* items;         // [row tiles, tile]: adapter; first block of S << 9 | first block << 5 | blocks
+  uint2* items;         // [row tiles, tile]: adapter; first block of S << 9 | its first block << 5
+                        // | its blocks
   uint8_t* low;         // [row tiles, most_blocks, rank * parts * 32 bytes]: S of the items' blocks
   int32_t tile;         // rows that a tile has room for
   int32_t step;         // rows of a tile: as many in each, in whole blocks
@@ -946,8 +947,9 @@ struct ProjectShared {
 
 template <typename T, typename O, int NT, int PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
-    project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
-                   const LoraArgs g, const int32_t split) {
+    project_kernel(const __grid_constant__ CUtensorMap wmap,
+                   const __grid_constant__ CUtensorMap xmap, const LoraArgs g,
+                   const int32_t split) {
   using S = Shape<NT, PAIR>;
   static_assert(S::kStages <= kMaxStages &&
                     (PAIR == 2 || S::kStages * S::kStageBytes >= NT * kTileN * 4),
@@ -1122,7 +1124,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             op.idesc = instruction<T, PAIR>(0) | (blocks * (kBlock >> 3)) << 17;
             op.next = blocks * kBlock * 2 / PAIR;
           }
-          if (lane == 0) sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
+          if (lane == 0)
+            sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
           __syncwarp();
           const uint32_t bar = shared_addr(&sh.full[stage]);
           if (lane == 0) bar_expect(bar, units * rc * 32);
@@ -1238,7 +1241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (;;) {
             if (!(ok = bar_wait(shared_addr(&sh.full[stage]), phase))) break;
             if (PAIR == 2) {
-              ok = wait_for([&] { return bar_told(shared_addr(&sh.peer[stage]), told >> stage & 1u); });
+              ok = wait_for(
+                  [&] { return bar_told(shared_addr(&sh.peer[stage]), told >> stage & 1u); });
               if (!ok) break;
               told ^= 1u << stage;
             }
@@ -1286,7 +1290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int32_t tile = first; tile < tiles && ok; tile += stride) {
       const int32_t rows = tile % g.row_tiles, outs = tile / g.row_tiles * PAIR + cta;
       const int32_t n = outs * kTileN + quarter * 32 + lane;
-      OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
+      OBits* out =
+          static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
       const int32_t have = min(g.step, g.T - rows * g.step);
       // 16 rows of the tile: for the cluster's sum, [row][output] in shared memory
       auto put = [&](int32_t c, const float (&v)[16]) {
@@ -1358,7 +1363,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int32_t rows = first % g.row_tiles, n = first / g.row_tiles * kTileN + lane * 4;
     const int32_t have = min(g.step, g.T - rows * g.step);
     using OBits = typename Dt<O>::Bits;
-    OBits* out = static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
+    OBits* out =
+        static_cast<OBits*>(g.out) + static_cast<int64_t>(rows) * g.step * g.out_stride + n;
     for (int32_t r = part + split * warp; r < have; r += split * (kThreads / 32)) {
       float4 v[kMaxSplit];
 #pragma unroll
@@ -1485,8 +1491,8 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   while (PAIR == 1 && split < kMaxSplit && tiles * split * 2 <= sms && split * 2 <= steps)
     split *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(split > 1 ? tiles * split
-                                                     : std::min<int64_t>(tiles, sms / PAIR) * PAIR));
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      split > 1 ? tiles * split : std::min<int64_t>(tiles, sms / PAIR) * PAIR));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = st;
@@ -1693,12 +1699,12 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
                    row_tiles,
                    out_tiles, fp32 && bf16 ? 3 : 2, pair};
   cudaStream_t st = as_stream(stream);
-  cudaError_t e;
-  if (bf16)
-    e = out_dtype == BPD_F32 ? launch_project<__nv_bfloat16, float>(wmap, xmap, amap, xrows, g, st)
-                             : launch_project<__nv_bfloat16, __nv_bfloat16>(wmap, xmap, amap, xrows, g, st);
-  else
-    e = out_dtype == BPD_F32 ? launch_project<__half, float>(wmap, xmap, amap, xrows, g, st)
-                             : launch_project<__half, __half>(wmap, xmap, amap, xrows, g, st);
+  auto launch = [&](auto in, auto result) {
+    return launch_project<decltype(in), decltype(result)>(wmap, xmap, amap, xrows, g, st);
+  };
+  const cudaError_t e = bf16 ? fp32 ? launch(__nv_bfloat16{}, float{})
+                                    : launch(__nv_bfloat16{}, __nv_bfloat16{})
+                        : fp32 ? launch(__half{}, float{})
+                               : launch(__half{}, __half{});
   return e == cudaSuccess ? BPD_OK : fail(BPD_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }

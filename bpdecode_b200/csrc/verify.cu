@@ -43,7 +43,6 @@ constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
 constexpr int kMaxChunks = 32;  // of a row
 constexpr int kScanCtas = 5, kLastCtas = 4;  // on an SM
-constexpr int kScanBlocks = 1;  // blocks of a draft's row that a warp reads at once
 constexpr int kRaceVecs = 2;    // vectors of a race that a lane reads at once
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -133,7 +132,8 @@ __device__ __forceinline__ float warp_max(float v) {
 struct Allow {
   const uint32_t* row;  // NULL: see `any`
   bool any;
-  __device__ __forceinline__ Allow(const VerifyArgs& a, int32_t state) : row(nullptr), any(!a.allow_bits) {
+  __device__ __forceinline__ Allow(const VerifyArgs& a, int32_t state)
+      : row(nullptr), any(!a.allow_bits) {
     if (a.allow_bits && state >= 0 && state < a.num_states)
       row = a.allow_bits + static_cast<int64_t>(state) * a.words_stride;
   }
@@ -153,7 +153,8 @@ struct Row {
   __device__ Row(const VerifyArgs& a, int64_t row)
       : p(static_cast<const Bits*>(a.src) + row * a.src_stride) {
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-    head = min(a.vocab_size, static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
+    head = min(a.vocab_size,
+               static_cast<int32_t>((16u - off) & 15u) / static_cast<int32_t>(sizeof(Bits)));
     vecs = (a.vocab_size - head) / kEpv;
   }
   __device__ __forceinline__ float at(int64_t t) const { return Dt<T>::to_float(p[t]); }
@@ -416,7 +417,8 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
     const int64_t d = a.drafts_int64 ? static_cast<const int64_t*>(a.drafts)[at]
                                  : static_cast<const int32_t*>(a.drafts)[at];
     if (d >= 0 && d < a.vocab_size) p.draft = static_cast<int32_t>(d);
-    if (heat_of(a, b) > 0.0f) p.uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + lane];
+    if (heat_of(a, b) > 0.0f)
+      p.uniform = a.uniforms[static_cast<int64_t>(b) * a.uniform_stride + lane];
     if (a.probs && p.draft >= 0)
       p.qd = load_prob(a.probs, a.probs_dtype, (pfirst + lane) * a.probs_stride + p.draft);
   }
@@ -469,22 +471,22 @@ struct ScanShared {
 
 // Looks at four vectors of each lane, `word` their allow bits. kRace: with the
 // noise, two at a time for the registers' sake.
-template <typename T, bool RACE, int N>
-__device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, const uint32_t (&word)[N], float c,
+template <typename T, bool RACE>
+__device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_t word, float c,
                                            const float* noise, bool noise_fits, Scan& k,
                                            ScanShared& sh) {
   constexpr int kEpv = Row<T>::kEpv;
-  constexpr int kAtOnce = RACE ? kRaceVecs : 4 * N;
+  constexpr int kAtOnce = RACE ? kRaceVecs : 4;
   const int32_t lane0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
-  auto vec_of = [&](int q) { return lane0 + q / 4 * kScanWarps * 128 + q % 4 * 32; };
+  auto vec_of = [&](int q) { return lane0 + q * 32; };
 #pragma unroll
-  for (int q0 = 0; q0 < 4 * N; q0 += kAtOnce) {
+  for (int q0 = 0; q0 < 4; q0 += kAtOnce) {
     uint32_t keep[kAtOnce];
     uint4 v[kAtOnce];
     float e[RACE ? kAtOnce : 1][kEpv];
 #pragma unroll
     for (int q = 0; q < kAtOnce; ++q) {
-      keep[q] = Row<T>::keep(word[(q0 + q) / 4], (q0 + q) % 4);
+      keep[q] = Row<T>::keep(word, q0 + q);
       v[q] = uint4{};
       if (keep[q]) v[q] = row.vec(vec_of(q0 + q));
       if constexpr (RACE) {
@@ -500,10 +502,8 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, const u
     for (int q = 0; q < kAtOnce; ++q) v[q] = masked<T>(v[q], keep[q], sh.lanes);
     uint4 larger = v[0];
     if constexpr (kAtOnce == 2) larger = vec_max2<T>(v[0], v[1]);
-    if constexpr (kAtOnce >= 4)
+    if constexpr (kAtOnce == 4)
       larger = vec_max2<T>(vec_max2<T>(v[0], v[1]), vec_max2<T>(v[2], v[3]));
-    if constexpr (kAtOnce >= 8)
-      larger = vec_max2<T>(larger, vec_max2<T>(vec_max2<T>(v[4], v[5]), vec_max2<T>(v[6], v[7])));
     const float top = vec_top<T>(larger);
     if (top > k.m) {
       k.from = b;
@@ -612,43 +612,29 @@ __device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t 
   }
 }
 
-// Whether n blocks with `mine` allowed tokens in this lane's words allow few
-// tokens: an eighth.
+// Whether a block with this lane's word allows few tokens: an eighth.
 template <typename T>
-__device__ __forceinline__ bool few(uint32_t mine, int n) {
+__device__ __forceinline__ bool few(uint32_t word) {
   const uint32_t lane = threadIdx.x & 31;
-  return __reduce_add_sync(kFull, lane < 4 * Row<T>::kEpv ? mine : 0u) <=
-         static_cast<uint32_t>(n * 16 * Row<T>::kEpv);
+  return __reduce_add_sync(kFull, lane < 4 * Row<T>::kEpv ? __popc(word) : 0u) <=
+         16u * Row<T>::kEpv;
 }
 
-// Calls f(blocks, their allow bits) for this warp's blocks of a chunk, N at a
-// time, with the next ones' bits on their way (0 behind the last block).
-template <int N, typename T, typename F>
+// Calls f(block, its allow bits) for this warp's blocks of a chunk that allow
+// any token, with the bits of the next two on their way.
+template <typename T, typename F>
 __device__ __forceinline__ void each_block(const Row<T>& row, const Allow& ok, int32_t chunk,
                                            int32_t chunks, int32_t V, F&& f) {
   int32_t first, end;
   row.chunk(chunk, chunks, first, end);
   int32_t b = first + static_cast<int32_t>(threadIdx.x >> 5);
-  constexpr int kStride = N * kScanWarps;
-  auto bits = [&](int32_t at, uint32_t (&word)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      word[i] = at + i * kScanWarps < end ? row.bits(ok, at + i * kScanWarps, V) : 0u;
-  };
-  uint32_t word[N], next[N], behind[N];
-  bits(b, word);
-  bits(b + kStride, next);
-  for (; b < end; b += kStride) {
-    bits(b + 2 * kStride, behind);
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) any |= word[i];
-    if (__any_sync(kFull, any != 0)) f(b, word);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      word[i] = next[i];
-      next[i] = behind[i];
-    }
+  auto bits = [&](int32_t at) { return at < end ? row.bits(ok, at, V) : 0u; };
+  uint32_t word = bits(b), next = bits(b + kScanWarps);
+  for (; b < end; b += kScanWarps) {
+    const uint32_t behind = bits(b + 2 * kScanWarps);
+    if (__any_sync(kFull, word != 0)) f(b, word);
+    word = next;
+    next = behind;
   }
 }
 
@@ -664,20 +650,12 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
   const bool noise_fits =
       RACE && (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   Scan k;
-  constexpr int kBlocks = RACE ? 1 : kScanBlocks;
-  auto block = [&](int32_t b, const uint32_t (&word)[kBlocks]) {
-    uint32_t all = 0;
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i) all += __popc(word[i]);
-    if (few<T>(all, kBlocks)) {
-#pragma unroll
-      for (int i = 0; i < kBlocks; ++i)
-        scan_few<T, RACE>(row, b + i * kScanWarps, word[i], c, noise, k, sh);
-    } else {
-      scan_block<T, RACE, kBlocks>(row, b, word, c, noise, noise_fits, k, sh);
-    }
-  };
-  each_block<kBlocks>(row, ok, chunk, chunks, V, block);
+  each_block(row, ok, chunk, chunks, V, [&](int32_t b, uint32_t word) {
+    if (few<T>(word))
+      scan_few<T, RACE>(row, b, word, c, noise, k, sh);
+    else
+      scan_block<T, RACE>(row, b, word, c, noise, noise_fits, k, sh);
+  });
   row.edges(chunk, chunks, V, [&](int32_t t) {
     const float x = ok.has(t) ? fmaxf(row.at(t), -INFINITY) : -INFINITY;
     if (!(x > -INFINITY)) return;
@@ -709,9 +687,9 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
     for (; lanes; lanes &= lanes - 1) {
       const int32_t l = __ffs(lanes) - 1, from = __shfl_sync(kFull, k.from, l);
 #pragma unroll
-      for (int q0 = 0; q0 < 4 * kBlocks; q0 += 32 / kEpv) {
+      for (int q0 = 0; q0 < 4; q0 += 32 / kEpv) {
         const int32_t q = q0 + lane / kEpv;
-        const int32_t j = (from + q / 4 * kScanWarps) * 128 + q % 4 * 32 + l;
+        const int32_t j = from * 128 + q * 32 + l;
         const int32_t t = row.token(j) + lane % kEpv;
         if (j < row.vecs && ok.has(t) && row.at(t) == m) idx = min(idx, t);
       }
@@ -795,8 +773,8 @@ __global__ void __launch_bounds__(kScanThreads, kScanCtas)
   const float inv = greedy ? 1.0f : 1.0f / heat;
   Part* parts = w.part + (static_cast<int64_t>(b) * (K + 1) + i) * kMaxChunks;
   Part part;
-  if (scan_chunk<T, false>(Row<T>(a, first_row(a, b) + i), Allow(a, state), chunk, chunks, a.vocab_size, inv,
-                           greedy, nullptr, sh, part)) {
+  if (scan_chunk<T, false>(Row<T>(a, first_row(a, b) + i), Allow(a, state), chunk, chunks,
+                           a.vocab_size, inv, greedy, nullptr, sh, part)) {
     parts[chunk] = part;
     __threadfence();
     sh.last = atomicAdd(&pos.arrived, 1u) == static_cast<uint32_t>(chunks) - 1;
@@ -890,9 +868,9 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
       }
     }
   };
-  auto block = [&](int32_t b, const uint32_t (&word)[1]) {
-    if (few<T>(__popc(word[0]), 1)) {
-      few_of(b, word[0]);
+  auto block = [&](int32_t b, uint32_t word) {
+    if (few<T>(word)) {
+      few_of(b, word);
       return;
     }
     const int32_t j0 = b * 128 + static_cast<int32_t>(threadIdx.x & 31);
@@ -903,7 +881,7 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
       float e[kRaceVecs][kEpv], left[kRaceVecs][kEpv];
 #pragma unroll
       for (int q = 0; q < kRaceVecs; ++q) {
-        keep[q] = Row<T>::keep(word[0], q0 + q);
+        keep[q] = Row<T>::keep(word, q0 + q);
         const int32_t j = j0 + (q0 + q) * 32, t = row.token(j);
 #pragma unroll
         for (int i = 0; i < kEpv; ++i) left[q][i] = 0.0f;
@@ -936,7 +914,7 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
       }
     }
   };
-  each_block<1>(row, ok, chunk, chunks, V, block);
+  each_block(row, ok, chunk, chunks, V, block);
   if (idx >= 0) offer(idx);
   row.edges(chunk, chunks, V, offer);
   return block_max(won, sh.warps);

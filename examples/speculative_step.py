@@ -1,15 +1,16 @@
 """Requests that share a model and a grammar, each with its own adapter, decoded
 several tokens to a step.
 
-    python -m examples.speculative_step.py [--batch 64] [--drafts 4] [--temperature 0.8]
+    python -m examples.speculative_step [--batch 64] [--drafts 4] [--temperature 0.8]
         [--grammar email]
 
 The model is a table of hidden rows, one for each token, and a projection to
 the vocabulary with random weights. What the projection gives without the
 adapters drafts a few tokens for each request, the likeliest that the grammar
-allows; one projection with them scores all drafts; one ``verify_drafts`` keeps the ones that the model and the grammar
-agree to, adds a token, and commits. A request ends with its end-of-sequence
-token and then takes no part. Prints one line of JSON.
+allows; one projection with them scores all drafts; one ``verify_drafts`` keeps
+the ones that the model and the grammar agree to, adds a token, and commits. A
+request ends with its end-of-sequence token and then takes no part. Prints one
+line of JSON.
 """
 
 from __future__ import annotations
