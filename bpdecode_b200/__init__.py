@@ -12,6 +12,13 @@ Drop-in modules mirroring bpdecode's serving path:
 * :mod:`bpdecode_b200.hf` -- ``GrammarLogitsProcessor`` /
   ``RegexLogitsProcessor``.
 
+And, on either side of the constrained step:
+
+* :mod:`bpdecode_b200.adapters` -- ``AdapterBank`` and ``project``, a projection
+  with each row's own low-rank adapter;
+* :mod:`bpdecode_b200.speculative` -- ``verify_drafts``, drafted tokens verified
+  (or tokens sampled) under each request's grammar.
+
 All per-step work runs in hand-written CUDA kernels behind the C ABI of
 ``include/bpdecode_b200.h`` (``libbpdecode_b200.so``, built by
 ``python -m bpdecode_b200.build``).
