@@ -129,7 +129,8 @@ def project(
     int64 [rows]) names each row's slot of ``bank``, any id outside the bank
     (such as -1) none. The result [rows, out_features] is of ``x``'s type, or
     fp32 (``out_dtype``), rounded once from fp32 sums; ``out`` receives it
-    (contiguous columns, any row stride). Launches on torch's current stream
+    (contiguous columns, any row stride). In fp16, ``scaling * A x`` must stay
+    below 65504. Launches on torch's current stream
     without synchronising."""
     _require_cuda(x, "x")
     dtype, dev = x.dtype, x.device

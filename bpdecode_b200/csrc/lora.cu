@@ -1624,7 +1624,8 @@ extern "C" size_t bpd_lora_workspace_bytes(int32_t rows, int32_t rank, int32_t n
 extern "C" bpd_status bpd_lora_take_error(int32_t* error_out) {
   BPD_REQUIRE(error_out, "bpd_lora_take_error: null pointer");
   uint32_t v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_error, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();  // streams that do not wait for the default one, too
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_error, sizeof(v));
   const uint32_t zero = 0;
   if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_error, &zero, sizeof(zero));
   if (e != cudaSuccess) {
