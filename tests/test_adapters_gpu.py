@@ -231,3 +231,45 @@ def test_no_projection_gave_up_waiting() -> None:
     project(x, w, bank, torch.arange(33, device="cuda") % 3)
     check_device()
     check_device()
+
+
+@pytest.mark.parametrize("T,N,out", [(200, 19500, BF16), (800, 700, BF16), (800, 700, F32),
+                                     (1100, 9000, BF16)])
+def test_one_row_does_not_touch_another_in_large_tiles(T, N, out) -> None:
+    from bpdecode_b200.adapters import project
+
+    x, w, a, b, scale, ids = make(T, 200, N, 5, 40, BF16, seed=T)
+    bank = bank_of(a, b, scale)
+    bad_rows = [0, 31, 130, T - 1]
+    ids[torch.tensor(bad_rows, device="cuda")] = torch.tensor([1, 2, -1, 3], device="cuda")
+    clean = project(x, w, bank, ids, out_dtype=out)
+    bad = x.clone()
+    bad[0], bad[31, 5], bad[130], bad[T - 1, 7] = float("nan"), float("inf"), float("nan"), 3e38
+    got = project(bad, w, bank, ids, out_dtype=out)
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[bad_rows] = False
+    assert torch.equal(got[rest], clean[rest])
+    assert bool(torch.isnan(got[0]).all()) and bool(torch.isnan(got[130]).all())
+    assert not bool(torch.isfinite(got[31]).any())
+
+
+@pytest.mark.parametrize("T,N", [(3, 500), (200, 19500), (800, 700)])
+def test_captured_in_a_graph(T, N) -> None:
+    from bpdecode_b200.adapters import project
+
+    x, w, a, b, scale, ids = make(T, 136, N, 4, 16, F16, seed=T + 1)
+    bank = bank_of(a, b, scale)
+    out = torch.empty(T, N, dtype=F16, device="cuda")
+    project(x, w, bank, ids, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        project(x, w, bank, ids, out=out)
+    for seed in (5, 6):
+        y = make(T, 136, N, 4, 16, F16, seed=seed)
+        x.copy_(y[0])
+        ids.copy_(y[5])
+        want = project(x, w, bank, ids)
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)

@@ -197,3 +197,26 @@ def test_refusals() -> None:
             b.step_sample(i, src, noise.double())
         with pytest.raises(KeyError):
             b.verify_drafts(["nobody"], src, drafts, uniforms, noise)
+
+
+def test_dense_step_captured_in_a_graph() -> None:
+    batch, ids = _dense(20)
+    twin, _ = _dense(20)
+    ids = tuple(ids)
+    src, drafts, uniforms, noise = _rows(20, 3, batch._t.vocab_size, 11)
+    twin.verify_drafts(ids, src, drafts, uniforms, noise)  # loads the kernels
+    batch._slots(ids)  # the slots are on the device
+    twin.reset_many(ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = batch.verify_drafts(ids, src, drafts, uniforms, noise)
+    for step in range(4):
+        for t, new in zip((src, drafts, uniforms, noise),
+                          _rows(20, 3, batch._t.vocab_size, 20 + step)):
+            t.copy_(new)
+        graph.replay()
+        want = twin.verify_drafts(ids, src, drafts, uniforms, noise)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert torch.equal(batch._state, twin._state)
