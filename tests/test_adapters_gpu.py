@@ -120,6 +120,18 @@ def test_tiles_for_every_sm(dtype, out, T, K, N, n, r, order) -> None:
     check(project(c[0], c[1], out_dtype=out), *c[:5], alone)
 
 
+@pytest.mark.parametrize("T,K,N", [(1, 64, 19000), (16, 200, 38000), (64, 72, 60000),
+                                   (100, 136, 37889), (128, 520, 18945)])
+def test_one_two_and_more_tiles_for_an_sm(T, K, N) -> None:
+    from bpdecode_b200.adapters import project
+
+    c = make(T, K, N, 5, 24, BF16, seed=N)
+    bank = bank_of(*c[2:5])
+    for out in (BF16, F32):
+        got = project(c[0], c[1], bank, c[5], out_dtype=out)
+        check(got, *c)
+
+
 def test_no_bank_is_the_projection_alone() -> None:
     from bpdecode_b200.adapters import project
 
