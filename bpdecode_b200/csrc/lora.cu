@@ -1253,15 +1253,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             const int32_t rc = shape >> 8, n = shape & 255;
+            // One item after the other in a short loop: what this thread does between
+            // instructions shows (64 rows by 128,256 to fp32: 208 us, 217 with a
+            // branch for each half), and so does going from item to item for each
+            // part (24 adapters of rank 64, 256 rows by 65,536: 226 us, 260 to 490).
+            const int32_t halves = rc > 16 ? 2 : 1, count = g.parts * halves;
             for (int32_t i = 0; i < n; ++i) {
-              const Op op = sh.op[stage][i];
-              uint64_t low = op.low;
-              for (int32_t p = 0; p < g.parts; ++p, low += op.next) {
-                mma<PAIR>(d + op.to, op.b, low, op.idesc, true);
-                if (rc > 16) {
-                  low += op.next;
-                  mma<PAIR>(d + op.to, op.b + kTileN * 2, low, op.idesc, true);
-                }
+              Op op = sh.op[stage][i];
+              for (int32_t p = 0; p < count; ++p) {
+                mma<PAIR>(d + op.to, op.b + (p & (halves - 1)) * (kTileN * 2), op.low, op.idesc,
+                          true);
+                op.low += op.next;
               }
             }
             finish();
