@@ -25,8 +25,8 @@
 // elements. Two CTAs then work as a pair (cta_group::2): an instruction of the
 // first multiplies 256 outputs by 256 rows, each CTA has its own 128 outputs of
 // W and half of the rows of x, and both accumulate their outputs for all rows.
-// The first CTA's barriers count the loads of both; copies that only a CTA's own
-// barrier can count (the adapters') are told on by a thread of the second.
+// The first CTA's barriers count the loads of both, the adapters' too: all of them
+// are tensor copies, which alone may be counted in another CTA.
 //
 // S is held as the sum of 16-bit values, each the rounding of what those before
 // it left off: two of them keep 2^-17 of it in bf16 and 2^-22 in fp16 (one would
@@ -161,27 +161,6 @@ template <int PAIR>
 __device__ __forceinline__ bool bar_wait_free(uint32_t bar, uint32_t parity) {
   return wait_for(
       [&] { return PAIR == 2 ? bar_try_cluster(bar, parity) : bar_try(bar, parity); });
-}
-// Says to the first CTA that copies have landed here. Nothing but the copies is
-// passed on, and a barrier has said that they are in place, so this needs no
-// ordering of its own (as a release it took a microsecond for each step).
-__device__ __forceinline__ void bar_tell(uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .b32 a;\n\t"
-      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
-      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ bool bar_told(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 // The barrier at the same place in the cluster's CTA `rank`.
 __device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t rank) {
@@ -933,7 +912,7 @@ struct __align__(16) Op {
 };
 
 struct ProjectShared {
-  uint64_t full[kMaxStages], empty[kMaxStages], peer[kMaxStages], done[2], free[2], last;
+  uint64_t full[kMaxStages], empty[kMaxStages], done[2], free[2], last;
   uint32_t shape[kMaxStages];   // of an adapters' step: rank step << 8 | items; kEnd
   Op op[kMaxStages][kMaxItems];  // its items
   uint32_t tmem;
@@ -945,10 +924,21 @@ struct ProjectShared {
   uint16_t step[257];       // first item of each step
 };
 
+// What the product copies by tensor maps: W, x and, for a pair, B and S as rows
+// of kFlatRow bytes. A copy of B has min(kRankStep, rank) inner elements of a tile
+// of outputs, or 16 where some step has only that many; one of S has as many of
+// 2, 4, 8 or 16 blocks, half of which are this CTA's rows.
+constexpr int kFlatRow = 512;
+struct ProjectMaps {
+  CUtensorMap w, x, b, s[4];
+};
+__host__ __device__ constexpr int32_t flat_inner(int32_t rank) {
+  return rank % kRankStep ? 16 : kRankStep;
+}
+
 template <typename T, typename O, int NT, int PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
-    project_kernel(const __grid_constant__ CUtensorMap wmap,
-                   const __grid_constant__ CUtensorMap xmap, const LoraArgs g,
+    project_kernel(const __grid_constant__ ProjectMaps maps, const LoraArgs g,
                    const int32_t split) {
   using S = Shape<NT, PAIR>;
   static_assert(S::kStages <= kMaxStages &&
@@ -974,7 +964,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < S::kStages; ++i) {
       bar_init(shared_addr(&sh.full[i]), 1);
       bar_init(shared_addr(&sh.empty[i]), 1);
-      bar_init(shared_addr(&sh.peer[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(shared_addr(&sh.done[i]), 1);
@@ -1019,9 +1008,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     int32_t stage = 0;
     uint32_t phase = 0;
     int32_t issued = 0;
-    // copies that this CTA's own barriers count, where the first CTA's count the
-    // others: stages that had any, and how often (its last bit)
-    uint32_t own = 0, uses = 0;
     auto next = [&] {
       ++issued;
       if (++stage == S::kStages) {
@@ -1038,13 +1024,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t bar = shared_addr(&sh.full[stage]), at = ring + stage * S::kStageBytes;
           if constexpr (PAIR == 1) {
             bar_expect(bar, S::kWeightBytes + g.step * kStepK * 2);
-            load_box(at, &wmap, s * kStepK, outs * kTileN, bar);
-            load_box(at + S::kWeightBytes, &xmap, s * kStepK, rows * g.step, bar);
+            load_box(at, &maps.w, s * kStepK, outs * kTileN, bar);
+            load_box(at + S::kWeightBytes, &maps.x, s * kStepK, rows * g.step, bar);
           } else {
             const uint32_t of_both = in_cta(bar, 0);
             if (cta == 0) bar_expect(bar, 2 * S::kWeightBytes + g.step * kStepK * 2);
-            load_box_for(at, &wmap, s * kStepK, outs * kTileN, of_both);
-            load_box_for(at + S::kWeightBytes, &xmap, s * kStepK,
+            load_box_for(at, &maps.w, s * kStepK, outs * kTileN, of_both);
+            load_box_for(at + S::kWeightBytes, &maps.x, s * kStepK,
                          rows * g.step + cta * (columns(rows) / 2), of_both);
           }
         }
@@ -1115,47 +1101,65 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int o = kMaxItems / 2; o > 0; o >>= 1) units += __shfl_xor_sync(kFull, units, o);
           ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
           if (!ok) break;
-          if (lane < n) {
-            const uint32_t blocks = item & 31u;
-            Op& op = sh.op[stage][lane];
-            op.b = desc_plain(at + ((item >> 20) & 2047u) * rc * 32, kTileN * 16);
-            op.low = desc_plain(at + ((item >> 9) & 2047u) * rc * 32, blocks * kBlock * 16 / PAIR);
-            op.to = ((item >> 5) & 15u) * kBlock;
-            op.idesc = instruction<T, PAIR>(0) | (blocks * (kBlock >> 3)) << 17;
-            op.next = blocks * kBlock * 2 / PAIR;
-          }
-          if (lane == 0)
-            sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
-          __syncwarp();
+          const uint32_t blocks = item & 31u;
           const uint32_t bar = shared_addr(&sh.full[stage]);
-          if (lane == 0) bar_expect(bar, units * rc * 32);
+          if (cta == 0) {  // who gives the instructions
+            if (lane < n) {
+              Op& op = sh.op[stage][lane];
+              op.b = desc_plain(at + ((item >> 20) & 2047u) * rc * 32, kTileN * 16);
+              op.low =
+                  desc_plain(at + ((item >> 9) & 2047u) * rc * 32, blocks * kBlock * 16 / PAIR);
+              op.to = ((item >> 5) & 15u) * kBlock;
+              op.idesc = instruction<T, PAIR>(0) | (blocks * (kBlock >> 3)) << 17;
+              op.next = blocks * kBlock * 2 / PAIR;
+            }
+            if (lane == 0)
+              sh.shape[stage] = static_cast<uint32_t>(rc) << 8 | static_cast<uint32_t>(n);
+            __syncwarp();
+            if (lane == 0) bar_expect(bar, PAIR * units * rc * 32);
+          }
           __syncwarp();
           if (lane < n) {
-            if (load)
-              load_bulk(at + ((item >> 20) & 2047u) * rc * 32,
-                        static_cast<const uint8_t*>(g.b) +
-                            ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles +
-                              min(outs, g.out_tiles - 1)) * g.rank + c) * (kTileN * 2),
-                        rc * kTileN * 2, bar);
-            load_bulk(at + ((item >> 9) & 2047u) * rc * 32,
-                      g.low + (static_cast<int64_t>(rows) * g.most_blocks + sh.blocks[i0 + lane]) *
-                                  (g.rank * g.parts * 32) + wide * (cta * g.rank + c) * 32,
-                      wide * rc * 32, bar);
+            const uint32_t to_b = at + ((item >> 20) & 2047u) * rc * 32;
+            uint32_t to_s = at + ((item >> 9) & 2047u) * rc * 32;
+            // bytes from the start of B and of S
+            const int64_t from_b = ((static_cast<int64_t>(sh.adapter[i0 + lane]) * g.out_tiles +
+                                     min(outs, g.out_tiles - 1)) * g.rank + c) * (kTileN * 2);
+            const int64_t from_s =
+                (static_cast<int64_t>(rows) * g.most_blocks + sh.blocks[i0 + lane]) *
+                    (g.rank * g.parts * 32) + wide * (cta * g.rank + c) * 32;
+            if constexpr (PAIR == 1) {
+              if (load)
+                load_bulk(to_b, static_cast<const uint8_t*>(g.b) + from_b, rc * kTileN * 2, bar);
+              load_bulk(to_s, g.low + from_s, wide * rc * 32, bar);
+            } else {
+              const uint32_t of_both = in_cta(bar, 0);
+              const int32_t inner = flat_inner(g.rank);
+              int32_t row_b = static_cast<int32_t>(from_b / kFlatRow);
+              int32_t row_s = static_cast<int32_t>(from_s / kFlatRow);
+              for (int32_t k = 0; k < rc; k += inner) {
+                if (load) load_box_for(to_b + k * kTileN * 2, &maps.b, 0, row_b, of_both);
+                row_b += inner * kTileN * 2 / kFlatRow;
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                  if ((blocks >> (j + 1) & 1u) == 0) continue;
+                  load_box_for(to_s, &maps.s[j], 0, row_s, of_both);
+                  to_s += (inner * 64) << j;
+                  row_s += (inner * 64 / kFlatRow) << j;
+                }
+              }
+            }
           }
-          own |= 1u << stage;
-          uses ^= 1u << stage;
           next();
         }
       }
       if (ok) {
         ok = __all_sync(kFull, bar_wait(shared_addr(&sh.empty[stage]), phase ^ 1));
         if (ok) {
-          if (lane == 0) {
+          if (lane == 0 && cta == 0) {
             sh.shape[stage] = kEnd;
             bar_arrive(shared_addr(&sh.full[stage]));
           }
-          own |= 1u << stage;
-          uses ^= 1u << stage;
           next();
         }
       }
@@ -1177,34 +1181,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int32_t open = min(issued, S::kStages);
         for (int32_t i = issued - open; i < issued; ++i)
           bar_wait(shared_addr(&sh.full[i % S::kStages]), (i / S::kStages) & 1);
-      } else {
-        for (int i = 0; i < S::kStages; ++i)
-          if (own >> i & 1u) bar_wait(shared_addr(&sh.full[i]), (uses >> i & 1u) ^ 1u);
       }
     }
-  } else if (warp == 1 && cta == 1) {
-    // --- a pair's second CTA says which of its adapters' steps are loaded -----
-    if (lane == 0 && g.ids) {
-      int32_t stage = 0;
-      uint32_t uses = 0;
-      for (int32_t tile = first; tile < tiles && ok; tile += stride) {
-        stage = (stage + s1 - s0) % S::kStages;
-        for (bool end = false; !end;) {
-          if (!(ok = bar_wait(shared_addr(&sh.full[stage]), uses >> stage & 1u))) break;
-          uses ^= 1u << stage;
-          end = sh.shape[stage] == kEnd;
-          bar_tell(shared_addr(&sh.peer[stage]));
-          if (++stage == S::kStages) stage = 0;
-        }
-      }
-      if (!ok) sh.failed = 1;
-    }
-    __syncwarp();
   } else if (warp == 1) {
     // --- products ------------------------------------------------------------
-    if (lane == 0) {
+    if (lane == 0 && cta == 0) {
       int32_t stage = 0, buffer = 0;
-      uint32_t phase = 0, turn = 0, told = 0;
+      uint32_t phase = 0, turn = 0;
       for (int32_t tile = first; tile < tiles && ok; tile += stride) {
         if (!(ok = bar_wait_free<PAIR>(shared_addr(&sh.free[buffer]), turn ^ 1))) break;
         fence_after();
@@ -1240,12 +1223,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (g.ids) {
           for (;;) {
             if (!(ok = bar_wait(shared_addr(&sh.full[stage]), phase))) break;
-            if (PAIR == 2) {
-              ok = wait_for(
-                  [&] { return bar_told(shared_addr(&sh.peer[stage]), told >> stage & 1u); });
-              if (!ok) break;
-              told ^= 1u << stage;
-            }
             fence_after();
             const uint32_t shape = sh.shape[stage];
             if (shape == kEnd) {
@@ -1436,6 +1413,17 @@ bool matrix_map(CUtensorMap* map, EncodeFn encode, const void* base, bool bf16, 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// `rows` rows of kFlatRow bytes each, in boxes of `box` of them.
+bool flat_map(CUtensorMap* map, EncodeFn encode, const void* base, int64_t rows, int32_t box) {
+  const cuuint64_t dims[2] = {kFlatRow / 2, static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {kFlatRow};
+  const cuuint32_t boxes[2] = {kFlatRow / 2, static_cast<cuuint32_t>(box)}, unit[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides,
+                boxes, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Rows of x of a tile: all of them where that is one tile, W is then read once.
 // (An fp32 result keeps its sums in registers, which hold 128.)
 int32_t row_tile(int32_t rows, bool fp32) {
@@ -1471,8 +1459,7 @@ Workspace workspace_of(int32_t rows, int32_t rank, int32_t adapters, bool fp32) 
 }
 
 template <typename T, typename O, int NT, int PAIR>
-cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const LoraArgs& g,
-                        cudaStream_t st) {
+cudaError_t launch_tile(const ProjectMaps& maps, const LoraArgs& g, cudaStream_t st) {
   static std::atomic<bool> ready[64];
   using S = Shape<NT, PAIR>;
   auto kernel = project_kernel<T, O, NT, PAIR>;
@@ -1507,7 +1494,7 @@ cudaError_t launch_tile(const CUtensorMap& wmap, const CUtensorMap& xmap, const 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split * PAIR > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, g, split);
+  return cudaLaunchKernelEx(&cfg, kernel, maps, g, split);
 }
 
 template <typename T, int RS>
@@ -1590,22 +1577,21 @@ cudaError_t launch_shrink(const LoraArgs& g, cudaStream_t st) {
 }
 
 template <typename T, typename O>
-cudaError_t launch_project(const CUtensorMap& wmap, const CUtensorMap& xmap,
-                           const CUtensorMap& amap, const CUtensorMap& xrows, const LoraArgs& g,
-                           cudaStream_t st) {
+cudaError_t launch_project(const ProjectMaps& maps, const CUtensorMap& amap,
+                           const CUtensorMap& xrows, const LoraArgs& g, cudaStream_t st) {
   cudaError_t e = !g.ids                       ? cudaSuccess
                   : g.row_tiles > kGatherTiles ? launch_shrink_wide<T>(g, amap, xrows, st)
                                                : launch_shrink<T>(g, st);
   if (e == cudaSuccess) {
     switch (g.tile) {
-      case 16: e = launch_tile<T, O, 16, 1>(wmap, xmap, g, st); break;
-      case 32: e = launch_tile<T, O, 32, 1>(wmap, xmap, g, st); break;
-      case 64: e = launch_tile<T, O, 64, 1>(wmap, xmap, g, st); break;
-      case 128: e = launch_tile<T, O, 128, 1>(wmap, xmap, g, st); break;
+      case 16: e = launch_tile<T, O, 16, 1>(maps, g, st); break;
+      case 32: e = launch_tile<T, O, 32, 1>(maps, g, st); break;
+      case 64: e = launch_tile<T, O, 64, 1>(maps, g, st); break;
+      case 128: e = launch_tile<T, O, 128, 1>(maps, g, st); break;
       default:  // an fp32 result has tiles of up to 128 rows
         if constexpr (!std::is_same_v<O, float>)
-          e = g.pair == 2 ? launch_tile<T, O, 256, 2>(wmap, xmap, g, st)
-                          : launch_tile<T, O, 256, 1>(wmap, xmap, g, st);
+          e = g.pair == 2 ? launch_tile<T, O, 256, 2>(maps, g, st)
+                          : launch_tile<T, O, 256, 1>(maps, g, st);
     }
   }
   if (e != cudaSuccess) (void)cudaGetLastError();
@@ -1679,13 +1665,23 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
   // adapters take 196 us as 160 and 140 rows, 198 where 256 are loaded for each, and
   // 229 as 256 and 44.
   const int32_t step = std::min(nt, (rows + row_tiles * 32 - 1) / (row_tiles * 32) * 32);
-  const int32_t pair = pair_of(nt, static_cast<int64_t>(row_tiles) * out_tiles, ids != nullptr);
+  const Workspace w = workspace_of(rows, rank, num_adapters, fp32);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int32_t parts = fp32 && dtype == BPD_BF16 ? 3 : 2;
+  int32_t pair = pair_of(nt, static_cast<int64_t>(row_tiles) * out_tiles, ids != nullptr);
+  // rows of B and of S as a pair copies them
+  const int64_t flat_b = static_cast<int64_t>(num_adapters) * out_tiles * rank * (kTileN * 2) /
+                         kFlatRow;
+  const int64_t flat_s = static_cast<int64_t>(row_tiles) * w.most_blocks * rank * parts * 32 /
+                         kFlatRow;
+  if (ids && std::max(flat_b, flat_s) > INT_MAX) pair = 1;
   const EncodeFn encode = encoder();
   if (!encode) return fail(BPD_ERR_CUDA, "%s: the driver has no tensor maps", what);
-  CUtensorMap wmap, xmap, amap{}, xrows{};
+  ProjectMaps maps{};
+  CUtensorMap amap{}, xrows{};
   const bool bf16 = dtype == BPD_BF16;
-  if (!matrix_map(&wmap, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
-      !matrix_map(&xmap, encode, x, bf16, rows, in_features, x_stride, step / pair))
+  if (!matrix_map(&maps.w, encode, weight, bf16, out_features, in_features, weight_stride, kTileN) ||
+      !matrix_map(&maps.x, encode, x, bf16, rows, in_features, x_stride, step / pair))
     return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
   if (ids && row_tiles > kGatherTiles) {
     if (static_cast<int64_t>(num_adapters) * rank > INT_MAX)
@@ -1694,17 +1690,22 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
         !matrix_map(&xrows, encode, x, bf16, rows, in_features, x_stride, kWideRows))
       return fail(BPD_ERR_INVALID, "%s: strides too large for a tensor map", what);
   }
-  const Workspace w = workspace_of(rows, rank, num_adapters, fp32);
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (ids && pair == 2) {
+    const int32_t inner = flat_inner(rank);
+    bool made = flat_map(&maps.b, encode, b, flat_b, inner * kTileN * 2 / kFlatRow);
+    for (int j = 0; j < 4; ++j)
+      made = made && flat_map(&maps.s[j], encode, ws + w.low, flat_s, (inner * 64 / kFlatRow) << j);
+    if (!made) return fail(BPD_ERR_INVALID, "%s: adapters too large for a tensor map", what);
+  }
   const LoraArgs g{x, x_stride, rows, in_features, out_features, a, b, scale, num_adapters, rank,
                    ids, ids_int64, out, out_stride,
                    reinterpret_cast<int32_t*>(ws + w.count),
                    reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, step, w.most_blocks,
                    row_tiles,
-                   out_tiles, fp32 && bf16 ? 3 : 2, pair};
+                   out_tiles, parts, pair};
   cudaStream_t st = as_stream(stream);
   auto launch = [&](auto in, auto result) {
-    return launch_project<decltype(in), decltype(result)>(wmap, xmap, amap, xrows, g, st);
+    return launch_project<decltype(in), decltype(result)>(maps, amap, xrows, g, st);
   };
   const cudaError_t e = bf16 ? fp32 ? launch(__nv_bfloat16{}, float{})
                                     : launch(__nv_bfloat16{}, __nv_bfloat16{})
