@@ -352,9 +352,27 @@ __device__ __forceinline__ float vec_top(const uint4& v) {
 // with a bar of its own some lane of a warp nearly always has a new best to
 // look at. A score has to be over the bar less this much to be looked at, more
 // than all roundings between them, so the winner always is, whatever the order
-// in which the bar rises.
-constexpr float kSlack = 1.0f - 3.0e-5f;
+// in which the bar rises. (Scores whose weights are exp2 of up to 128 in magnitude,
+// from arguments, logarithms and differences rounded to 2^-24 of that: 4e-5.)
+constexpr float kSlack = 1.0f - 1.0f / 8192;
 constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is still compared
+
+// The bar of a race that is run along with the scan: log2 of a score, `over` the
+// reference `ref` of the thread that found it (see Scan). The two are kept apart,
+// since at low temperatures, or with large logits, fp32 has no room in a
+// reference for the scores over it: at a logit of 20 and T = 1e-6 its unit is 2.
+struct Lead {
+  float ref, over;
+  __device__ __forceinline__ static Lead of(uint64_t v) {
+    return {__uint_as_float(static_cast<uint32_t>(v >> 32)),
+            __uint_as_float(static_cast<uint32_t>(v))};
+  }
+  __device__ __forceinline__ uint64_t bits() const {
+    return uint64_t(__float_as_uint(ref)) << 32 | __float_as_uint(over);
+  }
+  // as a score over another reference
+  __device__ __forceinline__ float from(float base) const { return (ref - base) + over; }
+};
 
 __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
   return pack_arg(__float_as_uint(score > 0.0f ? score : 0.0f), t);
@@ -442,19 +460,25 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
 // What a thread keeps of a row that it scans: the maximum m and the sum of
 // exp2(x c - ref) with c = log2(e) / T. ref is not the maximum but some value
 // within kReach of it (of the logits), so that it hardly ever changes; a term
-// is one multiply-add, one exponential and one addition.
+// is one multiply-add, one exponential and one addition. x c - ref is rounded once
+// however large the two are, so ref may be any number near them. A score over a
+// ref that is too large to be near them is let go with it: the tokens there are
+// nothing beside the one that raises ref.
+constexpr float kMostRef = 1 << 29;  // its unit is 64
+
 struct Scan {
   static constexpr float kReach = 16.0f;
   float m = -INFINITY, ref = 0.0f, limit = -INFINITY, s = 0.0f;
   int32_t from = -1;         // the block whose vectors have m (-1: see idx)
   int32_t idx = INT_MAX;     // the first token that has m
-  float score = -INFINITY;   // the race: log2 of this thread's best
+  float score = -INFINITY;   // the race: log2 of this thread's best, less ref
   float bar = 0.0f;          // what it has to pass, times -1
   int32_t best = -1;
   __device__ __forceinline__ void raise(float top, float c) {
     if (top > limit) {  // the first value, or one far above it
       const float to = top * c;
       s *= limit > -INFINITY ? exp2_fast(ref - to) : 0.0f;
+      score = fabsf(ref) < kMostRef ? score + (ref - to) : -INFINITY;
       ref = to;
       limit = top + kReach * fminf(1.0f / c, 3.0e38f);
     }
@@ -464,9 +488,21 @@ struct Scan {
 struct ScanShared {
   Lanes lanes;
   uint64_t warps[kScanWarps];
+  unsigned long long lead;  // of a scan's race: a Lead
   float sums[kScanWarps];
-  uint32_t bar;
+  uint32_t bar;             // of a race by itself: a score
   int32_t last;
+  __device__ __forceinline__ float bar_over(float ref) const {
+    return exp2_fast(Lead::of(*const_cast<const volatile unsigned long long*>(&lead)).from(ref));
+  }
+  // Raises the bar to this thread's best. Where another thread comes first the bar
+  // stays as that one left it, which only has more scores looked at (trying again,
+  // or a warp's best alone, took as long or up to 4 us more of 118).
+  __device__ __forceinline__ void offer(const Scan& k) {
+    const Lead mine{k.ref, fminf(k.score, __log2f(kMostScore))};
+    unsigned long long seen = *const_cast<volatile unsigned long long*>(&lead);
+    if (mine.from(Lead::of(seen).ref) > Lead::of(seen).over) atomicCAS(&lead, seen, mine.bits());
+  }
 };
 
 // Looks at four vectors of each lane, `word` their allow bits. kRace: with the
@@ -511,8 +547,7 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
       k.m = top;
     }
     k.raise(top, c);
-    if constexpr (RACE)
-      k.bar = exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - k.ref) * -kSlack;
+    if constexpr (RACE) k.bar = sh.bar_over(k.ref) * -kSlack;
     // ref is 0 as long as there is nothing but -inf: weights of 0
     const Pair c2 = pair_of(c, c), low = pair_of(-k.ref, -k.ref);
     const Pair bar2 = pair_of(k.bar, k.bar);
@@ -545,14 +580,13 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
         for (int q = 0; q < kAtOnce; ++q)
 #pragma unroll
           for (int i = 0; i < kEpv; ++i) {
-            const float f = __log2f(w[q][i]) + k.ref - __log2f(e[q][i]);
+            const float f = __log2f(w[q][i]) - __log2f(e[q][i]);
             if (f > k.score && w[q][i] > 0.0f) {
               k.score = f;
               k.best = row.token(vec_of(q0 + q)) + i;
             }
           }
-        const float rise = fminf(k.score, k.ref + __log2f(kMostScore));
-        if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+        sh.offer(k);
       }
     }
   }
@@ -588,8 +622,7 @@ __device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t 
         if (x[u] == top) k.idx = t[u];
     }
     k.raise(top, c);
-    const float bar =
-        RACE ? exp2_fast(key_value(*const_cast<volatile uint32_t*>(&sh.bar)) - k.ref) * kSlack : 0;
+    const float bar = RACE ? sh.bar_over(k.ref) * kSlack : 0.0f;
     float over = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -600,14 +633,13 @@ __device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t 
     if (RACE && over > 0.0f) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float f = __log2f(x[u]) + k.ref - __log2f(e[u]);
+        const float f = __log2f(x[u]) - __log2f(e[u]);
         if (f > k.score && x[u] > 0.0f) {
           k.score = f;
           k.best = t[u];
         }
       }
-      const float rise = fminf(k.score, k.ref + __log2f(kMostScore));
-      if (rise > -INFINITY) atomicMax(&sh.bar, order_key(rise));
+      sh.offer(k);
     }
   }
 }
@@ -669,7 +701,7 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
     }
     const float f = exp2_fast(fmaf(x, c, -k.ref));
     k.s += f;
-    if (RACE && __log2f(f) + k.ref - __log2f(noise[t]) > k.score) k.best = t;
+    if (RACE && __log2f(f) - __log2f(noise[t]) > k.score) k.best = t;
   });
   // the chunk's maximum, and where it is first
   float m = warp_max(k.m);
@@ -929,7 +961,7 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
   const int32_t b = static_cast<int32_t>(blockIdx.x / chunks);
   const int32_t tid = threadIdx.x, lane = tid & 31, K = a.max_drafts, V = a.vocab_size;
   if (sizeof(typename Dt<T>::Bits) == 2) sh.lanes.fill();
-  if (tid == 0) sh.bar = order_key(-INFINITY);
+  if (tid == 0) sh.lead = Lead{0.0f, -INFINITY}.bits();
   pdl_trigger();
   pdl_wait();
   Request& request = w.request[b];
