@@ -32,6 +32,7 @@
 // fast arithmetic. Nothing depends on the order in which CTAs run: chunks meet
 // in a fixed order, and a race takes the maximum of (score, lowest index).
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "common.cuh"
@@ -109,6 +110,11 @@ __device__ __forceinline__ void split(const Pair& p, float& lo, float& hi) {
 __device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
   Pair d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
 __device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
@@ -357,10 +363,10 @@ __device__ __forceinline__ float vec_top(const uint4& v) {
 constexpr float kSlack = 1.0f - 1.0f / 8192;
 constexpr float kMostScore = 1.0e30f;  // a bar is no higher: noise near 0 is still compared
 
-// The bar of a race that is run along with the scan: log2 of a score, `over` the
-// reference `ref` of the thread that found it (see Scan). The two are kept apart,
-// since at low temperatures, or with large logits, fp32 has no room in a
-// reference for the scores over it: at a logit of 20 and T = 1e-6 its unit is 2.
+// The bar of a race that is run along with the scan: log2 of a score, `over` that of
+// a token at the reference `ref` of the thread that found it (see Scan). The two
+// are kept apart, since at low temperatures, or with large logits, fp32 has no
+// room in ref c for the scores over it: at a logit of 20 and T = 1e-6 its unit is 2.
 struct Lead {
   float ref, over;
   __device__ __forceinline__ static Lead of(uint64_t v) {
@@ -370,8 +376,10 @@ struct Lead {
   __device__ __forceinline__ uint64_t bits() const {
     return uint64_t(__float_as_uint(ref)) << 32 | __float_as_uint(over);
   }
-  // as a score over another reference
-  __device__ __forceinline__ float from(float base) const { return (ref - base) + over; }
+  // over another reference
+  __device__ __forceinline__ float from(float base, float c) const {
+    return fmaf(ref - base, c, over);
+  }
 };
 
 __device__ __forceinline__ uint64_t race_key(float score, int32_t t) {
@@ -458,14 +466,12 @@ __global__ void __launch_bounds__(128) walk_kernel(const VerifyArgs a, const Wor
 
 // ---------------------------------------------------------------------------
 // What a thread keeps of a row that it scans: the maximum m and the sum of
-// exp2(x c - ref) with c = log2(e) / T. ref is not the maximum but some value
-// within kReach of it (of the logits), so that it hardly ever changes; a term
-// is one multiply-add, one exponential and one addition. x c - ref is rounded once
-// however large the two are, so ref may be any number near them. A score over a
-// ref that is too large to be near them is let go with it: the tokens there are
-// nothing beside the one that raises ref.
-constexpr float kMostRef = 1 << 29;  // its unit is 64
-
+// exp2((x - ref) c) with c = log2(e) / T. ref is not the maximum but some logit
+// within kReach of it, so that it hardly ever changes. The difference comes first:
+// ref c leaves the range of fp32 for logits like its lowest value and for the
+// lowest temperatures, and above 2^29 is rounded by more than an exponential can
+// take. (As x c - ref c, one multiply-add, 256 x 3 rows in fp32 took 118 us for
+// 121 so, rows in 16 bits the same.)
 struct Scan {
   static constexpr float kReach = 16.0f;
   float m = -INFINITY, ref = 0.0f, limit = -INFINITY, s = 0.0f;
@@ -476,10 +482,10 @@ struct Scan {
   int32_t best = -1;
   __device__ __forceinline__ void raise(float top, float c) {
     if (top > limit) {  // the first value, or one far above it
-      const float to = top * c;
-      s *= limit > -INFINITY ? exp2_fast(ref - to) : 0.0f;
-      score = fabsf(ref) < kMostRef ? score + (ref - to) : -INFINITY;
-      ref = to;
+      const float by = (ref - top) * c;
+      s *= limit > -INFINITY ? exp2_fast(by) : 0.0f;
+      score = limit > -INFINITY ? score + by : score;
+      ref = top;
       limit = top + kReach * fminf(1.0f / c, 3.0e38f);
     }
   }
@@ -492,16 +498,17 @@ struct ScanShared {
   float sums[kScanWarps];
   uint32_t bar;             // of a race by itself: a score
   int32_t last;
-  __device__ __forceinline__ float bar_over(float ref) const {
-    return exp2_fast(Lead::of(*const_cast<const volatile unsigned long long*>(&lead)).from(ref));
+  __device__ __forceinline__ float bar_over(float ref, float c) const {
+    return exp2_fast(
+        Lead::of(*const_cast<const volatile unsigned long long*>(&lead)).from(ref, c));
   }
   // Raises the bar to this thread's best. Where another thread comes first the bar
   // stays as that one left it, which only has more scores looked at (trying again,
   // or a warp's best alone, took as long or up to 4 us more of 118).
-  __device__ __forceinline__ void offer(const Scan& k) {
+  __device__ __forceinline__ void offer(const Scan& k, float c) {
     const Lead mine{k.ref, fminf(k.score, __log2f(kMostScore))};
     unsigned long long seen = *const_cast<volatile unsigned long long*>(&lead);
-    if (mine.from(Lead::of(seen).ref) > Lead::of(seen).over) atomicCAS(&lead, seen, mine.bits());
+    if (mine.from(Lead::of(seen).ref, c) > Lead::of(seen).over) atomicCAS(&lead, seen, mine.bits());
   }
 };
 
@@ -547,7 +554,7 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
       k.m = top;
     }
     k.raise(top, c);
-    if constexpr (RACE) k.bar = sh.bar_over(k.ref) * -kSlack;
+    if constexpr (RACE) k.bar = sh.bar_over(k.ref, c) * -kSlack;
     // ref is 0 as long as there is nothing but -inf: weights of 0
     const Pair c2 = pair_of(c, c), low = pair_of(-k.ref, -k.ref);
     const Pair bar2 = pair_of(k.bar, k.bar);
@@ -558,8 +565,8 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
 #pragma unroll
       for (int i = 0; i < kEpv; i += 2) {
         float lo, hi;
-        split(fma2(pair_of(Dt<T>::to_float(vec_get<T>(v[q], i)),
-                           Dt<T>::to_float(vec_get<T>(v[q], i + 1))), c2, low), lo, hi);
+        split(mul2(add2(pair_of(Dt<T>::to_float(vec_get<T>(v[q], i)),
+                                Dt<T>::to_float(vec_get<T>(v[q], i + 1))), low), c2), lo, hi);
         lo = exp2_fast(lo);
         hi = exp2_fast(hi);
         const Pair both = pair_of(lo, hi);
@@ -586,7 +593,7 @@ __device__ __forceinline__ void scan_block(const Row<T>& row, int32_t b, uint32_
               k.best = row.token(vec_of(q0 + q)) + i;
             }
           }
-        sh.offer(k);
+        sh.offer(k, c);
       }
     }
   }
@@ -622,11 +629,11 @@ __device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t 
         if (x[u] == top) k.idx = t[u];
     }
     k.raise(top, c);
-    const float bar = RACE ? sh.bar_over(k.ref) * kSlack : 0.0f;
+    const float bar = RACE ? sh.bar_over(k.ref, c) * kSlack : 0.0f;
     float over = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      x[u] = exp2_fast(fmaf(x[u], c, -k.ref));
+      x[u] = exp2_fast((x[u] - k.ref) * c);
       if (RACE) over = fmaxf(over, fmaf(-bar, e[u], x[u]));
     }
     k.s += (x[0] + x[1]) + (x[2] + x[3]);
@@ -639,7 +646,7 @@ __device__ __forceinline__ void scan_few(const Row<T>& row, int32_t b, uint32_t 
           k.best = t[u];
         }
       }
-      sh.offer(k);
+      sh.offer(k, c);
     }
   }
 }
@@ -699,7 +706,7 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
     } else if (x == k.m) {
       k.idx = k.from < 0 ? min(k.idx, t) : t;
     }
-    const float f = exp2_fast(fmaf(x, c, -k.ref));
+    const float f = exp2_fast((x - k.ref) * c);
     k.s += f;
     if (RACE && __log2f(f) - __log2f(noise[t]) > k.score) k.best = t;
   });
@@ -737,7 +744,7 @@ __device__ __forceinline__ bool scan_chunk(const Row<T>& row, const Allow& ok, i
   }
   const uint64_t mine = won;
   won = block_max(won, sh.warps);
-  float s = warp_sum(k.m > -INFINITY ? k.s * exp2_fast(fmaf(-m, c, k.ref)) : 0.0f);
+  float s = warp_sum(k.m > -INFINITY ? k.s * exp2_fast((k.ref - m) * c) : 0.0f);
   if (lane == 0) sh.sums[warp] = s;
   __syncthreads();
   s = warp_sum(lane < kScanWarps ? sh.sums[lane] : 0.0f);
@@ -858,7 +865,6 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
   }
   float top = -1.0f;
   int32_t idx = -1;
-  const float ref = m * c, fix = exp2_fast(-fmaf(m, c, -ref)) * rz;
   const bool noise_fits = (reinterpret_cast<uintptr_t>(noise + row.head) & 15u) == 0;
   const bool given_fits = given.p && given.template fits<kEpv>(row.head);
   auto look = [&](float left, float e, int32_t t) {
@@ -890,7 +896,7 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
       const float bar = __uint_as_float(*const_cast<volatile uint32_t*>(&sh.bar)) * kSlack;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        x[u] = fmaf(exp2_fast(fmaf(x[u], c, -ref)), fix, -q[u]);
+        x[u] = fmaf(exp2_fast((x[u] - m) * c), rz, -q[u]);
         over = fmaxf(over, fmaf(-bar, e[u], x[u]));
       }
       if (over > 0.0f) {
@@ -933,8 +939,8 @@ __device__ __forceinline__ uint64_t race_chunk(const Row<T>& row, const Allow& o
         float over = 0.0f;
 #pragma unroll
         for (int i = 0; i < kEpv; ++i) {
-          const float f = exp2_fast(fmaf(Dt<T>::to_float(vec_get<T>(x, i)), c, -ref));
-          left[q][i] = fmaf(f, fix, -left[q][i]);
+          const float f = exp2_fast((Dt<T>::to_float(vec_get<T>(x, i)) - m) * c);
+          left[q][i] = fmaf(f, rz, -left[q][i]);
           over = fmaxf(over, (keep[q] >> i) & 1u ? fmaf(-bar, e[q][i], left[q][i]) : 0.0f);
         }
         if (over > 0.0f) {
@@ -961,7 +967,7 @@ __global__ void __launch_bounds__(kScanThreads, kLastCtas)
   const int32_t b = static_cast<int32_t>(blockIdx.x / chunks);
   const int32_t tid = threadIdx.x, lane = tid & 31, K = a.max_drafts, V = a.vocab_size;
   if (sizeof(typename Dt<T>::Bits) == 2) sh.lanes.fill();
-  if (tid == 0) sh.lead = Lead{0.0f, -INFINITY}.bits();
+  if (tid == 0) sh.lead = Lead{-FLT_MAX, -INFINITY}.bits();  // below any score
   pdl_trigger();
   pdl_wait();
   Request& request = w.request[b];

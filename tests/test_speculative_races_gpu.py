@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from test_speculative_gpu import BF16, F32, check, make, plain, run
+from test_speculative_gpu import BF16, F16, F32, check, make, plain, run
 
 pytestmark = pytest.mark.gpu
 
@@ -72,6 +72,56 @@ def run_tokens(c, **more):
         c["uniforms"].cuda() if c["drafts"].shape[1] else None, c["noise"].cuda(),
         draft_probs=None if c["probs"] is None else c["probs"].cuda(),
         temperature=c["heats"].cuda(), **more)
+
+
+@pytest.mark.parametrize("place", PLACES)
+@pytest.mark.parametrize("heat", [1e-8, 1e-9, 1e-20, 1e-36])
+def test_ties_at_the_lowest_temperatures(heat: float, place: str) -> None:
+    """The logits over the temperature have no room for their differences, or none at all."""
+    for dtype, V in ((BF16, 8192), (F32, 8195)):
+        c = _ties(150, V, dtype, place, True, seed=int(-math.log10(heat)) + 3)
+        c["heats"] = torch.full((150,), heat)
+        run(c)
+
+
+@pytest.mark.parametrize("heat", [1.0, 0.1, 1e-3])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("V", [1024, 1003])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_rows_of_one_value(dtype, V: int, given: bool, heat: float) -> None:
+    """The lowest value of a type stands for what is masked in many programs; where
+    a row has nothing else all of its tokens are equally likely, and so at the
+    highest. Behind the last draft, and in place of a refused one."""
+    info = torch.finfo(dtype)
+    for value in (info.min, info.max, 0.0, -5.0):
+        c = make(6, 1, V, dtype, seed=V, ragged=False, heats="one", probs=F32 if given else None)
+        c["src"][:] = value
+        c["heats"] = torch.full((6,), heat)
+        c["uniforms"] = torch.tensor([0.0, 0.0, 0.0, 1.0, 1.0, 1.0])[:, None] * (1 - 2.0**-24)
+        got, _ = run(c)
+        assert bool((got.counts >= 1).all())
+
+
+def test_rows_of_the_lowest_value_under_a_grammar() -> None:
+    from test_speculative_gpu import tables
+
+    V = 2000
+    fsa, tn = tables(6, V, seed=3)
+    states = torch.arange(12, dtype=torch.int32) % 6
+    for dtype in (F32, BF16):
+        c = make(12, 2, V, dtype, seed=5, heats="one")
+        c["src"][:] = torch.finfo(dtype).min
+        got, _ = run(c, fsa, tn, states)
+        assert bool((got.counts >= 1).all())
+
+
+def test_temperatures_that_take_the_logits_out_of_range() -> None:
+    for heat in (1e-37, 1e-38, 2.0**-140):
+        c = make(8, 1, 1024, F32, seed=1, ragged=False, heats="one")
+        c["src"][:] = torch.where(c["src"] > 4.0, 50.0, c["src"])
+        c["heats"] = torch.full((8,), heat)
+        got, _ = run(c)
+        assert bool((got.counts >= 1).all())
 
 
 def test_ties_are_decided_alike_each_time() -> None:
