@@ -145,3 +145,41 @@ def test_token_does_not_depend_on_its_place_in_the_batch() -> None:
         one = {**c, "src": c["src"][b:b + 1], "noise": c["noise"][b:b + 1],
                "drafts": c["drafts"][b:b + 1], "heats": c["heats"][b:b + 1]}
         assert torch.equal(run_tokens(one).tokens[0], whole.tokens[b])
+
+
+def _close(B: int, V: int, seed: int):
+    """Refused drafts whose probabilities are those of the target but for a thousandth,
+    and noise that makes what is left of all tokens nearly equal in the race."""
+    c = make(B, 1, V, F32, seed=seed, ragged=False, heats="one", probs=F32, scale=1.0)
+    g = torch.Generator().manual_seed(seed)
+    p = torch.softmax(c["src"][0::2].double(), -1)
+    gap = torch.rand(B, V, generator=g, dtype=torch.float64) * 2e-3 - 1e-3
+    c["probs"] = (p * (1 + gap)).float()
+    c["drafts"] = gap.argmax(1, keepdim=True)
+    c["uniforms"][:] = 1.0 - 2.0**-24
+    left = (p - c["probs"].double()).clamp(min=0)
+    jitter = 1 + 1e-4 * torch.rand(B, V, generator=g, dtype=torch.float64)
+    c["noise"] = torch.where(left > 0, left / left.max() * jitter, 1.0).float().clamp(min=1e-12)
+    return c, p, left
+
+
+def test_refused_drafts_of_nearly_the_targets_probability() -> None:
+    c, p, left = _close(40, 20000, seed=2)
+    got = run_tokens(c)
+    assert bool((got.counts == 1).all())
+    # p in fp32: an argument of up to 10 rounded once, an exponential, the sum and a quotient,
+    # 2^-20 of it together at most; the token is the best up to what that does to p - q
+    slop = p * 2.0**-20
+    noise = c["noise"].double()
+    sure = ((left - slop) / noise).max(1).values
+    mine = ((left + slop) / noise).gather(1, got.tokens[:, :1].cpu())[:, 0]
+    assert bool((mine >= sure).all())
+
+
+def test_refused_drafts_are_replaced_alike_each_time() -> None:
+    c, _, _ = _close(64, 32000, seed=9)
+    first = run_tokens(c)
+    for _ in range(40):
+        again = run_tokens(c)
+        assert torch.equal(first.tokens, again.tokens)
+        assert torch.equal(first.logprobs, again.logprobs)
