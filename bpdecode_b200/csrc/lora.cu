@@ -92,6 +92,7 @@ struct LoraArgs {
   int32_t row_tiles, out_tiles;
   int32_t parts;        // 16-bit values that make up one of S
   int32_t pair;         // CTAs that share the product's instructions: 1 or 2
+  int32_t fp32;         // whether the result is
 };
 
 __device__ __forceinline__ int32_t adapter_of(const LoraArgs& g, int32_t t) {
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 1)
   const int32_t most = kWideRanks / g.rank;  // adapters at a time
   const int32_t chunks = (adapters + most - 1) / most;
   // as the product, an fp32 result's sums of 512 inner elements at a time
-  const int32_t group = g.parts == 3 ? kGroup : steps;
+  const int32_t group = g.fp32 ? kGroup : steps;
   bool ok = true;
   if (warp == 0) {
     int32_t stage = 0, issued = 0;
@@ -1702,7 +1703,7 @@ extern "C" bpd_status bpd_lora_project(const void* x, int64_t x_stride, const vo
                    reinterpret_cast<int32_t*>(ws + w.count),
                    reinterpret_cast<uint2*>(ws + w.items), ws + w.low, nt, step, w.most_blocks,
                    row_tiles,
-                   out_tiles, parts, pair};
+                   out_tiles, parts, pair, fp32};
   cudaStream_t st = as_stream(stream);
   auto launch = [&](auto in, auto result) {
     return launch_project<decltype(in), decltype(result)>(maps, amap, xrows, g, st);
