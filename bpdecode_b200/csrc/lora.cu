@@ -29,8 +29,9 @@
 // are tensor copies, which alone may be counted in another CTA.
 //
 // S is held as the sum of 16-bit values, each the rounding of what those before
-// it left off: two of them keep 2^-17 of it in bf16 and 2^-22 in fp16 (one would
-// cost 2^-9 of the adapter's part), and an fp32 result has a third in bf16.
+// it left off: two of them keep 2^-17 of it in bf16 (one would cost 2^-9 of the
+// adapter's part), and an fp32 result has a third. In fp16 two keep 2^-22 of it,
+// but nothing below 2^-25, where fp16 ends: 2^-22 of S from 1/8 on.
 //
 // The matrix unit cuts its sums off to fp32 at every step, always towards zero:
 // 4.4e-6 of the result at 4096 inner elements, and growing with them. A 16-bit

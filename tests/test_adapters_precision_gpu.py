@@ -126,3 +126,47 @@ def test_an_fp32_results_adapters_do_not_drift(T: int, K: int, dtype: torch.dtyp
     for i in range(n):
         want = (x[ids == i].double() @ a[i].double().T)[:, j[i]]
         assert float(((got[ids == i].double() - want).abs() / want).max()) <= DRIFT
+
+
+@pytest.mark.parametrize("T", [9, 200, 700])
+@pytest.mark.parametrize("scaling", [1.0, 1e-3, 1e-5])
+def test_small_sums_in_fp16_keep_what_its_parts_can_hold(scaling: float, T: int) -> None:
+    """Two parts hold 2^-22 of S, and nothing below 2^-25."""
+    from bpdecode_b200.adapters import AdapterBank, project
+
+    K, N, rank = 512, 130, 16
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.rand(T, K, generator=g, device="cuda").half()
+    a = (torch.rand(rank, K, generator=g, device="cuda") / 256).half()
+    j = torch.randint(0, rank, (N,), generator=g, device="cuda")
+    b = torch.zeros(N, rank, device="cuda").scatter_(1, j[:, None], 1.0)
+    bank = AdapterBank(K, N, 1, rank, dtype=F16)
+    bank.load(0, a, b, scaling=scaling)
+    ids = torch.zeros(T, dtype=torch.int32, device="cuda")
+    got = project(x, torch.zeros(N, K, dtype=F16, device="cuda"), bank, ids, out_dtype=F32)
+    scale = float(torch.tensor(scaling, dtype=F32))
+    want = scale * (x.double() @ a.double().T)[:, j]
+    assert bool(((got.double() - want).abs() <= DRIFT * want + 2.0**-25).all())
+
+
+@pytest.mark.parametrize("T", [9, 200, 700])
+@pytest.mark.parametrize("out", [F16, F32])
+def test_sums_beyond_fp16_stay_in_their_rows(out: torch.dtype, T: int) -> None:
+    """S of 65504 and more is no fp16 number: such a row has no finite result where
+    its adapter's B is not zero, and no other row notices."""
+    from bpdecode_b200.adapters import AdapterBank, project
+
+    K, N, rank = 128, 130, 16
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.rand(T, K, generator=g, device="cuda").half()
+    w = torch.rand(N, K, generator=g, device="cuda").half()
+    bank = AdapterBank(K, N, 2, rank, dtype=F16)
+    for i in range(2):
+        bank.load(i, torch.rand(rank, K, generator=g, device="cuda"), torch.ones(N, rank))
+    ids = torch.arange(T, dtype=torch.int32, device="cuda") % 3 - 1
+    large = x.clone()
+    large[4] = 2048.0  # adapter 0: sums of about 130,000
+    clean, got = (project(t, w, bank, ids, out_dtype=out) for t in (x, large))
+    rest = torch.arange(T, device="cuda") != 4
+    assert torch.equal(got[rest], clean[rest])
+    assert not bool(torch.isfinite(got[4]).any())
