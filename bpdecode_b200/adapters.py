@@ -130,8 +130,11 @@ def project(
     (such as -1) none. The result [rows, out_features] is of ``x``'s type, or
     fp32 (``out_dtype``), rounded once from fp32 sums; ``out`` receives it
     (contiguous columns, any row stride). In fp16, ``scaling * A x`` must stay
-    below 65504. Launches on torch's current stream
-    without synchronising."""
+    below 65504, and what is below 2^-25 of it is lost. No autograd graph is
+    recorded, whether inputs require gradients or not. With a bank a call takes
+    a workspace from torch's allocator: up to ``256 * rank`` bytes for each row
+    (384 for fp32 results of bf16), less where the bank has fewer than 64 slots.
+    Launches on torch's current stream without synchronising."""
     _require_cuda(x, "x")
     dtype, dev = x.dtype, x.device
     if dtype not in _TYPES:

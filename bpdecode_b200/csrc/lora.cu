@@ -19,7 +19,7 @@
 // each; they need not be sorted. A matrix instruction over few rows costs
 // nearly what one over 128 costs (about 87 cycles at 16 rows), which is why
 // items are wide rather than exact: with 16-row items alone, 256 rows with 24
-// adapters took 226 us at 65,536 outputs, against 161 so.
+// adapters took 226 us at 65,536 outputs, against 161 so (154 in pairs, see below).
 //
 // Tiles of 256 rows are bound by what an SM loads, 48 KB for every 64 inner
 // elements. Two CTAs then work as a pair (cta_group::2): an instruction of the
@@ -38,6 +38,11 @@
 // result does not see that. An fp32 result is therefore accumulated 512 inner
 // elements at a time, and these sums are added up in registers (5e-7, as fp32
 // arithmetic has it).
+//
+// Times in these comments are of calls that follow one another on the same
+// operands, a few at a time: what fits in L2 is there, and clocks are high. With
+// caches flushed, or for seconds on end, they are larger (4096 rows by 4096 x 8192,
+// 8 adapters of rank 64: 207 us here, 242 in a long run).
 #include <cuda.h>
 
 #include <algorithm>
@@ -59,8 +64,8 @@ constexpr int kGroup = 8;           // steps that an fp32 result is accumulated 
 constexpr int kReach = 4;          // blocks that an item spans for each row that it has, at most
 // Tiles of rows up to which S is gathered row by row beside the product: with
 // more, products of all of a block's adapters in front of it take less (750 rows
-// by 4096 x 8192, 8 adapters of rank 64: 61 us, gathered 79; 24 of rank 16: 76,
-// 85; 4096 rows: 201, 217), with fewer, more (500 rows, 24 of rank 16: 66, 52).
+// by 4096 x 8192, 8 adapters of rank 64: 61 us, gathered 79; 4096 rows: 201, 217),
+// with fewer, more (500 rows, 24 of rank 16: 66, gathered 52).
 constexpr int kGatherTiles = 2;
 constexpr int kMaxSplit = 8;       // CTAs of a cluster that share one tile's inner elements
 constexpr int kThreads = 192;      // loads, products, four warps that write
@@ -1233,7 +1238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int32_t rc = shape >> 8, n = shape & 255;
             // One item after the other in a short loop: what this thread does between
-            // instructions shows (64 rows by 128,256 to fp32: 208 us, 217 with a
+            // instructions shows (64 rows by 128,256 to fp32: 205 us, 217 with a
             // branch for each half), and so does going from item to item for each
             // part (24 adapters of rank 64, 256 rows by 65,536: 226 us, 260 to 490).
             const int32_t halves = rc > 16 ? 2 : 1, count = g.parts * halves;

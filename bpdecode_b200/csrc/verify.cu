@@ -28,9 +28,11 @@
 //
 // All are bound by HBM; few requests by the loads that depend on one another
 // (state, allow bits, logits). What a thread finds best in a race is scored
-// again with full precision, so only scores within one thread are compared in
-// fast arithmetic. Nothing depends on the order in which CTAs run: chunks meet
-// in a fixed order, and a race takes the maximum of (score, lowest index).
+// again with full precision: in the race along with a scan only scores within one
+// thread are compared in fast arithmetic, in that of a refused draft none are.
+// Nothing depends on the order in which CTAs or warps run: chunks meet in a fixed
+// order, a race takes the maximum of (score, lowest index), and what its threads
+// share only leaves out tokens that cannot win.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
